@@ -5,6 +5,8 @@ Public surface (mirrors the reference's names):
 * ``verify_matmul``, ``is_enabled``                      (dflash_mlx/verify_qmm.py)
 * ``QuantizedLinear``, ``VerifyQuantizedLinear``, ``is_verify_eligible``,
   ``install_verify_linears``, ``prewarm_verify_kernels`` (dflash_mlx/verify_linear.py)
+* ``gated_delta_rule`` (whole prompts and single tokens), ``verify_accept_sampled``
+  (sampled acceptance of drafts), ``route_experts`` / ``Router`` (expert routing)
 * ``tape_replay_kernel`` (dflash_mlx/kernels.py), ``RecurrentRollbackCache``
   (dflash_mlx/recurrent_rollback_cache.py), ``restore_after_acceptance``
   (dflash_mlx/engine/target_qwen_gdn.py)
@@ -14,10 +16,12 @@ its C ABI (``include/dflash_b200.h``); there is no CPU fallback.
 """
 
 from . import checkpoint, kernels, lm_head, moe, qmm_plan
-from .lm_head import lm_head_argmax_keys, lm_head_verify, match_acceptance_length, verify_accept
-from .kernels import (gated_delta_kernel_with_tape, gated_delta_tree_kernel,
+from .lm_head import (lm_head_argmax_keys, lm_head_verify, match_acceptance_length, verify_accept,
+                      verify_accept_sampled)
+from .kernels import (gated_delta_kernel_with_tape, gated_delta_rule, gated_delta_tree_kernel,
                       gated_delta_tree_tape_kernel, tape_replay_, tape_replay_kernel,
                       tree_depthwise_conv1d)
+from .moe import Router, route_experts
 from .recurrent_rollback_cache import (
     RecurrentRollbackCache,
     arm_rollback,
@@ -37,6 +41,10 @@ from .verify_linear import (
 )
 
 __all__ = [
+    "Router",
+    "gated_delta_rule",
+    "route_experts",
+    "verify_accept_sampled",
     "gated_delta_tree_kernel",
     "gated_delta_tree_tape_kernel",
     "tree_depthwise_conv1d",

@@ -58,6 +58,17 @@ SIGNATURES = {
                                      _c_int, _c_int, _c_int, _c_int, _c_int, _vp]),
     "dfl_gdn_forward_tape": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _vp, _vp, _vp, _vp, _vp, _vp,
                                       _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _vp]),
+    "dfl_gdn_rule_recurrent": (_c_int, [_vp, _c_int, _vp, _c_int, _vp, _c_int, _vp, _c_int, _vp, _vp, _vp,
+                                        _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                        _c_int, _vp]),
+    "dfl_verify_sampled_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int,
+                                                     ctypes.POINTER(_c_int)]),
+    "dfl_verify_accept_sampled": (_c_int, [_vp, _vp, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                           _c_size, _c_size, _c_size, _c_size, _c_int, _c_int, _c_int, _vp,
+                                           _c_size, _vp]),
+    "dfl_moe_route_experts": (_c_int, [_vp, _c_int, _c_size, _vp, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                       _c_int, ctypes.c_float, _vp, _vp, _vp]),
+    "dfl_moe_route_table": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _vp]),
     "dfl_lmhead_argmax": (_c_int, [_vp, _vp, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp,
                                    _c_size, _vp]),
     "dfl_lmhead_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, ctypes.POINTER(_c_int)]),

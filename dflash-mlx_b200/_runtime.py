@@ -66,6 +66,25 @@ def require_cuda(t: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name} must be a CUDA tensor (dflash-b200 has no CPU path)")
 
 
+def same_device(dev: torch.device, **tensors) -> None:
+    """Every given tensor (None: left out) is a CUDA tensor on ``dev``."""
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        require_cuda(t, name)
+        if t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, not on {dev}")
+
+
+def mask_bytes(mask: torch.Tensor, name: str) -> torch.Tensor:
+    """A bool or uint8 mask as contiguous uint8 (bool storage is read as it is)."""
+    if mask.dtype == torch.bool:
+        return mask.contiguous().view(torch.uint8)
+    if mask.dtype == torch.uint8:
+        return mask.contiguous()
+    raise ValueError(f"{name} must be bool or uint8, got {mask.dtype}")
+
+
 def as_u32_bits(w: torch.Tensor) -> torch.Tensor:
     """Packed weights as a contiguous 32-bit tensor (int32 or uint32 storage)."""
     if w.dtype not in (torch.int32, torch.uint32):

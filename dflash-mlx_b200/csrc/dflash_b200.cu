@@ -9,9 +9,12 @@
 #include "qmm_plan.cu"
 #include "gdn_replay.cu"
 #include "gdn_forward.cu"
+#include "gdn_rule.cu"
 #include "gdn_tree.cu"
 #include "lmhead.cu"
+#include "sampled.cu"
 #include "moe.cu"
+#include "route.cu"
 
 extern "C" const char* dfl_status_string(int status) {
   switch (status) {

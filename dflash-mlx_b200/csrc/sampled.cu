@@ -1,0 +1,575 @@
+// Verification of drafted tokens against the target's probabilities (sm_100a).
+//
+// For request b with temperature z, drafts x_1 .. x_n (n = draft_lens[b]), row i
+// of the target's logits after the i-th token of the block and, where the draft
+// model's logits are given, row i of those for the draft x_{i+1}:
+//     p_i = softmax(logits_i / z) without the suppressed ids,
+//     q_i = softmax(draft_i / z), or all on x_{i+1} (greedy drafts),
+//     draft i is accepted while u_i q_i(x_{i+1}) < p_i(x_{i+1});  a = accepted,
+//     next token ~ max(p_a - q_a, 0) when a < n, else ~ p_n, by inverse
+//     cumulative sum in id order: the first id whose sum exceeds sample_u x total.
+// The committed tokens are then distributed as samples of the target alone.
+// z = 0 (or below, or NaN) is greedy: p_i is all on the largest logit's id.
+//
+// Three launches.  rows_kernel reads every row once (the one pass that is bound
+// by HBM): maximum, its id and sum of exponentials of each segment, in 32 bits.
+// decide_kernel joins a request's segments, accepts, and, where the next token
+// comes from a difference of two softmaxes, adds the two rows' exponentials
+// again in 64 bits.  pick_kernel adds the weights of that one row's segments in
+// 64 bits, and the last CTA of a request finds the segment and the id.  The 64
+// bits are for the id: with 2^18 ids a weight is 2^-18 of the total, and a sum
+// in 32 bits would move a border by a sizeable part of it.
+//
+// A logit that is NaN or -inf has probability 0; rows with +inf spread over
+// those ids.  A row that has nothing left gives token -1.
+//
+// Replaces, for sampled decoding, the greedy tail of dflash_mlx/engine/
+// spec_epoch.py:2067-2072,2129 (greedy_tokens_with_mask engine/sampling.py:47-55
+// and match_acceptance_length engine/acceptance.py:9-16).
+
+namespace dfl {
+namespace smp {
+
+constexpr int THREADS = 256;
+constexpr int WARPS = THREADS / 32;
+constexpr int MAX_BLOCK = 256;    // tokens of a block
+constexpr int PICK_SEG = 4096;    // ids of a segment of the picked row
+
+struct Params {
+  const void* logits;    // [B, T] rows of V
+  const void* draft;     // [B, T - 1] rows of V, or null
+  const int32_t* ids;    // [B, T]
+  const float* accept_u; // [B, T - 1]
+  const float* sample_u; // [B]
+  const float* temperature;  // [B]
+  const int32_t* lens;   // [B] or null
+  const uint8_t* suppress;   // [V] or null
+  int32_t* accepted;     // [B]
+  int32_t* token;        // [B]
+  float* draft_prob;     // [B, T - 1]
+  long long ld, ldd;     // elements from one row to the next
+  long long bs, bsd;     // elements from one request to the next
+  int B, T, V;
+  int segs, seg;         // segments of a row and their length (rows_kernel)
+  int psegs;             // segments of PICK_SEG ids (decide_kernel, pick_kernel)
+  // workspace
+  float2* part;          // [B * T + B * (T - 1)][segs] (maximum, sum)
+  int* part_id;          // [B * T][segs] lowest id of the maximum
+  double* zsum;          // [2][B][psegs]
+  double* wsum;          // [2][B][psegs]
+  int* sel;              // [B] accepted
+  int* ticket;           // [B]
+};
+
+template <typename T>
+__device__ __forceinline__ float to_f(T x);
+template <>
+__device__ __forceinline__ float to_f<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_f<__half>(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// 0 for greedy, else the temperature kept where 1 / z and FLT_MAX / z are finite.
+__device__ __forceinline__ float clean_temperature(float z) {
+  return z > 0.f ? fminf(fmaxf(z, 1e-30f), 1e30f) : 0.f;
+}
+
+__device__ __forceinline__ int draft_len(const Params& p, int b) {
+  if (!p.lens) return p.T - 1;
+  const int n = p.lens[b];
+  const int c = min(max(n, 0), p.T - 1);
+  if (c != n && threadIdx.x == 0) atomicExch(&g_device_error, kDevBadInput);
+  return c;
+}
+
+template <typename T>
+__device__ __forceinline__ const T* target_row(const Params& p, int b, int i) {
+  return reinterpret_cast<const T*>(p.logits) + ((size_t)b * p.bs + (size_t)i * p.ld);
+}
+
+template <typename T>
+__device__ __forceinline__ const T* draft_row(const Params& p, int b, int i) {
+  return reinterpret_cast<const T*>(p.draft) + ((size_t)b * p.bsd + (size_t)i * p.ldd);
+}
+
+// (maximum, lowest id of it, sum of exp((x - maximum) / z)) of some ids; an
+// empty set is (-inf, INT_MAX, 0).
+struct Stat {
+  float m, s;
+  int id;
+};
+
+__device__ __forceinline__ float exp_scaled(float d, float c) {
+  // d <= 0; NaN (a NaN logit) and -inf become -FLT_MAX: exp gives 0
+  return exp2f(fmaxf(d, -FLT_MAX) * c);
+}
+
+__device__ __forceinline__ Stat join(const Stat& a, const Stat& b, float c) {
+  Stat r;
+  r.m = fmaxf(a.m, b.m);
+  r.id = a.m > b.m ? a.id : (b.m > a.m ? b.id : min(a.id, b.id));
+  // a part that holds the maximum keeps its sum; the other one is scaled (equal
+  // infinities would give NaN as a difference)
+  r.s = (a.m == r.m ? a.s : a.s * exp_scaled(a.m - r.m, c)) + (b.m == r.m ? b.s : b.s * exp_scaled(b.m - r.m, c));
+  return r;
+}
+
+__device__ __forceinline__ Stat warp_join(Stat a, float c) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Stat b;
+    b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
+    b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
+    b.id = __shfl_xor_sync(0xffffffffu, a.id, o);
+    a = join(a, b, c);
+  }
+  return a;
+}
+
+template <typename T>
+__device__ __forceinline__ void take(Stat& a, float x, int id, float c) {
+  if (x > a.m) {
+    a.s = a.m == -INFINITY ? 0.f : (x == INFINITY ? 0.f : a.s * exp_scaled(a.m - x, c));
+    a.m = x;
+    a.id = id;
+  }
+  // at +inf only the ids that hold it count (inf - inf is NaN: 0)
+  a.s += x == INFINITY ? 1.f : exp_scaled(x - a.m, c);
+}
+
+// Segment blockIdx.x of row blockIdx.y (target rows, then draft rows).
+template <typename T>
+__global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
+  __shared__ Stat sh[WARPS];
+  const int row = blockIdx.y;
+  const bool is_draft = row >= p.B * p.T;
+  const int r = is_draft ? row - p.B * p.T : row;
+  const int per = is_draft ? p.T - 1 : p.T;
+  const int b = r / per, i = r - b * per;
+  const int n = draft_len(p, b);
+  if (row == 0 && blockIdx.x == 0)
+    for (int x = threadIdx.x; x < p.B; x += THREADS) p.ticket[x] = 0;
+  if (is_draft ? i >= n : i > n) return;  // a row of no draft
+  const float z = clean_temperature(p.temperature[b]);
+  if (is_draft && z == 0.f) return;
+  const float c = z == 0.f ? 1.f : 1.44269504f / z;
+  const T* x = is_draft ? draft_row<T>(p, b, i) : target_row<T>(p, b, i);
+  const uint8_t* sup = is_draft ? nullptr : p.suppress;
+  const int v0 = blockIdx.x * p.seg, v1 = min(p.V, v0 + p.seg);
+  Stat a{-INFINITY, 0.f, 0x7fffffff};
+  for (int v = v0 + threadIdx.x; v < v1; v += THREADS) {
+    float f = to_f<T>(x[v]);
+    if (sup && sup[v]) f = -INFINITY;
+    take<T>(a, f, v, c);
+  }
+  a = warp_join(a, c);
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = a;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    a = threadIdx.x < WARPS ? sh[threadIdx.x] : Stat{-INFINITY, 0.f, 0x7fffffff};
+    a = warp_join(a, c);
+    if (threadIdx.x == 0) {
+      p.part[(size_t)row * p.segs + blockIdx.x] = make_float2(a.m, a.s);
+      if (!is_draft) p.part_id[(size_t)row * p.segs + blockIdx.x] = a.id;
+    }
+  }
+}
+
+// The whole row's statistics from its segments, in every lane of the warp;
+// the sum of exponentials relative to the maximum in 64 bits.
+__device__ __forceinline__ void row_stat(const Params& p, int row, bool with_id, float c, float* m, double* s,
+                                         int* id) {
+  const int lane = threadIdx.x & 31;
+  float mx = -INFINITY;
+  int at = 0x7fffffff;
+  for (int g = lane; g < p.segs; g += 32) {
+    const float x = p.part[(size_t)row * p.segs + g].x;
+    if (x > mx) {
+      mx = x;
+      at = with_id ? p.part_id[(size_t)row * p.segs + g] : 0;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float om = __shfl_xor_sync(0xffffffffu, mx, o);
+    const int oa = __shfl_xor_sync(0xffffffffu, at, o);
+    if (om > mx || (om == mx && oa < at)) {
+      mx = om;
+      at = oa;
+    }
+  }
+  double sum = 0.0;
+  for (int g = lane; g < p.segs; g += 32) {
+    const float2 x = p.part[(size_t)row * p.segs + g];
+    sum += x.x == mx ? (double)x.y : (double)x.y * (double)exp_scaled(x.x - mx, c);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  *m = mx;
+  *s = sum;
+  *id = at;
+}
+
+// exp((x - m) / z) in 64 bits; 0 for NaN and -inf, 1 for +inf under a +inf maximum.
+__device__ __forceinline__ double weight(float x, float m, double inv_z) {
+  if (x == m) return 1.0;
+  const double d = (double)x - (double)m;
+  return d < 0.0 ? exp(d * inv_z) : 0.0;   // NaN compares false; -inf gives exp(-inf) = 0
+}
+
+__device__ __forceinline__ double block_sum(double x, double* sh) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = x;
+  __syncthreads();
+  double r = 0.0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) r += sh[w];
+  return r;
+}
+
+// Accept (every CTA of a request alike; CTA 0 writes), then the 64-bit sums of
+// segment blockIdx.x of the rows that the next token is drawn from.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) decide_kernel(const Params p) {
+  __shared__ int first_bad;
+  __shared__ double sh[WARPS];
+  const int b = blockIdx.y;
+  const int n = draft_len(p, b);
+  const float z = clean_temperature(p.temperature[b]);
+  const float c = z == 0.f ? 1.f : 1.44269504f / z;
+  const double inv_z = z == 0.f ? 0.0 : 1.0 / (double)z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) first_bad = n;
+  __syncthreads();
+  for (int i = warp; i < p.T - 1; i += WARPS) {
+    double px = 0.0, qx = 1.0;
+    if (i < n) {
+      const int x = p.ids[(size_t)b * p.T + i + 1];
+      const bool in = x >= 0 && x < p.V;
+      float m;
+      double s;
+      int id;
+      row_stat(p, b * p.T + i, true, c, &m, &s, &id);
+      const bool open = in && !(p.suppress && p.suppress[x]);
+      const float lx = open ? to_f<T>(target_row<T>(p, b, i)[x]) : -INFINITY;
+      if (m > -INFINITY && open) px = z == 0.f ? (x == id ? 1.0 : 0.0) : weight(lx, m, inv_z) / s;
+      if (p.draft && z != 0.f) {
+        row_stat(p, p.B * p.T + b * (p.T - 1) + i, false, c, &m, &s, &id);
+        const float dx = in ? to_f<T>(draft_row<T>(p, b, i)[x]) : -INFINITY;
+        qx = m > -INFINITY && in ? weight(dx, m, inv_z) / s : 0.0;
+      }
+      if (lane == 0) {
+        const double u = p.accept_u[(size_t)b * (p.T - 1) + i];
+        if (!(u * qx < px)) atomicMin(&first_bad, i);
+      }
+    }
+    if (lane == 0 && blockIdx.x == 0) p.draft_prob[(size_t)b * (p.T - 1) + i] = float(px);
+  }
+  __syncthreads();
+  const int a = first_bad;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    p.accepted[b] = a;
+    p.sel[b] = a;
+  }
+  if (!(p.draft && a < n && z != 0.f)) return;
+  // normalisers of p_a and q_a
+  const int v0 = blockIdx.x * PICK_SEG, v1 = min(p.V, v0 + PICK_SEG);
+  float mp, mq;
+  double s;
+  int id;
+  row_stat(p, b * p.T + a, false, c, &mp, &s, &id);
+  row_stat(p, p.B * p.T + b * (p.T - 1) + a, false, c, &mq, &s, &id);
+  const T* lp = target_row<T>(p, b, a);
+  const T* lq = draft_row<T>(p, b, a);
+  double sp = 0.0, sq = 0.0;
+  for (int v = v0 + threadIdx.x; v < v1; v += THREADS) {
+    if (!(p.suppress && p.suppress[v])) sp += mp > -INFINITY ? weight(to_f<T>(lp[v]), mp, inv_z) : 0.0;
+    sq += mq > -INFINITY ? weight(to_f<T>(lq[v]), mq, inv_z) : 0.0;
+  }
+  sp = block_sum(sp, sh);
+  sq = block_sum(sq, sh);
+  if (threadIdx.x == 0) {
+    p.zsum[(size_t)b * p.psegs + blockIdx.x] = sp;
+    p.zsum[(size_t)(p.B + b) * p.psegs + blockIdx.x] = sq;
+  }
+}
+
+// What pick_kernel draws from: the target's row, the draft's row and id.
+template <typename T>
+struct Pick {
+  const T* lp;
+  const T* lq;     // null: no draft row to take away
+  const uint8_t* sup;
+  float mp, mq;
+  double inv_z, ip, iq;  // 1 / z, 1 / sums
+  int hot;         // id that a greedy draft takes away whole, or -1
+  // weights of id v: left after the draft, and the target's own
+  __device__ __forceinline__ void at(int v, double* left, double* whole) const {
+    double w = 0.0;
+    // the two products rounded alike, not fused into the difference: equal rows leave exactly 0
+    if (mp > -INFINITY && !(sup && sup[v])) w = __dmul_rn(weight(to_f<T>(lp[v]), mp, inv_z), ip);
+    *whole = w;
+    double l = v == hot ? 0.0 : w;
+    if (lq && mq > -INFINITY)
+      l = fmax(w - __dmul_rn(weight(to_f<T>(lq[v]), mq, inv_z), iq), 0.0);
+    *left = l;
+  }
+};
+
+__device__ __forceinline__ double fixed_sum(const double* x, int n, double* sh) {
+  double t = 0.0;
+  for (int g = threadIdx.x; g < n; g += THREADS) t += x[g];
+  return block_sum(t, sh);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS) pick_kernel(const Params p) {
+  __shared__ double sh[WARPS];
+  __shared__ int last;
+  __shared__ int found_seg, found_id, any_id;
+  __shared__ double before;
+  const int b = blockIdx.y;
+  const int n = draft_len(p, b);
+  const float z = clean_temperature(p.temperature[b]);
+  const float c = z == 0.f ? 1.f : 1.44269504f / z;
+  const int a = p.sel[b];
+  float m;
+  double s;
+  int id;
+  row_stat(p, b * p.T + a, true, c, &m, &s, &id);
+  if (z == 0.f) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.token[b] = m > -INFINITY ? id : -1;
+    return;
+  }
+  Pick<T> k;
+  k.lp = target_row<T>(p, b, a);
+  k.lq = nullptr;
+  k.sup = p.suppress;
+  k.mp = m;
+  k.mq = -INFINITY;
+  k.inv_z = 1.0 / (double)z;
+  k.ip = k.iq = 1.0;
+  k.hot = -1;
+  if (a < n) {
+    if (p.draft) {
+      k.lq = draft_row<T>(p, b, a);
+      row_stat(p, p.B * p.T + b * (p.T - 1) + a, false, c, &k.mq, &s, &id);
+      const double sp = fixed_sum(p.zsum + (size_t)b * p.psegs, p.psegs, sh);
+      const double sq = fixed_sum(p.zsum + (size_t)(p.B + b) * p.psegs, p.psegs, sh);
+      k.ip = sp > 0.0 ? 1.0 / sp : 0.0;
+      k.iq = sq > 0.0 ? 1.0 / sq : 0.0;
+    } else {
+      k.hot = p.ids[(size_t)b * p.T + a + 1];
+    }
+  }
+  const int v0 = blockIdx.x * PICK_SEG, v1 = min(p.V, v0 + PICK_SEG);
+  double left = 0.0, whole = 0.0;
+  for (int v = v0 + threadIdx.x; v < v1; v += THREADS) {
+    double l, w;
+    k.at(v, &l, &w);
+    left += l;
+    whole += w;
+  }
+  left = block_sum(left, sh);
+  whole = block_sum(whole, sh);
+  if (threadIdx.x == 0) {
+    p.wsum[(size_t)b * p.psegs + blockIdx.x] = left;
+    p.wsum[(size_t)(p.B + b) * p.psegs + blockIdx.x] = whole;
+    __threadfence();
+    last = atomicAdd(&p.ticket[b], 1) == int(gridDim.x) - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  // The last CTA of the request: total, the segment that the border falls in,
+  // then the id inside it.  Which CTA this is changes no sum.
+  double total = fixed_sum(p.wsum + (size_t)b * p.psegs, p.psegs, sh);
+  const bool use_left = total > 0.0;   // nothing left after the draft: the target's own weights
+  const double* ws = p.wsum + (size_t)(use_left ? b : p.B + b) * p.psegs;
+  if (!use_left) total = fixed_sum(ws, p.psegs, sh);
+  if (!(total > 0.0)) {
+    if (threadIdx.x == 0) p.token[b] = -1;
+    return;
+  }
+  if (threadIdx.x == 0) {
+    float u = p.sample_u[b];
+    u = u > 0.f ? u : 0.f;
+    const double border = (double)u * total;
+    double run = 0.0, at = 0.0;
+    int g = -1;
+    for (int x = 0; x < p.psegs; ++x) {
+      if (!(ws[x] > 0.0)) continue;
+      g = x;       // the last segment that has any, should the sums round below the border
+      at = run;
+      run += ws[x];
+      if (run > border) break;
+    }
+    found_seg = g;
+    before = border - at;
+    found_id = 0x7fffffff;
+    any_id = -1;
+  }
+  __syncthreads();
+  // ids of the segment: each thread a contiguous piece, exclusive sums of the pieces in order
+  constexpr int PER = PICK_SEG / THREADS;
+  const int w0 = found_seg * PICK_SEG + threadIdx.x * PER;
+  double mine = 0.0, piece[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    double l = 0.0, w = 0.0;
+    if (w0 + j < p.V) k.at(w0 + j, &l, &w);
+    piece[j] = use_left ? l : w;
+    mine += piece[j];
+  }
+  __shared__ double pre[THREADS];
+  pre[threadIdx.x] = mine;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double run = 0.0;
+    for (int t = 0; t < THREADS; ++t) {
+      const double x = pre[t];
+      pre[t] = run;
+      run += x;
+    }
+  }
+  __syncthreads();
+  double run = pre[threadIdx.x];
+  int hit = 0x7fffffff, any = -1;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    run += piece[j];
+    if (piece[j] > 0.0) {
+      any = w0 + j;
+      if (run > before && hit == 0x7fffffff) hit = w0 + j;
+    }
+  }
+  if (hit != 0x7fffffff) atomicMin(&found_id, hit);
+  if (any >= 0) atomicMax(&any_id, any);
+  __syncthreads();
+  if (threadIdx.x == 0) p.token[b] = found_id != 0x7fffffff ? found_id : any_id;
+}
+
+// Segment length of rows_kernel: long enough that a CTA's start-up is small
+// beside its loads, short enough that a few rows still fill the card.
+inline void geometry(int B, int T, int V, bool draft, int sms, int* seg, int* segs, int* psegs) {
+  const long long rows = (long long)B * T + (draft ? (long long)B * (T - 1) : 0);
+  int s = 32768;
+  while (s > 4096 && rows * ((V + s - 1) / s) < 8ll * sms) s /= 2;
+  *seg = s;
+  *segs = (V + s - 1) / s;
+  *psegs = (V + PICK_SEG - 1) / PICK_SEG;
+}
+
+inline size_t round16(size_t x) { return (x + 15) & ~size_t(15); }
+
+inline size_t layout(Params* p, uint8_t* base) {
+  const size_t rows = (size_t)p->B * p->T + (p->draft ? (size_t)p->B * (p->T - 1) : 0);
+  size_t at = 0;
+  auto put = [&](size_t bytes) {
+    uint8_t* r = base + at;
+    at += round16(bytes);
+    return r;
+  };
+  p->part = reinterpret_cast<float2*>(put(rows * p->segs * sizeof(float2)));
+  p->zsum = reinterpret_cast<double*>(put((size_t)2 * p->B * p->psegs * sizeof(double)));
+  p->wsum = reinterpret_cast<double*>(put((size_t)2 * p->B * p->psegs * sizeof(double)));
+  p->part_id = reinterpret_cast<int*>(put((size_t)p->B * p->T * p->segs * sizeof(int)));
+  p->sel = reinterpret_cast<int*>(put((size_t)p->B * sizeof(int)));
+  p->ticket = reinterpret_cast<int*>(put((size_t)p->B * sizeof(int)));
+  return at;
+}
+
+template <typename T>
+int launch(const Params& p, cudaStream_t stream) {
+  const int rows = p.B * p.T + (p.draft ? p.B * (p.T - 1) : 0);
+  rows_kernel<T><<<dim3(p.segs, rows), THREADS, 0, stream>>>(p);
+  int st = host::launch_status();
+  if (st != DFL_OK) return st;
+  decide_kernel<T><<<dim3(p.psegs, p.B), THREADS, 0, stream>>>(p);
+  st = host::launch_status();
+  if (st != DFL_OK) return st;
+  pick_kernel<T><<<dim3(p.psegs, p.B), THREADS, 0, stream>>>(p);
+  return host::launch_status();
+}
+
+// rows <= 65535: the grid's y dimension
+inline bool sizes_ok(int B, int T, int V, bool draft) {
+  if (B < 0 || T < 1 || T > MAX_BLOCK || V < 1 || V > (1 << 24)) return false;
+  return (long long)B * T + (draft ? (long long)B * (T - 1) : 0) <= 65535;
+}
+
+}  // namespace smp
+}  // namespace dfl
+
+extern "C" size_t dfl_verify_sampled_workspace_bytes(int B, int T, int V, int with_draft, int* status) {
+  using namespace dfl;
+  int dummy;
+  int* st = status ? status : &dummy;
+  if (!smp::sizes_ok(B, T, V, with_draft != 0)) {
+    *st = DFL_ERR_BAD_SHAPE;
+    return 0;
+  }
+  int dev, sms;
+  *st = host::current_device(&dev, &sms);
+  if (*st != DFL_OK) return 0;
+  smp::Params p;
+  p.B = B;
+  p.T = T;
+  p.V = V;
+  p.draft = with_draft ? &p : nullptr;
+  smp::geometry(B, T, V, with_draft != 0, sms, &p.seg, &p.segs, &p.psegs);
+  return smp::layout(&p, nullptr);
+}
+
+extern "C" int dfl_verify_accept_sampled(const void* logits, const void* draft_logits, int dtype,
+                                         const int32_t* verify_ids, const float* accept_u,
+                                         const float* sample_u, const float* temperature,
+                                         const int32_t* draft_lens, const uint8_t* suppress, int32_t* acceptance,
+                                         int32_t* next_token, float* draft_prob, size_t ld_logits, size_t bs_logits,
+                                         size_t ld_draft, size_t bs_draft, int B, int T, int V,
+                                         void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace dfl;
+  if (!smp::sizes_ok(B, T, V, draft_logits != nullptr)) return DFL_ERR_BAD_SHAPE;
+  if (dtype < 0 || dtype > 2) return DFL_ERR_UNSUPPORTED;
+  const size_t far = (size_t)1 << 40;
+  if (ld_logits > far || bs_logits > far || ld_draft > far || bs_draft > far) return DFL_ERR_BAD_SHAPE;
+  if (B == 0) return DFL_OK;
+  if (!logits || !sample_u || !temperature || !acceptance || !next_token) return DFL_ERR_NULL_POINTER;
+  if (T > 1 && (!verify_ids || !accept_u || !draft_prob)) return DFL_ERR_NULL_POINTER;
+  const uintptr_t esz = dtype == 2 ? 4 : 2;
+  if (!host::aligned(logits, esz) || !host::aligned(draft_logits, esz)) return DFL_ERR_MISALIGNED;
+  int dev, sms;
+  const int st = host::current_device(&dev, &sms);
+  if (st != DFL_OK) return st;
+  smp::Params p;
+  p.logits = logits;
+  p.draft = draft_logits;
+  p.ids = verify_ids;
+  p.accept_u = accept_u;
+  p.sample_u = sample_u;
+  p.temperature = temperature;
+  p.lens = draft_lens;
+  p.suppress = suppress;
+  p.accepted = acceptance;
+  p.token = next_token;
+  p.draft_prob = draft_prob;
+  p.ld = (long long)ld_logits;
+  p.ldd = (long long)ld_draft;
+  p.bs = (long long)bs_logits;
+  p.bsd = (long long)bs_draft;
+  p.B = B;
+  p.T = T;
+  p.V = V;
+  smp::geometry(B, T, V, draft_logits != nullptr, sms, &p.seg, &p.segs, &p.psegs);
+  if (!workspace || !host::aligned(workspace, 16)) return workspace ? DFL_ERR_MISALIGNED : DFL_ERR_WORKSPACE;
+  if (workspace_bytes < smp::layout(&p, reinterpret_cast<uint8_t*>(workspace))) return DFL_ERR_WORKSPACE;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case 0: return smp::launch<__nv_bfloat16>(p, s);
+    case 1: return smp::launch<__half>(p, s);
+    default: return smp::launch<float>(p, s);
+  }
+}

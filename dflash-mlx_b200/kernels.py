@@ -16,6 +16,11 @@ Mirrors ``dflash_mlx/kernels.py``:
 * ``tape_replay_(state, tape, k, g, steps)`` -- the in-place form the
   rollback uses on B200: replays the first ``steps[b]`` steps of each
   sequence and does not touch sequences with nothing to replay.
+* ``gated_delta_rule(q, k, v, g, beta, state, ...)`` -- the same recurrence
+  without a tape, for prompts of any length (padded with a mask, or packed
+  with ``cu_seqlens``) and for single tokens; the reference runs it through
+  mlx-lm's ``gated_delta_update`` for caches that are not armed
+  (``engine/target_qwen_gdn.py:551-651``).
 
 The update per replayed step is ``S <- S * g_t`` then ``S <- S + delta_t k_t``,
 two separately rounded fp32 operations in the order of the mx-op reference
@@ -31,7 +36,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._runtime import require_cuda, stream_ptr
+from ._runtime import mask_bytes, require_cuda, same_device, stream_ptr
 
 
 def _check(tape, k, g, state, steps=None, mask=None):
@@ -152,6 +157,121 @@ def gated_delta_kernel_with_tape(q: torch.Tensor, k: torch.Tensor, v: torch.Tens
             tape.data_ptr(), b, t_steps, hv, hk, dv, dk, stream_ptr(state.device))
     _lib.check("dfl_gdn_forward_tape", st)
     return y, out, tape
+
+
+# ------------------------------------------------- whole sequences, no tape
+def _token_rows(x: torch.Tensor):
+    """``x [B, T, H, D]`` as tokens one fixed stride apart: ``(tensor, stride)``.
+    Views of a wider projection (heads and values next to each other, tokens
+    further apart) are read in place when their rows are 16-byte aligned;
+    everything else is copied."""
+    b, t, h, d = x.shape
+    step = x.stride(1) if t > 1 else (x.stride(0) if b > 1 else h * d)
+    fits = ((d == 1 or x.stride(3) == 1) and (h == 1 or x.stride(2) == d) and step >= h * d
+            and (b == 1 or t == 1 or x.stride(0) == t * step) and step % 8 == 0 and step < 2**31
+            and x.data_ptr() % 16 == 0)
+    return (x, step) if fits else (x.contiguous(), h * d)
+
+
+def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor,
+                     beta: torch.Tensor, state: torch.Tensor, *, mask: Optional[torch.Tensor] = None,
+                     cu_seqlens: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                     out_state: Optional[torch.Tensor] = None):
+    """The gated delta rule over whole sequences: ``(y, new_state)``.
+
+    ``q, k [B, T, Hk, Dk]`` and ``v [B, T, Hv, Dv]`` bf16 (views of a wider
+    projection output are read in place), ``g [B, T, Hv]`` or ``[B, T, Hv,
+    Dk]`` and ``beta [B, T, Hv]`` fp32; ``y`` bf16 ``[B, T, Hv, Dv]``.
+
+    * Padded batch: ``state`` fp32 ``[B, Hv, Dv, Dk]``, optional bool ``mask
+      [B, T]``; a step whose mask is False leaves the state, its ``y`` is 0 and
+      what its inputs hold does not matter.
+    * Packed: ``B = 1`` and ``cu_seqlens`` int32 ``[N + 1]`` on the device;
+      sequence n is tokens ``cu_seqlens[n] .. cu_seqlens[n + 1] - 1`` (lengths
+      of 0 and 1 included) and starts from ``state[n]``, ``[N, Hv, Dv, Dk]``.
+
+    ``out`` receives y (rows that belong to no sequence are left as they were;
+    a new y has zeros there).  ``out_state`` receives the new state and may be
+    ``state`` itself; without it ``state`` is left untouched.  Nothing is read
+    back to the host; the call can be captured into a CUDA graph.
+    """
+    require_cuda(state, "state")
+    dev = state.device
+    same_device(dev, q=q, k=k, v=v, g=g, beta=beta, mask=mask, cu_seqlens=cu_seqlens, out=out,
+                out_state=out_state)
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        if t.dtype != torch.bfloat16:
+            raise NotImplementedError(f"{name} must be bfloat16, got {t.dtype}")
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be [B, T, heads, dim], got {tuple(t.shape)}")
+    if g.dtype != torch.float32 or beta.dtype != torch.float32:
+        raise NotImplementedError("g and beta must be float32")
+    if state.dtype != torch.float32:
+        raise NotImplementedError(f"state must be float32, got {state.dtype}")
+    b, t_steps, hk, dk = k.shape
+    hv, dv = v.shape[2:]
+    if q.shape != k.shape:
+        raise ValueError("q and k must have the same shape")
+    if hk < 1 or hv < 1 or hv % hk != 0:
+        raise ValueError(f"Cannot align K heads {hk} to V heads {hv}")
+    if dk not in (32, 64, 128, 256) or dv < 32 or dv % 32 != 0:
+        raise ValueError(f"Dk must be 32, 64, 128 or 256 and Dv a multiple of 32, got {dk} and {dv}")
+    if v.shape[:2] != (b, t_steps) or beta.shape != (b, t_steps, hv):
+        raise ValueError("v must be [B, T, Hv, Dv] and beta [B, T, Hv]")
+    if g.shape not in ((b, t_steps, hv), (b, t_steps, hv, dk)):
+        raise ValueError(f"Unsupported gating shape {tuple(g.shape)}")
+    seqs = b
+    if cu_seqlens is not None:
+        if b != 1:
+            raise ValueError(f"packed sequences take B = 1, got {b}")
+        if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+            raise ValueError("cu_seqlens must be int32 [sequences + 1]")
+        seqs = cu_seqlens.numel() - 1
+        cu_seqlens = cu_seqlens.contiguous()
+    if state.shape != (seqs, hv, dv, dk):
+        raise ValueError(f"state must be [B, Hv, Dv, Dk] = {(seqs, hv, dv, dk)}, got {tuple(state.shape)}")
+    if mask is not None:
+        if mask.shape != (b, t_steps):
+            raise ValueError(f"mask must be [B, T] = {(b, t_steps)}, got {tuple(mask.shape)}")
+        mask = mask_bytes(mask, "mask")
+    zero_gaps = out is None
+    if out is None:
+        new = torch.zeros if seqs == 0 else torch.empty
+        out = new((b, t_steps, hv, dv), dtype=torch.bfloat16, device=dev)
+    elif (out.dtype != torch.bfloat16 or out.shape != (b, t_steps, hv, dv) or not out.is_contiguous()
+          or out.data_ptr() % 16 != 0):
+        raise ValueError(f"out must be contiguous, 16-byte aligned bf16 {(b, t_steps, hv, dv)}")
+    if out_state is None:
+        out_state = torch.empty((seqs, hv, dv, dk), dtype=torch.float32, device=dev)
+        state = _aligned(state)
+    else:
+        if (out_state.dtype != torch.float32 or out_state.shape != state.shape
+                or not out_state.is_contiguous() or out_state.data_ptr() % 16 != 0):
+            raise ValueError(f"out_state must be contiguous, 16-byte aligned fp32 {tuple(state.shape)}")
+        if out_state.data_ptr() == state.data_ptr() and state.is_contiguous():
+            pass   # in place
+        elif out_state.untyped_storage().data_ptr() == state.untyped_storage().data_ptr():
+            state = state.clone(memory_format=torch.contiguous_format)   # may overlap in part
+        else:
+            state = _aligned(state)
+    q, ldq = _token_rows(q)
+    k, ldk = _token_rows(k)
+    v, ldv = _token_rows(v)
+    g, beta = g.contiguous(), beta.contiguous()
+    with torch.cuda.device(dev):
+        st = _lib.load().dfl_gdn_rule_recurrent(
+            q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, g.data_ptr(),
+            1 if g.dim() == 4 else 0, beta.data_ptr(), None if mask is None else mask.data_ptr(),
+            None if cu_seqlens is None else cu_seqlens.data_ptr(), state.data_ptr(), out_state.data_ptr(),
+            out.data_ptr(), 1 if zero_gaps else 0, seqs, t_steps, hv, hk, dv, dk, stream_ptr(dev))
+    _lib.check("dfl_gdn_rule_recurrent", st)
+    return out, out_state
+
+
+def _aligned(x: torch.Tensor) -> torch.Tensor:
+    """``x`` contiguous with 16-byte aligned storage."""
+    x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
 # ------------------------------------------------------------------ DDTree

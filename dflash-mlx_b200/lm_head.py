@@ -14,6 +14,8 @@ Mirrors the reference's verify tail (``dflash_mlx/engine/spec_epoch.py:2067-2072
   acceptance scan on device.
 * :func:`lm_head_verify` -- both, for one device or, with a process group,
   for a vocabulary split across ranks (all-gather of the keys).
+* :func:`verify_accept_sampled` -- sampled decoding: accept drafts against the
+  target's probabilities and draw the next token, from given random numbers.
 * :func:`match_acceptance_length` -- the reference helper on device tensors.
 """
 
@@ -25,7 +27,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._runtime import require_cuda, stream_ptr, workspace
+from ._runtime import mask_bytes, require_cuda, same_device, stream_ptr, workspace
 
 
 def workspace_bytes(rows: int, dim: int, vocab: int) -> int:
@@ -122,6 +124,109 @@ def lm_head_verify(hidden: torch.Tensor, weight: torch.Tensor, verify_ids: Optio
     if group is not None:
         keys = gather_keys(keys, group)
     return verify_accept(keys, verify_ids, block=block)
+
+
+_LOGIT_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _logit_rows(x: torch.Tensor):
+    """``x [B, R, V]`` with neighbouring ids next to each other, the row and the
+    request strides (rows are read where they are: a view of some of a larger
+    buffer's rows costs no copy)."""
+    if x.shape[2] > 1 and x.stride(2) != 1:
+        x = x.contiguous()
+    return x, int(x.stride(1)), int(x.stride(0))
+
+
+def verify_accept_sampled(logits: torch.Tensor, verify_ids: torch.Tensor, accept_u: torch.Tensor,
+                          sample_u: torch.Tensor, *, draft_logits: Optional[torch.Tensor] = None,
+                          temperature=1.0, draft_lens: Optional[torch.Tensor] = None,
+                          suppress_token_mask: Optional[torch.Tensor] = None):
+    """Sampled acceptance of drafted tokens: ``(acceptance int32 [B], next_token
+    int32 [B], draft_prob fp32 [B, T - 1])``.
+
+    ``logits [B, T, V]`` (bf16, fp16 or fp32) are the target's, row i after
+    token i of the block; ``verify_ids [B, T]`` holds the staged token and then
+    the drafts, as for :func:`verify_accept`.  With ``p_i = softmax(logits[:,
+    i] / temperature)`` without the suppressed ids, and ``q_i`` the draft
+    model's ``softmax(draft_logits[:, i] / temperature)`` (``draft_logits [B,
+    T - 1, V]``; None: greedy drafts, ``q_i`` all on the drafted id), draft
+    ``x = verify_ids[:, i + 1]`` is accepted while ``accept_u[:, i] * q_i(x) <
+    p_i(x)``; the next token is drawn with ``sample_u`` from ``max(p - q, 0)``
+    at the first rejected draft, or from the target's row after the last
+    draft, by inverse cumulative sum in id order.  Committed tokens are then
+    distributed as the target's own samples.
+
+    ``temperature`` is a number or an fp32 tensor ``[B]`` (0: greedy, as
+    :func:`verify_accept`); ``draft_lens`` int32 ``[B]`` counts each request's
+    drafts (0: only a next token; rows past it are not read); ``accept_u [B,
+    T - 1]`` and ``sample_u [B]`` are uniform in [0, 1).  ``T = 1`` samples
+    single tokens.  ``draft_prob[b, i]`` is ``p_i`` of the draft (0 past
+    ``draft_lens``).  A row with nothing to draw from (every id suppressed, -inf
+    or NaN) gives ``next_token = -1``.  Nothing is read back to the host.
+    """
+    require_cuda(logits, "logits")
+    dev = logits.device
+    if logits.dtype not in _LOGIT_TYPES:
+        raise NotImplementedError(f"logits must be bfloat16, float16 or float32, got {logits.dtype}")
+    if logits.dim() != 3 or logits.shape[1] < 1 or logits.shape[2] < 1:
+        raise ValueError(f"logits must be [B, T, V], got {tuple(logits.shape)}")
+    b, t, v = (int(x) for x in logits.shape)
+    same_device(dev, verify_ids=verify_ids, accept_u=accept_u, sample_u=sample_u,
+                draft_logits=draft_logits, draft_lens=draft_lens, suppress_token_mask=suppress_token_mask)
+    if tuple(verify_ids.shape) != (b, t) or verify_ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"verify_ids must be int32 or int64 {(b, t)}")
+    if tuple(accept_u.shape) != (b, t - 1) or tuple(sample_u.shape) != (b,):
+        raise ValueError(f"accept_u must be {(b, t - 1)} and sample_u {(b,)}")
+    if accept_u.dtype != torch.float32 or sample_u.dtype != torch.float32:
+        raise ValueError("accept_u and sample_u must be float32")
+    if draft_logits is not None:
+        if tuple(draft_logits.shape) != (b, t - 1, v) or draft_logits.dtype != logits.dtype:
+            raise ValueError(f"draft_logits must be {logits.dtype} {(b, t - 1, v)}")
+        if t == 1:
+            draft_logits = None
+    if isinstance(temperature, torch.Tensor):
+        same_device(dev, temperature=temperature)
+        if temperature.dtype != torch.float32 or tuple(temperature.shape) != (b,):
+            raise ValueError(f"temperature must be a number or float32 {(b,)}")
+        temperature = temperature.contiguous()
+    else:
+        if not float(temperature) >= 0.0:
+            raise ValueError(f"temperature must be >= 0, got {temperature}")
+        temperature = torch.full((b,), float(temperature), dtype=torch.float32, device=dev)
+    if draft_lens is not None:
+        if draft_lens.dtype != torch.int32 or tuple(draft_lens.shape) != (b,):
+            raise ValueError(f"draft_lens must be int32 {(b,)}")
+        draft_lens = draft_lens.contiguous()
+    sup = None
+    if suppress_token_mask is not None:
+        if tuple(suppress_token_mask.shape) != (v,):
+            raise ValueError(f"suppress_token_mask must be {(v,)}")
+        sup = mask_bytes(suppress_token_mask, "suppress_token_mask")
+    logits, ld, bs = _logit_rows(logits)
+    ldd = bsd = 0
+    if draft_logits is not None:
+        draft_logits, ldd, bsd = _logit_rows(draft_logits)
+    ids = verify_ids.to(torch.int32).contiguous()
+    accept_u, sample_u = accept_u.contiguous(), sample_u.contiguous()
+    acc = torch.empty(b, dtype=torch.int32, device=dev)
+    nxt = torch.empty(b, dtype=torch.int32, device=dev)
+    prob = torch.empty((b, t - 1), dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        st = ctypes.c_int(0)
+        n = _lib.load().dfl_verify_sampled_workspace_bytes(b, t, v, 0 if draft_logits is None else 1,
+                                                           ctypes.byref(st))
+        _lib.check("dfl_verify_sampled_workspace_bytes", st.value)
+        # scratch of this call alone (any content), not one of the zero-filled workspaces
+        ws = torch.empty(max(int(n), 16), dtype=torch.uint8, device=dev)
+        status = _lib.load().dfl_verify_accept_sampled(
+            logits.data_ptr(), None if draft_logits is None else draft_logits.data_ptr(),
+            _LOGIT_TYPES[logits.dtype], ids.data_ptr(), accept_u.data_ptr(), sample_u.data_ptr(),
+            temperature.data_ptr(), None if draft_lens is None else draft_lens.data_ptr(),
+            None if sup is None else sup.data_ptr(), acc.data_ptr(), nxt.data_ptr(), prob.data_ptr(),
+            ld, bs, ldd, bsd, b, t, v, ws.data_ptr(), ws.numel(), stream_ptr(dev))
+    _lib.check("dfl_verify_accept_sampled", status)
+    return acc, nxt, prob
 
 
 # ------------------------------------------------- vocabulary split (host side)

@@ -26,7 +26,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._runtime import require_cuda, stream_ptr, workspace
+from ._runtime import require_cuda, same_device, stream_ptr, workspace
 from .verify_qmm import qmm_w4g64
 
 
@@ -86,6 +86,104 @@ def route(router_logits: torch.Tensor, top_k: int = 8):
                                        w.data_ptr(), ids.data_ptr(), stream_ptr(dev))
     _lib.check("dfl_moe_route", st)
     return table, w, ids
+
+
+_ROUTE_SIGMOID, _ROUTE_GROUP_TOP2, _ROUTE_RENORM = 1, 2, 4
+_LOGIT_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def route_experts(router_logits: torch.Tensor, top_k: int, *, score: str = "softmax",
+                  bias: Optional[torch.Tensor] = None, n_groups: int = 1,
+                  topk_groups: Optional[int] = None, group_score: Optional[str] = None,
+                  renormalize: bool = True, scale: float = 1.0):
+    """Routing of any number of tokens: ``(weights fp32 [T, k], topk_ids int32 [T, k])``.
+
+    ``s = softmax(logits)`` or ``sigmoid(logits)`` (``score``); experts are
+    chosen by ``c = s + bias`` (``bias`` fp32 ``[E]``, a balance bias that does
+    not enter the weights): of ``n_groups`` groups of neighbours the
+    ``topk_groups`` best stay (by the sum of their two largest c, ``group_score
+    = "top2"``, the default for sigmoid scores, or by their largest, ``"max"``,
+    the default for softmax), and of their experts the ``top_k`` with the
+    largest c, largest first, ties to the lower id.  The weights are the
+    chosen ``s``, divided by their sum (``renormalize``), times ``scale``.
+
+    ``router_logits [T, E]`` is bf16, fp16 or fp32 and may be row-strided.  An
+    expert whose logit is NaN or -inf has weight 0 and is named only where no
+    other is left, so a token with nothing to choose has valid ids and zero
+    weights.
+    """
+    require_cuda(router_logits, "router_logits")
+    lg = router_logits
+    dev = lg.device
+    if lg.dtype not in _LOGIT_TYPES:
+        raise NotImplementedError(f"router_logits must be bfloat16, float16 or float32, got {lg.dtype}")
+    if lg.dim() != 2 or lg.shape[1] < 1:
+        raise ValueError(f"router_logits must be [T, E], got {tuple(lg.shape)}")
+    t, e = (int(x) for x in lg.shape)
+    if score not in ("softmax", "sigmoid"):
+        raise ValueError(f"score must be softmax or sigmoid, got {score!r}")
+    group_score = group_score or ("top2" if score == "sigmoid" else "max")
+    if group_score not in ("top2", "max"):
+        raise ValueError(f"group_score must be top2 or max, got {group_score!r}")
+    groups = int(n_groups)
+    kept = groups if topk_groups is None else int(topk_groups)
+    if groups < 1 or e % groups != 0 or not 1 <= kept <= groups:
+        raise ValueError(f"{e} experts in {groups} groups, {kept} of them kept")
+    if not 1 <= int(top_k) <= min(32, kept * (e // groups)):
+        raise ValueError(f"top_k = {top_k}: 1 to 32, and at most the {kept * (e // groups)} experts of the kept groups")
+    if bias is not None:
+        same_device(dev, bias=bias)
+        if bias.dtype != torch.float32 or tuple(bias.shape) != (e,):
+            raise ValueError(f"bias must be float32 {(e,)}")
+        bias = bias.contiguous()
+    if (e > 1 and lg.stride(1) != 1) or (t > 1 and lg.stride(0) < e):
+        lg = lg.contiguous()
+    w = torch.empty((t, int(top_k)), dtype=torch.float32, device=dev)
+    ids = torch.empty((t, int(top_k)), dtype=torch.int32, device=dev)
+    flags = ((_ROUTE_SIGMOID if score == "sigmoid" else 0) | (_ROUTE_GROUP_TOP2 if group_score == "top2" else 0)
+             | (_ROUTE_RENORM if renormalize else 0))
+    with torch.cuda.device(dev):
+        st = _lib.load().dfl_moe_route_experts(
+            lg.data_ptr(), _LOGIT_TYPES[lg.dtype], int(lg.stride(0)) if t > 1 else e,
+            None if bias is None else bias.data_ptr(), t, e, int(top_k), groups, kept, flags, float(scale),
+            w.data_ptr(), ids.data_ptr(), stream_ptr(dev))
+    _lib.check("dfl_moe_route_experts", st)
+    return w, ids
+
+
+@dataclass
+class Router:
+    """How a MoE block's router scores and chooses experts (:func:`route_experts`);
+    :func:`moe_layer` and :class:`MoEPlanLayer` take one as ``router``."""
+
+    score: str = "softmax"
+    bias: Optional[torch.Tensor] = None
+    n_groups: int = 1
+    topk_groups: Optional[int] = None
+    group_score: Optional[str] = None
+    renormalize: bool = True
+    scale: float = 1.0
+
+    def __call__(self, router_logits: torch.Tensor, top_k: int):
+        return route_experts(router_logits, top_k, score=self.score, bias=self.bias, n_groups=self.n_groups,
+                             topk_groups=self.topk_groups, group_score=self.group_score,
+                             renormalize=self.renormalize, scale=self.scale)
+
+
+def route_table(topk_ids: torch.Tensor, n_experts: int) -> torch.Tensor:
+    """The route table of :func:`route` from given ids (int32 ``[T, k]``, T and k <= 16)."""
+    require_cuda(topk_ids, "topk_ids")
+    if topk_ids.dtype != torch.int32 or topk_ids.dim() != 2:
+        raise ValueError("topk_ids must be int32 [T, k]")
+    ids = topk_ids.contiguous()
+    t, k = (int(x) for x in ids.shape)
+    dev = ids.device
+    table = torch.empty(int(_lib.load().dfl_moe_route_table_ints(int(n_experts))), dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        st = _lib.load().dfl_moe_route_table(ids.data_ptr(), t, k, int(n_experts), table.data_ptr(),
+                                             stream_ptr(dev))
+    _lib.check("dfl_moe_route_table", st)
+    return table
 
 
 def gather_qmm(x: torch.Tensor, weight: QuantWeight, table: torch.Tensor, *, rows_out: int,
@@ -205,17 +303,23 @@ def dense_mlp(x: torch.Tensor, gate: QuantWeight, up: QuantWeight, down: QuantWe
 
 
 def moe_layer(x: torch.Tensor, router_logits: torch.Tensor, experts: dict, shared: Optional[dict],
-              top_k: int = 8) -> torch.Tensor:
+              top_k: int = 8, router: Optional[Router] = None) -> torch.Tensor:
     """One MoE verify layer: ``x`` bf16 ``[T, H]`` -> bf16 ``[T, H]``.
 
     ``experts``: QuantWeight stacks ``gate`` / ``up`` ``[E, I, H/8]`` (or one
     interleaved ``gate_up`` stack ``[E, 2I, H/8]``, :func:`fuse_expert_gate_up`)
     and ``down`` ``[E, H, I/8]``; ``shared``: unstacked QuantWeights ``gate`` /
-    ``up`` (or an interleaved ``gate_up``) and ``down``, or None.
+    ``up`` (or an interleaved ``gate_up``) and ``down``, or None.  ``router``:
+    scores and choice of another router (:class:`Router`) than the softmax
+    top-k of :func:`route`.
     """
     require_cuda(x, "x")
     t = x.shape[0]
-    table, w, _ = route(router_logits, top_k)
+    if router is None:
+        table, w, _ = route(router_logits, top_k)
+    else:
+        w, ids = router(router_logits, top_k)
+        table = route_table(ids, router_logits.shape[1])
     # The shared expert does not depend on the routing: run it first, so the
     # grouped launches after it find the route table already complete and can
     # stream their weights while the launch before them finishes.
@@ -348,12 +452,15 @@ class MoEPlanLayer:
     interleaved ``gate_up`` (:func:`fuse_expert_gate_up`) and ``down``
     ``[E, H, I/8]``; ``shared``: QuantWeights ``gate`` / ``up`` (or
     ``gate_up``) and ``down``, or None.  ``stack_shared=False`` keeps a
-    same-shaped shared expert in dense phases too.  Needs I % 64 == 0,
+    same-shaped shared expert in dense phases too.  ``router``: scores and
+    choice of another router (:class:`Router`) than the softmax top-k; routing
+    and sorting are then two launches, and a shared expert stays in dense
+    phases.  Needs I % 64 == 0,
     H % 128 == 0 and ``tokens * top_k`` <= 240.
     """
 
     def __init__(self, experts: dict, shared: Optional[dict], tokens: int, top_k: int = 8,
-                 stack_shared: bool = True):
+                 stack_shared: bool = True, router: Optional[Router] = None):
         from .qmm_plan import PlanPhase, ProjectionPlan, sorted_route_ints, tile_expert_stack, tile_weight
         from .verify_qmm import interleave_gate_up
 
@@ -369,6 +476,8 @@ class MoEPlanLayer:
         if not 1 <= t * k <= 240 or t > 16:
             raise ValueError(f"{t} tokens x top-{k}: the route kernels take <= 16 tokens, <= 240 pairs")
         dev = gu.q.device
+        self.router = router
+        stack_shared = stack_shared and router is None
         self.tokens, self.top_k, self.experts, self.hidden, self.inter = t, k, e, h, inter
         bf = dict(dtype=torch.bfloat16, device=dev)
         pairs = t * k
@@ -428,9 +537,14 @@ class MoEPlanLayer:
         if tuple(router_logits.shape) != (self.tokens, self.experts):
             raise ValueError(f"router_logits must be {(self.tokens, self.experts)}")
         dense_shared = self.shared_out is not None and not self.shared_stacked
-        w, _ = route_sorted(router_logits, x, self.top_k, route_out=self.route, x_sorted=self.x_sorted,
-                            x_copy=self.x_in if dense_shared else None, weights_out=self.weights,
-                            ids_out=self.ids, shared_expert=self.shared_stacked)
+        if self.router is not None:
+            w, ids = self.router(router_logits, self.top_k)
+            sort_pairs(ids, x, self.experts, route_out=self.route, x_sorted=self.x_sorted,
+                       x_copy=self.x_in if dense_shared else None)
+        else:
+            w, _ = route_sorted(router_logits, x, self.top_k, route_out=self.route, x_sorted=self.x_sorted,
+                                x_copy=self.x_in if dense_shared else None, weights_out=self.weights,
+                                ids_out=self.ids, shared_expert=self.shared_stacked)
         self.plan.run()
         pairs = self.tokens * self.top_k
         return combine(self.pair_out[:pairs], w, self.shared_out)

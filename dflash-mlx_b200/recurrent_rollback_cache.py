@@ -6,6 +6,9 @@ and the restore policy of ``dflash_mlx/engine/target_qwen_gdn.py:1025-1055``:
 * ``arm_rollback`` snapshots ``[conv_state, ssm_state]`` (``:96-103``);
 * ``record_tape`` keeps the verify forward's innovation tape, k, g and qkv
   (``:110-121``);
+* ``advance(q, k, v, g, beta)`` runs a layer's recurrence on the cached state:
+  with the tape when armed, over a whole prompt or a single token otherwise
+  (``engine/target_qwen_gdn.py:610-642``);
 * ``rollback(n_accepted)`` restores the snapshot and replays
   ``n_accepted + 1`` steps of the tape (``:142-165``), rebuilding the conv
   state from the last ``conv_kernel_size - 1`` inputs (``:123-140``);
@@ -26,7 +29,7 @@ from typing import Any, Optional, Sequence, Union
 
 import torch
 
-from .kernels import tape_replay_
+from .kernels import gated_delta_kernel_with_tape, gated_delta_rule, tape_replay_
 
 
 class RecurrentRollbackCache:
@@ -68,6 +71,25 @@ class RecurrentRollbackCache:
         self._tape_k = k.contiguous()
         self._tape_g = g.contiguous()
         self._tape_qkv = None if qkv is None else qkv.contiguous()
+
+    def advance(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor, *,
+                qkv: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``y`` of a GDN layer's tokens; ``cache[1]`` becomes the state after them
+        (an empty cache starts from zeros).  Armed, the verify forward runs and
+        its tape is recorded (T <= 64); otherwise ``gated_delta_rule``."""
+        state = self.cache[1]
+        if state is None:
+            state = torch.zeros((k.shape[0], v.shape[2], v.shape[3], k.shape[3]), dtype=torch.float32,
+                                device=k.device)
+            if self._armed and self._snapshot is not None:
+                self._snapshot[1] = state
+        if self._armed:
+            y, new, tape = gated_delta_kernel_with_tape(q, k, v, g, beta, state, mask)
+            self.record_tape(tape=tape, k=k, g=g, qkv=qkv)
+        else:
+            y, new = gated_delta_rule(q, k, v, g, beta, state, mask=mask)
+        self.cache[1] = new
+        return y
 
     def _rebuild_conv_state(self, accepted_steps: torch.Tensor) -> Optional[torch.Tensor]:
         """Last ``conv_kernel_size - 1`` conv inputs after ``accepted_steps[b]``

@@ -317,6 +317,36 @@ int dfl_gdn_forward_tape(const uint16_t* q, const uint16_t* k, const uint16_t* v
                          int B, int T, int Hv, int Hk, int Dv, int Dk, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Gated delta rule over whole sequences: prompts of any length and single
+ * tokens, without a tape.
+ *
+ * For every sequence n, value head hv (q/k head hk = hv / (Hv / Hk)) and step t:
+ *     S' = S * g_t;  delta = (v_t - S' k_t) * beta_t;  S = S' + delta (x) k_t;  y_t = S q_t
+ * from state_in[n] to state_out[n].  A step with mask 0 leaves S and writes
+ * y = 0; its q, k, v, g and beta may hold anything.
+ *   cu_seqlens NULL: B sequences of T tokens each (token b * T + t);
+ *   else int32 [B + 1] on the device: T tokens in all, sequence n is tokens
+ *     cu_seqlens[n] .. cu_seqlens[n + 1] - 1 (lengths of 0 and 1 are fine).  y rows of no
+ *     sequence are set to 0 (zero_gaps) or left as they were.  Offsets that
+ *     decrease or leave [0, T] set the device error word and are cut to it.
+ *   q, k   bf16, token i at q + i * ldq (ldq >= Hk * Dk elements), heads [Hk, Dk]
+ *   v      bf16, token i at v + i * ldv (ldv >= Hv * Dv), heads [Hv, Dv]
+ *   g      fp32 [tokens, Hv] or [tokens, Hv, Dk] (g_vectorized)   beta fp32 [tokens, Hv]
+ *   mask   uint8 [tokens] or NULL
+ *   state  fp32 [B, Hv, Dv, Dk], 16-byte aligned (state_out may be state_in)
+ *   y      bf16 [tokens, Hv, Dv], 16-byte aligned
+ * Constraints: Dk in {32, 64, 128, 256}, Dv % 32 == 0, Hv % Hk == 0.
+ * dfl_gdn_rule_recurrent takes one step after the other (fp32 throughout).
+ * The reference reaches this step, for caches that record no tape, through
+ * mlx-lm's gated_delta_update (third party) from the hook at
+ * dflash_mlx/engine/target_qwen_gdn.py:551-651. */
+int dfl_gdn_rule_recurrent(const uint16_t* q, int ldq, const uint16_t* k, int ldk, const uint16_t* v,
+                           int ldv, const float* g, int g_vectorized, const float* beta,
+                           const uint8_t* mask, const int32_t* cu_seqlens, const float* state_in,
+                           float* state_out, uint16_t* y, int zero_gaps, int B, int T, int Hv, int Hk,
+                           int Dv, int Dk, void* stream);
+
+/* ------------------------------------------------------------------------
  * DDTree verify: the GDN recurrence over a token tree.
  *
  * Node t starts from the state of node parent_ids[t] (parents before
@@ -393,6 +423,43 @@ int dfl_lmhead_accept(const uint64_t* keys, int G, const int32_t* verify_ids, in
  * Replaces match_acceptance_length (dflash_mlx/engine/acceptance.py:9-16). */
 int dfl_match_acceptance(const int32_t* drafted, const int32_t* posterior, int B, int L,
                          int32_t* acceptance, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Sampled verification of drafted tokens, from given random numbers.
+ *
+ * For request b with temperature z = temperature[b], n = draft_lens[b] drafts
+ * (draft_lens NULL: T - 1; cut to [0, T - 1]) x_i = verify_ids[b, i] (i = 1 ..
+ * n; verify_ids[b, 0] is the staged token), and row i of the target's logits
+ * after the block's token i:
+ *     p_i = softmax(logits[b, i] / z) without the suppressed ids,
+ *     q_i = softmax(draft_logits[b, i] / z), or, draft_logits NULL, all on x_{i+1};
+ *     acceptance[b] = first i < n with not (accept_u[b, i] * q_i(x_{i+1}) < p_i(x_{i+1})), else n;
+ *     next_token[b] = the first id v whose sum of weights over ids <= v
+ *       exceeds sample_u[b] * total, the weights being max(p_a - q_a, 0)
+ *       after a rejection (p_a where nothing is left) and p_n otherwise, a the acceptance;
+ *     draft_prob[b, i] = p_i(x_{i+1}) for i < n, 0 for the rest.
+ * z <= 0 or NaN is greedy: p_i is all on the largest logit's lowest id.  A
+ * logit of NaN or -inf has probability 0 (what a suppressed id's logit holds
+ * does not matter); a row with nothing left gives next_token -1; a draft id
+ * outside [0, V) is rejected.  Rows past draft_lens[b] are not read.
+ *   logits [B, T, V] and draft_logits [B, T - 1, V]: bf16 (dtype 0), fp16 (1)
+ *   or fp32 (2), rows ld_* and requests bs_* elements apart; verify_ids int32
+ *   [B, T]; accept_u fp32 [B, T - 1] and sample_u fp32 [B], in [0, 1);
+ *   temperature fp32 [B]; suppress uint8 [V] or NULL; acceptance and
+ *   next_token int32 [B]; draft_prob fp32 [B, T - 1].
+ * Constraints: 1 <= T <= 256, V <= 2^24, B * (2 T - 1) <= 65535 rows.
+ * workspace: dfl_verify_sampled_workspace_bytes bytes, 16-byte aligned, with
+ * any content; it must not be one of the zero-filled workspaces above.
+ * Sampled form of the tail that dfl_lmhead_argmax + dfl_lmhead_accept are the
+ * greedy form of (dflash_mlx/engine/spec_epoch.py:2067-2072,2129). */
+size_t dfl_verify_sampled_workspace_bytes(int B, int T, int V, int with_draft, int* status);
+int dfl_verify_accept_sampled(const void* logits, const void* draft_logits, int dtype,
+                              const int32_t* verify_ids, const float* accept_u, const float* sample_u,
+                              const float* temperature, const int32_t* draft_lens,
+                              const uint8_t* suppress, int32_t* acceptance, int32_t* next_token,
+                              float* draft_prob, size_t ld_logits, size_t bs_logits, size_t ld_draft,
+                              size_t bs_draft, int B, int T, int V, void* workspace,
+                              size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
  * MoE expert path (routed experts of one verify block).
@@ -488,6 +555,35 @@ int dfl_moe_sort_pairs(const int32_t* topk_ids, int T, int top_k, int E, const u
 int dfl_moe_route_sorted(const float* logits, int T, int E, int top_k, int shared_expert,
                          const uint16_t* x, int ldx, int H, int32_t* route, float* weights,
                          int32_t* topk_ids, uint16_t* x_sorted, uint16_t* x_copy, void* stream);
+
+/* Routing with the scores of other MoE routers, for any number of tokens.
+ * For each row l of logits [T, E] (rows ld elements apart; bf16 (dtype 0),
+ * fp16 (1) or fp32 (2)):
+ *     s = sigmoid(l) (DFL_ROUTE_SIGMOID) or softmax(l);  c = s + bias (fp32 [E] or NULL);
+ *     n_groups > 1: experts in n_groups groups of E / n_groups neighbours, a
+ *       group's score its largest c, or the sum of its two largest
+ *       (DFL_ROUTE_GROUP_TOP2); the topk_groups best groups stay;
+ *     topk_ids = the top_k experts of those by c, largest first;
+ *     weights = s[topk_ids], over their sum (DFL_ROUTE_RENORM), times scale.
+ * Ties go to the lower id (group, expert).  Scores are in 64 bits.  An expert
+ * whose logit is NaN or -inf, or whose c is -inf or NaN, has weight 0 and
+ * fills a slot only where no other is left (ids stay distinct and in [0, E)).
+ * Constraints: E <= 4096, top_k <= 32, top_k <= topk_groups * (E / n_groups).
+ *
+ * dfl_moe_route_table: dfl_moe_route's route table from given ids
+ * (topk_ids int32 [T, top_k], T <= 16, top_k <= 16), for dfl_moe_qmm_w4g64.  An id
+ * outside [0, E), or an expert that occurs more than 16 times, sets the device
+ * error word and the pair is left out of the table.
+ * The router of the MoE blocks that the reference reaches from
+ * dflash_mlx/engine/target_qwen_gdn.py:863-865 (mlx-lm, third party). */
+#define DFL_ROUTE_SIGMOID 1
+#define DFL_ROUTE_GROUP_TOP2 2
+#define DFL_ROUTE_RENORM 4
+int dfl_moe_route_experts(const void* logits, int dtype, size_t ld, const float* bias, int T, int E,
+                          int top_k, int n_groups, int topk_groups, int flags, float scale,
+                          float* weights, int32_t* topk_ids, void* stream);
+int dfl_moe_route_table(const int32_t* topk_ids, int T, int top_k, int E, int32_t* route_table,
+                        void* stream);
 
 #ifdef __cplusplus
 }

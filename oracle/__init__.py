@@ -18,6 +18,7 @@ reference file:line it follows (paths relative to the dflash-mlx project):
 * ``lmhead``   -- ``engine/sampling.py:47-55`` (argmax with a -1e9 floor on
   suppressed ids) and ``engine/acceptance.py:9-16`` (sum of cumprod of
   matches), composed as at ``engine/spec_epoch.py:2067-2072``.
+* ``sampled``  -- sampled acceptance of drafts (the definition in float64).
 * ``gdn``      -- ``dflash_mlx/kernels.py:125-167`` (gated-delta forward with
   innovation tape), ``kernels.py:421-458`` (tree forward, used to pin the
   replay identity) and ``kernels.py:790-820`` (tape replay).

@@ -181,3 +181,34 @@ def tree_depthwise_conv1d(qkv, prefix, weight, bias, path_indices):
     if bias is not None:
         acc = (acc + np.asarray(bias, np.float32)[None, None, :]).astype(np.float32)
     return (acc / (np.float32(1.0) + np.exp(-acc))).astype(np.float32)
+
+
+def gated_delta_rule(q, k, v, g, beta, state, mask=None, lens=None):
+    """The recurrence without a tape, in float64: ``(y, new state)``.
+
+    Padded ``[B, T, ...]`` inputs with an optional ``mask [B, T]``, or packed
+    ones (``B = 1``) with the sequences' ``(first, end)`` token ranges in
+    ``lens`` and one state per sequence.  Masked steps are skipped, so what
+    they hold enters nothing.
+    """
+    q, k, v, g, beta = (np.asarray(a, np.float64) for a in (q, k, v, g, beta))
+    s_all = np.array(state, np.float64, copy=True)
+    hv = v.shape[2]
+    r = hv // k.shape[2]
+    y = np.zeros(v.shape, np.float64)
+    if lens is None:
+        rows = [(b, range(k.shape[1]), b) for b in range(k.shape[0])]
+    else:
+        rows = [(0, range(a, e), n) for n, (a, e) in enumerate(lens)]
+    for b, steps, n in rows:
+        s = s_all[n]
+        for t in steps:
+            if mask is not None and not mask[b, t]:
+                continue
+            kt, qt = np.repeat(k[b, t], r, axis=0), np.repeat(q[b, t], r, axis=0)
+            s = s * (g[b, t][:, None, None] if g.ndim == 3 else g[b, t][:, None, :])
+            d = beta[b, t][:, None] * (v[b, t] - np.einsum("hij,hj->hi", s, kt))
+            s = s + d[:, :, None] * kt[:, None, :]
+            y[b, t] = np.einsum("hij,hj->hi", s, qt)
+        s_all[n] = s
+    return y, s_all

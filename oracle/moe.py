@@ -95,3 +95,42 @@ def moe_layer(x, router_logits, experts, shared, top_k: int = 8):
 def distinct_experts(router_logits, top_k: int = 8) -> int:
     ids, _ = route_topk(router_logits, top_k)
     return int(np.unique(ids).size)
+
+
+def route_experts(logits, top_k, score="softmax", bias=None, n_groups=1, topk_groups=None, group_score=None,
+                  renormalize=True, scale=1.0):
+    """Scores, groups and choice of a general router in float64, one token at a
+    time: (weights float64 [T, k], ids int32 [T, k]).  Experts that cannot be
+    had (NaN or -inf logits) come last, by id, with weight 0."""
+    lg = np.asarray(logits, np.float64)
+    t, e = lg.shape
+    size = e // n_groups
+    keep = n_groups if topk_groups is None else topk_groups
+    two = (group_score or ("top2" if score == "sigmoid" else "max")) == "top2"
+    ids = np.zeros((t, top_k), np.int32)
+    weights = np.zeros((t, top_k))
+    for i in range(t):
+        have = lg[i] > -np.inf
+        s = np.zeros(e)
+        if score == "sigmoid":
+            s[have] = 1.0 / (1.0 + np.exp(-lg[i][have]))
+        elif have.any():
+            x = lg[i][have]
+            w = (x == np.inf).astype(float) if x.max() == np.inf else np.exp(x - x.max())
+            s[have] = w / w.sum()
+        c = np.where(have, s + (0.0 if bias is None else np.asarray(bias, np.float64)), -np.inf)
+        c[np.isnan(c)] = -np.inf
+        left = np.ones(e, bool)
+        if n_groups > 1:
+            gs = []
+            for g in range(n_groups):
+                best = np.sort(c[g * size:(g + 1) * size])[::-1]
+                gs.append(best[0] + best[1] if two and size > 1 and best[1] > -np.inf else best[0])
+            order = sorted(range(n_groups), key=lambda g: (-gs[g], g))[:keep]
+            left = np.isin(np.arange(e) // size, order)
+        order = sorted(np.nonzero(left)[0], key=lambda x: (-c[x], x))[:top_k]
+        ids[i] = order
+        weights[i] = [s[x] if c[x] > -np.inf else 0.0 for x in order]
+        if renormalize:
+            weights[i] = weights[i] / weights[i].sum() if weights[i].sum() > 0 else 0.0
+    return weights * scale, ids
