@@ -216,6 +216,572 @@ int launch_recurrent(const RuleParams& p, cudaStream_t stream) {
   return host::launch_status();
 }
 
+// --------------------------------------------------------------- chunked form
+// Steps are taken 64 at a time.  With D_ij = g_{j+1} .. g_i (1 for i = j),
+// c_i = g_0 .. g_i, S the state before the chunk and K, Q, V the chunk's rows,
+//     A_ij = beta_i D_ij (k_i . k_j) for j < i, else 0,   T = (I + A)^-1,
+//     R = diag(beta) (V - diag(c) K S^T),                 Delta = T R,
+//     Y = diag(c) Q S^T + P Delta,  P_ij = D_ij (q_i . k_j) for j <= i,
+//     S <- c_63 S + sum_i D_63,i delta_i (x) k_i
+// is what the 64 steps give one after the other.  D is formed by products, not
+// as a quotient or an exponential of sums, so decays of 0 or of any size are
+// exact cases.
+//
+// A CTA owns up to 128 value rows of one head and walks the sequence's chunks.
+// All products run on the tensor cores transposed, value rows in the 128 TMEM
+// lanes: S K^T, S Q^T, R T^T, Delta P^T and Delta K, so the state row, R and
+// Delta of a value row stay with its threads (fp32 in registers), enter the
+// products from TMEM, and only K, Q, T and P are read from shared memory, K
+// both as it is and transposed from the same tile.
+//
+// fp32 in bf16 products: K and Q are bf16 already.  The state and the update
+// go in as three bf16 parts (24 bits), so what is carried from chunk to chunk
+// keeps 32-bit accuracy; R, T - I, P, and the state's and Delta's share of y
+// as two parts each (16 bits, without the product of the two second parts):
+// they are corrections to R that is added in fp32, or end in y's 8 bits.
+//
+// Warps: 0-3 load a stage ahead (cp.async, zeros for masked steps and behind
+// the end) and prepare T and P of the next chunk (K K^T and Q K^T from one
+// product, inverse by blocks of 16, 32 and 64 in fp32); 4-11 (two threads per
+// value row, half the columns each) carry the state; 12 issues the products.
+constexpr int CH = 64;               // steps of a chunk
+constexpr int C_THREADS = 13 * 32;
+constexpr int C_STAGES = 3;
+constexpr int C_PREP = 128, C_STATE = 256;
+
+template <int DK>
+struct CCfg {
+  static constexpr int ATOM = 128 * 128;                 // 128 rows (K, then Q) x 64 columns
+  static constexpr int KQ_BYTES = (DK / 64) * ATOM;
+  static constexpr int V_BYTES = CH * 256;               // 64 rows x 128 columns
+  static constexpr int STAGE_BYTES = KQ_BYTES + V_BYTES;
+  static constexpr int TP_BYTES = 4 * CH * 128;          // T and P, two parts each
+  static constexpr int TP_OFF = C_STAGES * STAGE_BYTES;
+  static constexpr int SMALL_OFF = TP_OFF + 2 * TP_BYTES;
+  static constexpr int SMALL_BYTES = (C_STAGES * 2 + 2 * 2) * CH * 4 + 256;
+  static constexpr int SMEM_BYTES = SMALL_OFF + SMALL_BYTES + 1024;
+  // TMEM columns
+  static constexpr int S_PART = DK / 2;                  // columns of one part of the state
+  static constexpr int COL_S = 0;                        // state parts; later Delta K's three parts
+  static constexpr int COL_D = 192;                      // S K^T, then R T^T, then Delta K
+  static constexpr int COL_G = 256;                      // [K; Q] K^T, over Delta K's second half
+  static constexpr int COL_SQ = 320;                     // S Q^T
+  static constexpr int COL_R = 384;                      // R's parts, then Delta's
+  static constexpr int COL_Y = 448;                      // Delta P^T
+};
+
+// The bf16 parts of two values, leading part returned, the rest left in a, b.
+__device__ __forceinline__ uint32_t take_part(float& a, float& b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  const uint32_t u = *reinterpret_cast<const uint32_t*>(&h);
+  a -= __uint_as_float(u << 16);
+  b -= __uint_as_float(u & 0xffff0000u);
+  return u;
+}
+
+// X parts of a row (n values) into TMEM columns col + part * stride.
+template <int PARTS, int N>
+__device__ __forceinline__ void store_parts(uint32_t taddr, int stride, const float (&x)[N]) {
+  static_assert(N % 32 == 0, "32 values, 16 columns at a time");
+#pragma unroll
+  for (int h = 0; h < N / 32; ++h) {
+    float r[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) r[i] = x[32 * h + i];
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+      uint32_t u[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) u[i] = take_part(r[2 * i], r[2 * i + 1]);
+      tmem_st_32x32b_x16(taddr + p * stride + 16 * h, u);
+    }
+  }
+}
+
+struct ChunkBars {
+  uint64_t full[C_STAGES], freed[C_STAGES];
+  uint64_t tp_full[2], tp_freed[2];
+  uint64_t g_full, g_read;
+  uint64_t s_ready, d1_done, r_ready, d3_done, delta_ready, d4_done, y_done, y_read;
+};
+
+// Unit lower triangular inverse of I + A in place, A 64 x 64 (strictly lower
+// part used), by the 128 preparing threads: diagonal blocks of 16 by forward
+// substitution, then T21 = -T22 (A21 T11) for blocks of 16 and of 32.
+__device__ __forceinline__ void invert_unit_lower(float* a, int t) {
+  if (t < 64) {
+    float* blk = a + (t / 16) * 16 * (CH + 1);
+    const int c = t % 16;
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float s0 = i == c ? 1.f : 0.f, s1 = 0.f;
+#pragma unroll
+      for (int j = 0; j < i; ++j) {
+        const float m = blk[i * CH + j];
+        if (j & 1) s1 = __fmaf_rn(-m, x[j], s1);
+        else s0 = __fmaf_rn(-m, x[j], s0);
+      }
+      x[i] = s0 + s1;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) blk[i * CH + c] = x[i];
+  }
+  named_bar_sync(1, C_PREP);
+  {
+    // two pairs of blocks of 16: 4 columns of one row per thread
+    const int pr = t / 64, i = (t % 64) / 4, c = (t % 4) * 4;
+    float* t11 = a + pr * 32 * (CH + 1);
+    float* a21 = t11 + 16 * CH;
+    const float* t22 = t11 + 16 * (CH + 1);
+    float4 m = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float x = a21[i * CH + j];
+      const float4 y = *reinterpret_cast<const float4*>(t11 + j * CH + c);
+      m.x = __fmaf_rn(x, y.x, m.x); m.y = __fmaf_rn(x, y.y, m.y);
+      m.z = __fmaf_rn(x, y.z, m.z); m.w = __fmaf_rn(x, y.w, m.w);
+    }
+    named_bar_sync(1, C_PREP);
+    *reinterpret_cast<float4*>(a21 + i * CH + c) = m;
+    named_bar_sync(1, C_PREP);
+    m = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float x = t22[i * CH + j];
+      const float4 y = *reinterpret_cast<const float4*>(a21 + j * CH + c);
+      m.x = __fmaf_rn(-x, y.x, m.x); m.y = __fmaf_rn(-x, y.y, m.y);
+      m.z = __fmaf_rn(-x, y.z, m.z); m.w = __fmaf_rn(-x, y.w, m.w);
+    }
+    named_bar_sync(1, C_PREP);
+    *reinterpret_cast<float4*>(a21 + i * CH + c) = m;
+    // the blocks above the diagonal hold A's zeros
+    named_bar_sync(1, C_PREP);
+  }
+  {
+    // one pair of blocks of 32: 4 columns of two rows per thread
+    const int i = (t / 8) * 2, c = (t % 8) * 4;
+    float* a21 = a + 32 * CH;
+    const float* t22 = a + 32 * (CH + 1);
+    float4 m0 = make_float4(0.f, 0.f, 0.f, 0.f), m1 = m0;
+#pragma unroll 8
+    for (int j = 0; j < 32; ++j) {
+      const float x0 = a21[i * CH + j], x1 = a21[(i + 1) * CH + j];
+      const float4 y = *reinterpret_cast<const float4*>(a + j * CH + c);
+      m0.x = __fmaf_rn(x0, y.x, m0.x); m0.y = __fmaf_rn(x0, y.y, m0.y);
+      m0.z = __fmaf_rn(x0, y.z, m0.z); m0.w = __fmaf_rn(x0, y.w, m0.w);
+      m1.x = __fmaf_rn(x1, y.x, m1.x); m1.y = __fmaf_rn(x1, y.y, m1.y);
+      m1.z = __fmaf_rn(x1, y.z, m1.z); m1.w = __fmaf_rn(x1, y.w, m1.w);
+    }
+    named_bar_sync(1, C_PREP);
+    *reinterpret_cast<float4*>(a21 + i * CH + c) = m0;
+    *reinterpret_cast<float4*>(a21 + (i + 1) * CH + c) = m1;
+    named_bar_sync(1, C_PREP);
+    m0 = make_float4(0.f, 0.f, 0.f, 0.f);
+    m1 = m0;
+#pragma unroll 8
+    for (int j = 0; j < 32; ++j) {
+      const float x0 = t22[i * CH + j], x1 = t22[(i + 1) * CH + j];
+      const float4 y = *reinterpret_cast<const float4*>(a21 + j * CH + c);
+      m0.x = __fmaf_rn(-x0, y.x, m0.x); m0.y = __fmaf_rn(-x0, y.y, m0.y);
+      m0.z = __fmaf_rn(-x0, y.z, m0.z); m0.w = __fmaf_rn(-x0, y.w, m0.w);
+      m1.x = __fmaf_rn(-x1, y.x, m1.x); m1.y = __fmaf_rn(-x1, y.y, m1.y);
+      m1.z = __fmaf_rn(-x1, y.z, m1.z); m1.w = __fmaf_rn(-x1, y.w, m1.w);
+    }
+    named_bar_sync(1, C_PREP);
+    *reinterpret_cast<float4*>(a21 + i * CH + c) = m0;
+    *reinterpret_cast<float4*>(a21 + (i + 1) * CH + c) = m1;
+    named_bar_sync(1, C_PREP);
+  }
+}
+
+template <int DK>
+__global__ void __launch_bounds__(C_THREADS, 1) gdn_rule_chunked(const RuleParams p) {
+  using C = CCfg<DK>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ ChunkBars bars;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_word;
+
+  const int tiles = (p.Dv + 127) / 128;
+  const int nh = blockIdx.x / tiles;  // n * Hv + hv
+  const int dv0 = (blockIdx.x - nh * tiles) * 128;
+  const int n = nh / p.Hv;
+  const int hv = nh - n * p.Hv;
+  const int hk = hv / (p.Hv / p.Hk);
+  const int cols = min(128, p.Dv - dv0);  // value rows of this CTA
+  size_t first;
+  int len;
+  sequence_range(p, n, &first, &len);
+  zero_gap_rows(p, n, hv, dv0, cols);
+  const int chunks = (len + CH - 1) / CH;
+  const size_t state_off = ((size_t)nh * p.Dv + dv0) * DK;
+  if (chunks == 0) {
+    if (p.state_in != p.state_out)
+      for (int i = threadIdx.x; i < cols * DK / 4; i += C_THREADS)
+        reinterpret_cast<float4*>(p.state_out + state_off)[i] =
+            reinterpret_cast<const float4*>(p.state_in + state_off)[i];
+    return;
+  }
+
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t smem_base = smem_u32(smem);
+  float* small = reinterpret_cast<float*>(smem + C::SMALL_OFF);
+  // g and beta of a stage; c_i and D_63,i of a prepared chunk
+  auto g_of = [&](int s) { return small + s * 2 * CH; };
+  auto b_of = [&](int s) { return small + s * 2 * CH + CH; };
+  auto cum_of = [&](int s) { return small + C_STAGES * 2 * CH + s * 2 * CH; };
+  auto until_of = [&](int s) { return small + C_STAGES * 2 * CH + s * 2 * CH + CH; };
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C_STAGES; ++s) {
+      mbar_init(&bars.full[s], C_PREP);
+      mbar_init(&bars.freed[s], 1 + C_STATE / 32);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars.tp_full[s], C_PREP);
+      mbar_init(&bars.tp_freed[s], 1 + C_STATE / 32);
+    }
+    mbar_init(&bars.g_full, 1);
+    mbar_init(&bars.g_read, C_PREP);
+    mbar_init(&bars.s_ready, C_STATE);
+    mbar_init(&bars.d1_done, 1);
+    mbar_init(&bars.r_ready, C_STATE);
+    mbar_init(&bars.d3_done, 1);
+    mbar_init(&bars.delta_ready, C_STATE);
+    mbar_init(&bars.d4_done, 1);
+    mbar_init(&bars.y_done, 1);
+    mbar_init(&bars.y_read, C_STATE);
+    abort_word = 0;
+    fence_barrier_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(&tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  auto wait = [&](uint64_t* bar, int parity) { mbar_wait_abortable(bar, uint32_t(parity & 1), &abort_word); };
+
+  if (warp < 4) {
+    // ------------------------------------------------ loads and preparation
+    const int t = threadIdx.x;
+    float g_next = 1.f, b_next = 0.f;
+    auto load = [&](int c) {
+      const int s = c % C_STAGES;
+      const uint32_t kq = smem_base + s * C::STAGE_BYTES, vt = kq + C::KQ_BYTES;
+      const size_t tok0 = first + (size_t)c * CH;
+      const int rows = min(CH, len - c * CH);
+      constexpr int PER_ROW = DK / 8;
+      for (int i = t; i < CH * PER_ROW; i += C_PREP) {
+        const int r = i / PER_ROW, x = i % PER_ROW;
+        const bool on = r < rows && (!p.mask || p.mask[tok0 + r] != 0);
+        const size_t tok = on ? tok0 + r : first;
+        const uint32_t dst = kq + (x / 8) * C::ATOM + r * 128 + (((x % 8) ^ (r & 7)) * 16);
+        cp_async_16(dst, p.k + tok * p.ldk + (size_t)hk * DK + x * 8, on ? 16 : 0);
+        cp_async_16(dst + 64 * 128, p.q + tok * p.ldq + (size_t)hk * DK + x * 8, on ? 16 : 0);
+      }
+      for (int i = t; i < CH * 16; i += C_PREP) {
+        const int r = i / 16, x = i % 16;
+        const bool on = r < rows && x * 8 < cols && (!p.mask || p.mask[tok0 + r] != 0);
+        const __nv_bfloat16* src = on ? p.v + (tok0 + r) * p.ldv + (size_t)hv * p.Dv + dv0 + x * 8 : p.v;
+        cp_async_16(vt + r * 256 + x * 16, src, on ? 16 : 0);
+      }
+      cp_async_commit();
+      g_next = 1.f;
+      b_next = 0.f;
+      if (t < rows && (!p.mask || p.mask[tok0 + t] != 0)) {
+        g_next = p.g[(tok0 + t) * p.Hv + hv];
+        b_next = p.beta[(tok0 + t) * p.Hv + hv];
+      }
+    };
+    // the newest load's g and beta become visible with its tiles
+    auto publish = [&](int c, float gv, float bv) {
+      const int s = c % C_STAGES;
+      if (t < CH) {
+        g_of(s)[t] = gv;
+        b_of(s)[t] = bv;
+      }
+      fence_proxy_async_shared();
+      mbar_arrive(&bars.full[s]);
+    };
+    load(0);
+    cp_async_wait_all();
+    publish(0, g_next, b_next);
+    if (chunks > 1) load(1);
+    for (int c = 0; c < chunks; ++c) {
+      const int s = c % C_STAGES, ts = c % 2;
+      const int i = t & 63;       // this thread's step: row of K K^T (t < 64) or of Q K^T
+      wait(&bars.g_full, c);
+      tc_fence_after();
+      uint32_t gr[2][32];
+      const uint32_t gaddr = tmem + (uint32_t(warp * 32) << 16) + C::COL_G;
+      tmem_ld_32x32b_x32(gaddr, gr[0]);
+      tmem_ld_32x32b_x32(gaddr + 32, gr[1]);
+      tmem_ld_wait();
+      tc_fence_before();
+      mbar_arrive(&bars.g_read);
+      if (c >= 2) wait(&bars.tp_freed[ts], (c / 2) - 1);
+      // all threads' g and beta of this stage were published before g_full
+      const float* gs = g_of(s);
+      const float beta = b_of(s)[i];
+      uint8_t* tp = smem + C::TP_OFF + ts * C::TP_BYTES;
+      float* am = reinterpret_cast<float*>(tp);
+      float d = 0.f;
+#pragma unroll
+      for (int j4 = CH - 4; j4 >= 0; j4 -= 4) {
+        float o[4];
+#pragma unroll
+        for (int e = 3; e >= 0; --e) {
+          const int j = j4 + e;
+          const float next = j + 1 < CH ? gs[(j + 1) & 63] : 1.f;
+          d = j == i ? 1.f : (j < i ? d * next : 0.f);
+          if (t == 63) until_of(ts)[j] = d;
+          const float x = __uint_as_float(gr[j / 32][j % 32]);
+          o[e] = t < 64 ? (j < i ? beta * (d * x) : 0.f) : (j <= i ? d * x : 0.f);
+        }
+        if (t < 64) {
+          *reinterpret_cast<float4*>(am + i * CH + j4) = make_float4(o[0], o[1], o[2], o[3]);
+        } else {
+          // parts of P: 8-byte halves of the row's 16-byte pieces
+          uint32_t h0 = take_part(o[0], o[1]), h1 = take_part(o[2], o[3]);
+          const int at = i * 128 + (((j4 / 8) ^ (i & 7)) * 16) + (j4 % 8) * 2;
+          *reinterpret_cast<uint2*>(tp + 2 * CH * 128 + at) = make_uint2(h0, h1);
+          h0 = take_part(o[0], o[1]);
+          h1 = take_part(o[2], o[3]);
+          *reinterpret_cast<uint2*>(tp + 3 * CH * 128 + at) = make_uint2(h0, h1);
+        }
+      }
+      if (t < 64) cum_of(ts)[i] = d * gs[0];
+      named_bar_sync(1, C_PREP);
+      invert_unit_lower(am, t);
+      // T - I in two parts over the same memory: half a row per thread
+      {
+        const int r = t / 2, c0 = (t % 2) * 32;
+        float x[32];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float4 y = *reinterpret_cast<const float4*>(am + r * CH + c0 + 4 * q);
+          x[4 * q] = y.x; x[4 * q + 1] = y.y; x[4 * q + 2] = y.z; x[4 * q + 3] = y.w;
+        }
+#pragma unroll
+        for (int q = 0; q < 32; ++q) x[q] = c0 + q < r ? x[q] : 0.f;
+        named_bar_sync(1, C_PREP);
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint4 u;
+            u.x = take_part(x[8 * q], x[8 * q + 1]);
+            u.y = take_part(x[8 * q + 2], x[8 * q + 3]);
+            u.z = take_part(x[8 * q + 4], x[8 * q + 5]);
+            u.w = take_part(x[8 * q + 6], x[8 * q + 7]);
+            *reinterpret_cast<uint4*>(tp + part * CH * 128 + r * 128 + (((c0 / 8 + q) ^ (r & 7)) * 16)) = u;
+          }
+      }
+      fence_proxy_async_shared();
+      mbar_arrive(&bars.tp_full[ts]);
+      if (c + 1 < chunks) {
+        cp_async_wait_all();
+        publish(c + 1, g_next, b_next);
+      }
+      if (c + 2 < chunks) {
+        if (c >= 1) wait(&bars.freed[(c + 2) % C_STAGES], (c - 1) / C_STAGES);
+        load(c + 2);
+      }
+    }
+  } else if (warp < 12) {
+    // --------------------------------------------------------- the state rows
+    const int h = (warp - 4) / 4;            // which half of the columns
+    const int row = (warp % 4) * 32 + lane;  // TMEM lane, value row dv0 + row
+    const bool live = row < cols;
+    const uint32_t ta = tmem + (uint32_t((warp % 4) * 32) << 16);
+    constexpr int NS = DK / 2;               // state columns of this thread
+    float s[NS];
+    const float* src = p.state_in + state_off + (size_t)row * DK + h * NS;
+#pragma unroll
+    for (int i = 0; i < NS; i += 4) {
+      const float4 x = live ? *reinterpret_cast<const float4*>(src + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+      s[i] = x.x; s[i + 1] = x.y; s[i + 2] = x.z; s[i + 3] = x.w;
+    }
+    store_parts<3>(ta + C::COL_S + h * (NS / 2), C::S_PART, s);
+    tmem_st_wait();
+    tc_fence_before();
+    mbar_arrive(&bars.s_ready);
+    for (int c = 0; c < chunks; ++c) {
+      const int st = c % C_STAGES, ts = c % 2;
+      // R = beta (V - c K S^T)
+      wait(&bars.tp_full[ts], c / 2);
+      wait(&bars.d1_done, c);
+      tc_fence_after();
+      uint32_t d[32];
+      tmem_ld_32x32b_x32(ta + C::COL_D + h * 32, d);
+      const __nv_bfloat16* vt =
+          reinterpret_cast<const __nv_bfloat16*>(smem + st * C::STAGE_BYTES + C::KQ_BYTES) + h * 32 * 128 + row;
+      const float* bs = b_of(st) + h * 32;
+      const float* cs = cum_of(ts) + h * 32;
+      tmem_ld_wait();
+      float r[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        r[j] = bs[j] * (__bfloat162float(vt[j * 128]) - cs[j] * __uint_as_float(d[j]));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.freed[st]);
+      store_parts<2>(ta + C::COL_R + h * 16, 32, r);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&bars.r_ready);
+      // Delta = R + (T - I) R
+      wait(&bars.d3_done, c);
+      tc_fence_after();
+      tmem_ld_32x32b_x32(ta + C::COL_D + h * 32, d);
+      const float* us = until_of(ts) + h * 32;
+      tmem_ld_wait();
+      float w[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        r[j] += __uint_as_float(d[j]);
+        w[j] = us[j] * r[j];
+      }
+      store_parts<3>(ta + C::COL_S + h * 16, 32, w);
+      store_parts<2>(ta + C::COL_R + h * 16, 32, r);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&bars.delta_ready);
+      // S <- c_63 S + Delta K
+      const float keep = cum_of(ts)[CH - 1];
+      wait(&bars.d4_done, c);
+      tc_fence_after();
+#pragma unroll
+      for (int b = 0; b < NS / 32; ++b) {
+        tmem_ld_32x32b_x32(ta + C::COL_D + h * NS + 32 * b, d);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) s[32 * b + j] = __fmaf_rn(keep, s[32 * b + j], __uint_as_float(d[j]));
+      }
+      if (c + 1 < chunks) {
+        store_parts<3>(ta + C::COL_S + h * (NS / 2), C::S_PART, s);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&bars.s_ready);
+      }
+      // Y = c Q S^T + P Delta, while the next chunk's K S^T runs
+      wait(&bars.y_done, c);
+      tc_fence_after();
+      uint32_t e[32];
+      tmem_ld_32x32b_x32(ta + C::COL_SQ + h * 32, d);
+      tmem_ld_32x32b_x32(ta + C::COL_Y + h * 32, e);
+      tmem_ld_wait();
+      tc_fence_before();
+      mbar_arrive(&bars.y_read);
+      const int rows = min(CH, len - c * CH) - h * 32;
+      __nv_bfloat16* out = p.y + ((first + (size_t)c * CH + h * 32) * p.Hv + hv) * p.Dv + dv0 + row;
+      const size_t step = (size_t)p.Hv * p.Dv;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const float y = __fmaf_rn(cs[j], __uint_as_float(d[j]), __uint_as_float(e[j]));
+        if (live && j < rows) out[j * step] = __float2bfloat16_rn(y);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.tp_freed[ts]);
+    }
+    if (live) {
+      float* dst = p.state_out + state_off + (size_t)row * DK + h * NS;
+#pragma unroll
+      for (int i = 0; i < NS; i += 4)
+        *reinterpret_cast<float4*>(dst + i) = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
+    }
+  } else if (lane == 0) {
+    // ------------------------------------------------------------- products
+    constexpr uint32_t ID64 = make_idesc_bf16(128, 64);
+    constexpr uint32_t IDK = make_idesc_bf16(128, DK) | kIdescBTransposed;
+    auto kq_desc = [&](int s, int row, int k) {   // 16 columns from 16 k on
+      return make_sw128_desc(smem_base + s * C::STAGE_BYTES + (k / 4) * C::ATOM + row * 128 + (k % 4) * 32);
+    };
+    auto grams = [&](int c) {   // [K; Q] K^T
+      const int s = c % C_STAGES;
+      wait(&bars.full[s], c / C_STAGES);
+      for (int k = 0; k < DK / 16; ++k)
+        mma_bf16_ss(tmem + C::COL_G, kq_desc(s, 0, k), kq_desc(s, 0, k), ID64, k > 0);
+      tc_commit(&bars.g_full);
+    };
+    grams(0);
+    for (int c = 0; c < chunks; ++c) {
+      const int s = c % C_STAGES, ts = c % 2;
+      const uint32_t tp = smem_base + C::TP_OFF + ts * C::TP_BYTES;
+      wait(&bars.s_ready, c);
+      if (c == 0) wait(&bars.g_read, 0);
+      tc_fence_after();
+      for (int part = 0; part < 3; ++part)
+        for (int k = 0; k < DK / 16; ++k)
+          mma_bf16_ts(tmem + C::COL_D, tmem + C::COL_S + part * C::S_PART + k * 8, kq_desc(s, 0, k), ID64,
+                      part + k > 0);
+      tc_commit(&bars.d1_done);
+      if (c > 0) {
+        wait(&bars.y_read, c - 1);
+        tc_fence_after();
+      }
+      for (int part = 0; part < 2; ++part)
+        for (int k = 0; k < DK / 16; ++k)
+          mma_bf16_ts(tmem + C::COL_SQ, tmem + C::COL_S + part * C::S_PART + k * 8, kq_desc(s, 64, k), ID64,
+                      part + k > 0);
+      wait(&bars.tp_full[ts], c / 2);
+      wait(&bars.r_ready, c);
+      tc_fence_after();
+      // first parts, then second part x first part both ways round
+      for (int m = 0; m < 3; ++m)
+        for (int k = 0; k < CH / 16; ++k)
+          mma_bf16_ts(tmem + C::COL_D, tmem + C::COL_R + (m == 1 ? 32 : 0) + k * 8,
+                      make_sw128_desc(tp + (m == 2 ? CH * 128 : 0) + k * 32), ID64, m + k > 0);
+      tc_commit(&bars.d3_done);
+      if (c + 1 < chunks) grams(c + 1);
+      wait(&bars.delta_ready, c);
+      if (c + 1 < chunks) wait(&bars.g_read, c + 1);
+      tc_fence_after();
+      for (int part = 0; part < 3; ++part)
+        for (int k = 0; k < CH / 16; ++k)
+          mma_bf16_ts(tmem + C::COL_D, tmem + C::COL_S + part * 32 + k * 8,
+                      make_sw128_mn_desc(smem_base + s * C::STAGE_BYTES + k * 16 * 128, C::ATOM), IDK,
+                      part + k > 0);
+      tc_commit(&bars.d4_done);
+      tc_commit(&bars.freed[s]);
+      for (int m = 0; m < 3; ++m)
+        for (int k = 0; k < CH / 16; ++k)
+          mma_bf16_ts(tmem + C::COL_Y, tmem + C::COL_R + (m == 1 ? 32 : 0) + k * 8,
+                      make_sw128_desc(tp + (m == 2 ? 3 : 2) * CH * 128 + k * 32), ID64, m + k > 0);
+      tc_commit(&bars.y_done);
+      tc_commit(&bars.tp_freed[ts]);
+    }
+    // every commit's arrival has landed before the CTA gives its memory back
+    wait(&bars.y_done, chunks - 1);
+    for (int c = max(0, chunks - 2); c < chunks; ++c) wait(&bars.tp_freed[c % 2], c / 2);
+    for (int c = max(0, chunks - C_STAGES); c < chunks; ++c) wait(&bars.freed[c % C_STAGES], c / C_STAGES);
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+template <int DK>
+int launch_chunked(const RuleParams& p, cudaStream_t stream) {
+  static std::atomic<uint64_t> done{0};
+  const long long grid = (long long)p.B * p.Hv * ((p.Dv + 127) / 128);
+  if (grid > 0x7fffffffll) return DFL_ERR_BAD_SHAPE;
+  int dev, sms;
+  int st = host::current_device(&dev, &sms);
+  if (st != DFL_OK) return st;
+  st = host::ensure_smem(gdn_rule_chunked<DK>, CCfg<DK>::SMEM_BYTES, dev, done);
+  if (st != DFL_OK) return st;
+  gdn_rule_chunked<DK><<<int(grid), C_THREADS, CCfg<DK>::SMEM_BYTES, stream>>>(p);
+  return host::launch_status();
+}
+
 // Checks shared by the two forms; fills *p.  *done: nothing to launch.
 inline int rule_params(const uint16_t* q, int ldq, const uint16_t* k, int ldk, const uint16_t* v, int ldv,
                        const float* g, int g_vec, const float* beta, const uint8_t* mask,
@@ -280,4 +846,24 @@ extern "C" int dfl_gdn_rule_recurrent(const uint16_t* q, int ldq, const uint16_t
     case 128: return gdnr::launch_recurrent<128>(p, s);
     default: return gdnr::launch_recurrent<256>(p, s);
   }
+}
+
+extern "C" int dfl_gdn_rule_chunked(const uint16_t* q, int ldq, const uint16_t* k, int ldk, const uint16_t* v,
+                                    int ldv, const float* g, const float* beta, const uint8_t* mask,
+                                    const int32_t* cu_seqlens, const float* state_in, float* state_out,
+                                    uint16_t* y, int zero_gaps, int B, int T, int Hv, int Hk, int Dv, int Dk,
+                                    void* stream) {
+  using namespace dfl;
+  gdnr::RuleParams p;
+  bool done;
+  const int st = gdnr::rule_params(q, ldq, k, ldk, v, ldv, g, 0, beta, mask, cu_seqlens, state_in, state_out, y,
+                                   zero_gaps, B, T, Hv, Hk, Dv, Dk, &p, &done);
+  if (st != DFL_OK || done) return st;
+  if (Dk != 64 && Dk != 128) return DFL_ERR_BAD_SHAPE;
+  // 16-byte copies: tokens and heads on 16-byte borders
+  if (ldq % 8 != 0 || ldk % 8 != 0 || ldv % 8 != 0 || !host::aligned(q, 16) || !host::aligned(k, 16) ||
+      !host::aligned(v, 16))
+    return DFL_ERR_MISALIGNED;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return Dk == 64 ? gdnr::launch_chunked<64>(p, s) : gdnr::launch_chunked<128>(p, s);
 }

@@ -258,14 +258,27 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     k, ldk = _token_rows(k)
     v, ldv = _token_rows(v)
     g, beta = g.contiguous(), beta.contiguous()
+    mask_ptr = None if mask is None else mask.data_ptr()
+    cu_ptr = None if cu_seqlens is None else cu_seqlens.data_ptr()
+    steps = t_steps if cu_seqlens is None else t_steps // max(seqs, 1)
+    # bytes that both entries address alike: q, k, v rows, then the rest
+    head = (q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, g.data_ptr())
+    tail = (beta.data_ptr(), mask_ptr, cu_ptr, state.data_ptr(), out_state.data_ptr(), out.data_ptr(),
+            1 if zero_gaps else 0, seqs, t_steps, hv, hk, dv, dk)
     with torch.cuda.device(dev):
-        st = _lib.load().dfl_gdn_rule_recurrent(
-            q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, g.data_ptr(),
-            1 if g.dim() == 4 else 0, beta.data_ptr(), None if mask is None else mask.data_ptr(),
-            None if cu_seqlens is None else cu_seqlens.data_ptr(), state.data_ptr(), out_state.data_ptr(),
-            out.data_ptr(), 1 if zero_gaps else 0, seqs, t_steps, hv, hk, dv, dk, stream_ptr(dev))
-    _lib.check("dfl_gdn_rule_recurrent", st)
+        if g.dim() == 3 and dk in (64, 128) and steps >= _CHUNKED_STEPS:
+            entry = "dfl_gdn_rule_chunked"
+            st = _lib.load().dfl_gdn_rule_chunked(*head, *tail, stream_ptr(dev))
+        else:
+            entry = "dfl_gdn_rule_recurrent"
+            st = _lib.load().dfl_gdn_rule_recurrent(*head, 1 if g.dim() == 4 else 0, *tail, stream_ptr(dev))
+    _lib.check(entry, st)
     return out, out_state
+
+
+#: Mean steps per sequence from which 64 steps at a time are faster than one
+#: after the other.
+_CHUNKED_STEPS = 16
 
 
 def _aligned(x: torch.Tensor) -> torch.Tensor:

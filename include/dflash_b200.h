@@ -337,6 +337,10 @@ int dfl_gdn_forward_tape(const uint16_t* q, const uint16_t* k, const uint16_t* v
  *   y      bf16 [tokens, Hv, Dv], 16-byte aligned
  * Constraints: Dk in {32, 64, 128, 256}, Dv % 32 == 0, Hv % Hk == 0.
  * dfl_gdn_rule_recurrent takes one step after the other (fp32 throughout).
+ * dfl_gdn_rule_chunked takes 64 steps at a time as products on the tensor
+ * cores (same results up to the order of fp32 sums; Dk 64 or 128, one decay
+ * per head, keys of about unit length as for any use of the rule; q, k and v
+ * 16-byte aligned, ldq, ldk and ldv multiples of 8).
  * The reference reaches this step, for caches that record no tape, through
  * mlx-lm's gated_delta_update (third party) from the hook at
  * dflash_mlx/engine/target_qwen_gdn.py:551-651. */
@@ -345,6 +349,10 @@ int dfl_gdn_rule_recurrent(const uint16_t* q, int ldq, const uint16_t* k, int ld
                            const uint8_t* mask, const int32_t* cu_seqlens, const float* state_in,
                            float* state_out, uint16_t* y, int zero_gaps, int B, int T, int Hv, int Hk,
                            int Dv, int Dk, void* stream);
+int dfl_gdn_rule_chunked(const uint16_t* q, int ldq, const uint16_t* k, int ldk, const uint16_t* v,
+                         int ldv, const float* g, const float* beta, const uint8_t* mask,
+                         const int32_t* cu_seqlens, const float* state_in, float* state_out, uint16_t* y,
+                         int zero_gaps, int B, int T, int Hv, int Hk, int Dv, int Dk, void* stream);
 
 /* ------------------------------------------------------------------------
  * DDTree verify: the GDN recurrence over a token tree.

@@ -15,10 +15,8 @@ def _rule(lib, **kw):
     a = dict(q=P, ldq=256, k=P, ldk=256, v=P, ldv=512, g=P, gv=0, beta=P, mask=None, cu=None, s=P, so=P, y=P,
              zero=1, B=2, T=4, Hv=4, Hk=2, Dv=128, Dk=128)
     a.update(kw)
-    return [getattr(lib, name)(*a.values(), None) for name in ENTRIES]
-
-
-ENTRIES = ["dfl_gdn_rule_recurrent"]
+    chunked = {k: x for k, x in a.items() if k != "gv"}
+    return [lib.dfl_gdn_rule_recurrent(*a.values(), None), lib.dfl_gdn_rule_chunked(*chunked.values(), None)]
 
 
 @pytest.mark.parametrize("kw,status", [
@@ -33,6 +31,16 @@ def test_gated_delta_rule(pkg, kw, status):
     from dflash_mlx_b200 import _lib
 
     assert set(_rule(_lib.load(), **kw)) == {status}
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(Dk=256, ldq=512, ldk=512), 2), (dict(Dk=32), 2), (dict(ldq=257), 3), (dict(ldk=260), 3), (dict(ldv=513), 3),
+    (dict(q=ODD), 3), (dict(k=ODD), 3), (dict(v=ODD), 3),
+])
+def test_chunked_form_alone(pkg, kw, status):
+    from dflash_mlx_b200 import _lib
+
+    assert _rule(_lib.load(), **kw)[1] == status
 
 
 def _sampled(lib, **kw):
