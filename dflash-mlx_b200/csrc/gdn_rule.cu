@@ -234,20 +234,22 @@ int launch_recurrent(const RuleParams& p, cudaStream_t stream) {
 // products from TMEM, and only K, Q, T and P are read from shared memory, K
 // both as it is and transposed from the same tile.
 //
-// fp32 in bf16 products: K and Q are bf16 already.  The state and the update
+// fp32 in bf16 products: K and Q are bf16 already.  The state, R and the update
 // go in as three bf16 parts (24 bits), so what is carried from chunk to chunk
-// keeps 32-bit accuracy; R, T - I, P, and the state's and Delta's share of y
-// as two parts each (16 bits, without the product of the two second parts):
-// they are corrections to R that is added in fp32, or end in y's 8 bits.
+// keeps 32-bit accuracy; T as two (its unit diagonal is exact, what lies below
+// it is a correction), P, and the state's and Delta's share of y, which ends in
+// 8 bits, as two, each without the product of the two second parts.
 //
-// Warps: 0-3 load a stage ahead (cp.async, zeros for masked steps and behind
-// the end) and prepare T and P of the next chunk (K K^T and Q K^T from one
-// product, inverse by blocks of 16, 32 and 64 in fp32); 4-11 (two threads per
-// value row, half the columns each) carry the state; 12 issues the products.
+// Warps: 0-3 prepare T and P of the next chunk (K K^T and Q K^T from one
+// product, inverse by blocks of 16, 32 and 64 in fp32) and put zeros over rows
+// of masked steps and behind the end; 4-11 (two threads per value row, half the
+// columns each) carry the state; 12 loads (TMA, two chunks ahead) and issues
+// the products.
 constexpr int CH = 64;               // steps of a chunk
 constexpr int C_THREADS = 13 * 32;
 constexpr int C_STAGES = 3;
 constexpr int C_PREP = 128, C_STATE = 256;
+constexpr int INV_LD = CH + 4;       // floats of a row of the inverse (no bank conflicts between rows)
 
 template <int DK>
 struct CCfg {
@@ -255,149 +257,160 @@ struct CCfg {
   static constexpr int KQ_BYTES = (DK / 64) * ATOM;
   static constexpr int V_BYTES = CH * 256;               // 64 rows x 128 columns
   static constexpr int STAGE_BYTES = KQ_BYTES + V_BYTES;
-  static constexpr int TP_BYTES = 4 * CH * 128;          // T and P, two parts each
+  static constexpr int T_BYTES = INV_LD * CH * 4;        // fp32 inverse, then T's two parts
+  static constexpr int TP_BYTES = T_BYTES + 2 * CH * 128;  // ... and P's
   static constexpr int TP_OFF = C_STAGES * STAGE_BYTES;
   static constexpr int SMALL_OFF = TP_OFF + 2 * TP_BYTES;
-  static constexpr int SMALL_BYTES = (C_STAGES * 2 + 2 * 2) * CH * 4 + 256;
+  static constexpr int SMALL_BYTES = (C_STAGES * 2 + 2 * 2) * CH * 4;
   static constexpr int SMEM_BYTES = SMALL_OFF + SMALL_BYTES + 1024;
+  static_assert(T_BYTES % 1024 == 0 && T_BYTES >= 2 * CH * 128, "P's parts start on a swizzle atom");
   // TMEM columns
   static constexpr int S_PART = DK / 2;                  // columns of one part of the state
   static constexpr int COL_S = 0;                        // state parts; later Delta K's three parts
   static constexpr int COL_D = 192;                      // S K^T, then R T^T, then Delta K
   static constexpr int COL_G = 256;                      // [K; Q] K^T, over Delta K's second half
+  static constexpr int COL_R3 = 256;                     // R's third part, before the next [K; Q] K^T
   static constexpr int COL_SQ = 320;                     // S Q^T
-  static constexpr int COL_R = 384;                      // R's parts, then Delta's
+  static constexpr int COL_R = 384;                      // R's first parts, then Delta's
   static constexpr int COL_Y = 448;                      // Delta P^T
 };
 
-// The bf16 parts of two values, leading part returned, the rest left in a, b.
+// The leading bf16 parts of two values; what they leave stays in a, b (exact).
 __device__ __forceinline__ uint32_t take_part(float& a, float& b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   const uint32_t u = *reinterpret_cast<const uint32_t*>(&h);
-  a -= __uint_as_float(u << 16);
-  b -= __uint_as_float(u & 0xffff0000u);
+  asm("{\n\t.reg .b64 x, y, m;\n\t"
+      "mov.b64 x, {%2, %3};\n\t"
+      "mov.b64 y, {%0, %1};\n\t"
+      "mov.b64 m, 0xbf800000bf800000;\n\t"
+      "fma.rn.f32x2 y, x, m, y;\n\t"
+      "mov.b64 {%0, %1}, y;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(__uint_as_float(u << 16)), "f"(__uint_as_float(u & 0xffff0000u)));
   return u;
 }
 
-// X parts of a row (n values) into TMEM columns col + part * stride.
-template <int PARTS, int N>
-__device__ __forceinline__ void store_parts(uint32_t taddr, int stride, const float (&x)[N]) {
-  static_assert(N % 32 == 0, "32 values, 16 columns at a time");
+// The parts of 16 values into 8 TMEM columns each, at the given addresses.
+template <int PARTS>
+__device__ __forceinline__ void store_parts(const uint32_t (&taddr)[PARTS], float (&x)[16]) {
 #pragma unroll
-  for (int h = 0; h < N / 32; ++h) {
-    float r[32];
+  for (int p = 0; p < PARTS; ++p) {
+    uint32_t u[8];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) r[i] = x[32 * h + i];
-#pragma unroll
-    for (int p = 0; p < PARTS; ++p) {
-      uint32_t u[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) u[i] = take_part(r[2 * i], r[2 * i + 1]);
-      tmem_st_32x32b_x16(taddr + p * stride + 16 * h, u);
-    }
+    for (int i = 0; i < 8; ++i) u[i] = take_part(x[2 * i], x[2 * i + 1]);
+    tmem_st_32x32b_x8(taddr[p], u);
   }
 }
 
 struct ChunkBars {
-  uint64_t full[C_STAGES], freed[C_STAGES];
+  uint64_t loaded[C_STAGES], full[C_STAGES];
   uint64_t tp_full[2], tp_freed[2];
   uint64_t g_full, g_read;
   uint64_t s_ready, d1_done, r_ready, d3_done, delta_ready, d4_done, y_done, y_read;
 };
 
-// Unit lower triangular inverse of I + A in place, A 64 x 64 (strictly lower
-// part used), by the 128 preparing threads: diagonal blocks of 16 by forward
-// substitution, then T21 = -T22 (A21 T11) for blocks of 16 and of 32.
-__device__ __forceinline__ void invert_unit_lower(float* a, int t) {
-  if (t < 64) {
-    float* blk = a + (t / 16) * 16 * (CH + 1);
-    const int c = t % 16;
-    float x[16];
+// m += x . y over four j: x a row's four values, y rows j .. j + 3 at column c
+__device__ __forceinline__ void fma_4x4(float4& m, const float4& x, const float4& y0, const float4& y1,
+                                        const float4& y2, const float4& y3) {
+  m.x = __fmaf_rn(x.x, y0.x, m.x); m.y = __fmaf_rn(x.x, y0.y, m.y);
+  m.z = __fmaf_rn(x.x, y0.z, m.z); m.w = __fmaf_rn(x.x, y0.w, m.w);
+  m.x = __fmaf_rn(x.y, y1.x, m.x); m.y = __fmaf_rn(x.y, y1.y, m.y);
+  m.z = __fmaf_rn(x.y, y1.z, m.z); m.w = __fmaf_rn(x.y, y1.w, m.w);
+  m.x = __fmaf_rn(x.z, y2.x, m.x); m.y = __fmaf_rn(x.z, y2.y, m.y);
+  m.z = __fmaf_rn(x.z, y2.z, m.z); m.w = __fmaf_rn(x.z, y2.w, m.w);
+  m.x = __fmaf_rn(x.w, y3.x, m.x); m.y = __fmaf_rn(x.w, y3.y, m.y);
+  m.z = __fmaf_rn(x.w, y3.z, m.z); m.w = __fmaf_rn(x.w, y3.w, m.w);
+}
+
+__device__ __forceinline__ float4 at4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+
+__device__ __forceinline__ float4 neg4(const float4& x) { return make_float4(-x.x, -x.y, -x.z, -x.w); }
+
+// Inverse of the diagonal block of 16 rows of a unit lower triangular matrix
+// (strictly lower part used) by forward substitution, column c per lane, 16
+// lanes of one warp a block.
+__device__ __forceinline__ void invert_block16(float* blk, int c) {
+  float x[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float s0 = i == c ? 1.f : 0.f, s1 = 0.f;
+  for (int i = 0; i < 16; ++i) {
+    float s0 = i == c ? 1.f : 0.f, s1 = 0.f;
 #pragma unroll
-      for (int j = 0; j < i; ++j) {
-        const float m = blk[i * CH + j];
-        if (j & 1) s1 = __fmaf_rn(-m, x[j], s1);
-        else s0 = __fmaf_rn(-m, x[j], s0);
-      }
-      x[i] = s0 + s1;
+    for (int j = 0; j < i; j += 4) {
+      const float4 m = at4(blk + i * INV_LD + j);
+      s0 = __fmaf_rn(-m.x, x[j], s0);
+      if (j + 1 < i) s1 = __fmaf_rn(-m.y, x[j + 1], s1);
+      if (j + 2 < i) s0 = __fmaf_rn(-m.z, x[j + 2], s0);
+      if (j + 3 < i) s1 = __fmaf_rn(-m.w, x[j + 3], s1);
     }
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) blk[i * CH + c] = x[i];
+    x[i] = s0 + s1;
   }
-  named_bar_sync(1, C_PREP);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) blk[i * INV_LD + c] = x[i];
+}
+
+// The rest of the 64 x 64 inverse from its diagonal blocks, by the 128
+// preparing threads: T21 = -T22 (A21 T11) for blocks of 16, then of 32.
+__device__ __forceinline__ void invert_join(float* a, int t) {
+  constexpr int L = INV_LD;
   {
-    // two pairs of blocks of 16: 4 columns of one row per thread
-    const int pr = t / 64, i = (t % 64) / 4, c = (t % 4) * 4;
-    float* t11 = a + pr * 32 * (CH + 1);
-    float* a21 = t11 + 16 * CH;
-    const float* t22 = t11 + 16 * (CH + 1);
+    const int pr = t / 64, i = (t % 64) / 4, c = (t % 4) * 4;   // 4 columns of one row
+    float* t11 = a + pr * 32 * (L + 1);
+    float* a21 = t11 + 16 * L;
+    const float* t22 = t11 + 16 * (L + 1);
     float4 m = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float x = a21[i * CH + j];
-      const float4 y = *reinterpret_cast<const float4*>(t11 + j * CH + c);
-      m.x = __fmaf_rn(x, y.x, m.x); m.y = __fmaf_rn(x, y.y, m.y);
-      m.z = __fmaf_rn(x, y.z, m.z); m.w = __fmaf_rn(x, y.w, m.w);
-    }
+    for (int j = 0; j < 16; j += 4)
+      fma_4x4(m, at4(a21 + i * L + j), at4(t11 + j * L + c), at4(t11 + (j + 1) * L + c),
+              at4(t11 + (j + 2) * L + c), at4(t11 + (j + 3) * L + c));
     named_bar_sync(1, C_PREP);
-    *reinterpret_cast<float4*>(a21 + i * CH + c) = m;
+    *reinterpret_cast<float4*>(a21 + i * L + c) = m;
     named_bar_sync(1, C_PREP);
     m = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float x = t22[i * CH + j];
-      const float4 y = *reinterpret_cast<const float4*>(a21 + j * CH + c);
-      m.x = __fmaf_rn(-x, y.x, m.x); m.y = __fmaf_rn(-x, y.y, m.y);
-      m.z = __fmaf_rn(-x, y.z, m.z); m.w = __fmaf_rn(-x, y.w, m.w);
-    }
+    for (int j = 0; j < 16; j += 4)
+      fma_4x4(m, at4(t22 + i * L + j), at4(a21 + j * L + c), at4(a21 + (j + 1) * L + c),
+              at4(a21 + (j + 2) * L + c), at4(a21 + (j + 3) * L + c));
     named_bar_sync(1, C_PREP);
-    *reinterpret_cast<float4*>(a21 + i * CH + c) = m;
-    // the blocks above the diagonal hold A's zeros
+    *reinterpret_cast<float4*>(a21 + i * L + c) = neg4(m);
     named_bar_sync(1, C_PREP);
   }
   {
-    // one pair of blocks of 32: 4 columns of two rows per thread
-    const int i = (t / 8) * 2, c = (t % 8) * 4;
-    float* a21 = a + 32 * CH;
-    const float* t22 = a + 32 * (CH + 1);
+    const int i = (t / 8) * 2, c = (t % 8) * 4;   // 4 columns of two rows
+    float* a21 = a + 32 * L;
+    const float* t22 = a + 32 * (L + 1);
     float4 m0 = make_float4(0.f, 0.f, 0.f, 0.f), m1 = m0;
-#pragma unroll 8
-    for (int j = 0; j < 32; ++j) {
-      const float x0 = a21[i * CH + j], x1 = a21[(i + 1) * CH + j];
-      const float4 y = *reinterpret_cast<const float4*>(a + j * CH + c);
-      m0.x = __fmaf_rn(x0, y.x, m0.x); m0.y = __fmaf_rn(x0, y.y, m0.y);
-      m0.z = __fmaf_rn(x0, y.z, m0.z); m0.w = __fmaf_rn(x0, y.w, m0.w);
-      m1.x = __fmaf_rn(x1, y.x, m1.x); m1.y = __fmaf_rn(x1, y.y, m1.y);
-      m1.z = __fmaf_rn(x1, y.z, m1.z); m1.w = __fmaf_rn(x1, y.w, m1.w);
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 y0 = at4(a + j * L + c), y1 = at4(a + (j + 1) * L + c), y2 = at4(a + (j + 2) * L + c),
+                   y3 = at4(a + (j + 3) * L + c);
+      fma_4x4(m0, at4(a21 + i * L + j), y0, y1, y2, y3);
+      fma_4x4(m1, at4(a21 + (i + 1) * L + j), y0, y1, y2, y3);
     }
     named_bar_sync(1, C_PREP);
-    *reinterpret_cast<float4*>(a21 + i * CH + c) = m0;
-    *reinterpret_cast<float4*>(a21 + (i + 1) * CH + c) = m1;
+    *reinterpret_cast<float4*>(a21 + i * L + c) = m0;
+    *reinterpret_cast<float4*>(a21 + (i + 1) * L + c) = m1;
     named_bar_sync(1, C_PREP);
     m0 = make_float4(0.f, 0.f, 0.f, 0.f);
     m1 = m0;
-#pragma unroll 8
-    for (int j = 0; j < 32; ++j) {
-      const float x0 = t22[i * CH + j], x1 = t22[(i + 1) * CH + j];
-      const float4 y = *reinterpret_cast<const float4*>(a21 + j * CH + c);
-      m0.x = __fmaf_rn(-x0, y.x, m0.x); m0.y = __fmaf_rn(-x0, y.y, m0.y);
-      m0.z = __fmaf_rn(-x0, y.z, m0.z); m0.w = __fmaf_rn(-x0, y.w, m0.w);
-      m1.x = __fmaf_rn(-x1, y.x, m1.x); m1.y = __fmaf_rn(-x1, y.y, m1.y);
-      m1.z = __fmaf_rn(-x1, y.z, m1.z); m1.w = __fmaf_rn(-x1, y.w, m1.w);
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 y0 = at4(a21 + j * L + c), y1 = at4(a21 + (j + 1) * L + c), y2 = at4(a21 + (j + 2) * L + c),
+                   y3 = at4(a21 + (j + 3) * L + c);
+      fma_4x4(m0, at4(t22 + i * L + j), y0, y1, y2, y3);
+      fma_4x4(m1, at4(t22 + (i + 1) * L + j), y0, y1, y2, y3);
     }
     named_bar_sync(1, C_PREP);
-    *reinterpret_cast<float4*>(a21 + i * CH + c) = m0;
-    *reinterpret_cast<float4*>(a21 + (i + 1) * CH + c) = m1;
+    *reinterpret_cast<float4*>(a21 + i * L + c) = neg4(m0);
+    *reinterpret_cast<float4*>(a21 + (i + 1) * L + c) = neg4(m1);
     named_bar_sync(1, C_PREP);
   }
 }
 
 template <int DK>
-__global__ void __launch_bounds__(C_THREADS, 1) gdn_rule_chunked(const RuleParams p) {
+__global__ void __launch_bounds__(C_THREADS, 1)
+    gdn_rule_chunked(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                     const __grid_constant__ CUtensorMap tm_v, const RuleParams p) {
   using C = CCfg<DK>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ ChunkBars bars;
@@ -437,8 +450,8 @@ __global__ void __launch_bounds__(C_THREADS, 1) gdn_rule_chunked(const RuleParam
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < C_STAGES; ++s) {
+      mbar_init(&bars.loaded[s], 1);
       mbar_init(&bars.full[s], C_PREP);
-      mbar_init(&bars.freed[s], 1 + C_STATE / 32);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bars.tp_full[s], C_PREP);
@@ -468,51 +481,36 @@ __global__ void __launch_bounds__(C_THREADS, 1) gdn_rule_chunked(const RuleParam
   auto wait = [&](uint64_t* bar, int parity) { mbar_wait_abortable(bar, uint32_t(parity & 1), &abort_word); };
 
   if (warp < 4) {
-    // ------------------------------------------------ loads and preparation
+    // ---------------------------------------------------------- preparation
     const int t = threadIdx.x;
-    float g_next = 1.f, b_next = 0.f;
-    auto load = [&](int c) {
+    // Chunk c's tiles have landed: zeros over rows of no step, g and beta (1
+    // and 0 there: a step that changes nothing) beside them.
+    auto publish = [&](int c) {
       const int s = c % C_STAGES;
-      const uint32_t kq = smem_base + s * C::STAGE_BYTES, vt = kq + C::KQ_BYTES;
       const size_t tok0 = first + (size_t)c * CH;
       const int rows = min(CH, len - c * CH);
-      constexpr int PER_ROW = DK / 8;
-      for (int i = t; i < CH * PER_ROW; i += C_PREP) {
-        const int r = i / PER_ROW, x = i % PER_ROW;
-        const bool on = r < rows && (!p.mask || p.mask[tok0 + r] != 0);
-        const size_t tok = on ? tok0 + r : first;
-        const uint32_t dst = kq + (x / 8) * C::ATOM + r * 128 + (((x % 8) ^ (r & 7)) * 16);
-        cp_async_16(dst, p.k + tok * p.ldk + (size_t)hk * DK + x * 8, on ? 16 : 0);
-        cp_async_16(dst + 64 * 128, p.q + tok * p.ldq + (size_t)hk * DK + x * 8, on ? 16 : 0);
+      const int r = t / 2;
+      const bool on = r < rows && (!p.mask || p.mask[tok0 + r] != 0);
+      if (t % 2 == 0) {
+        g_of(s)[r] = on ? p.g[(tok0 + r) * p.Hv + hv] : 1.f;
+        b_of(s)[r] = on ? p.beta[(tok0 + r) * p.Hv + hv] : 0.f;
       }
-      for (int i = t; i < CH * 16; i += C_PREP) {
-        const int r = i / 16, x = i % 16;
-        const bool on = r < rows && x * 8 < cols && (!p.mask || p.mask[tok0 + r] != 0);
-        const __nv_bfloat16* src = on ? p.v + (tok0 + r) * p.ldv + (size_t)hv * p.Dv + dv0 + x * 8 : p.v;
-        cp_async_16(vt + r * 256 + x * 16, src, on ? 16 : 0);
-      }
-      cp_async_commit();
-      g_next = 1.f;
-      b_next = 0.f;
-      if (t < rows && (!p.mask || p.mask[tok0 + t] != 0)) {
-        g_next = p.g[(tok0 + t) * p.Hv + hv];
-        b_next = p.beta[(tok0 + t) * p.Hv + hv];
-      }
-    };
-    // the newest load's g and beta become visible with its tiles
-    auto publish = [&](int c, float gv, float bv) {
-      const int s = c % C_STAGES;
-      if (t < CH) {
-        g_of(s)[t] = gv;
-        b_of(s)[t] = bv;
+      wait(&bars.loaded[s], c / C_STAGES);
+      if (!on) {
+        uint8_t* kq = smem + s * C::STAGE_BYTES;
+        const uint4 z = make_uint4(0, 0, 0, 0);
+        for (int a = 0; a < DK / 64; ++a)
+#pragma unroll
+          for (int x = 0; x < 8; ++x)   // one of the row's K and Q per thread
+            *reinterpret_cast<uint4*>(kq + a * C::ATOM + ((t % 2) * 64 + r) * 128 + x * 16) = z;
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          *reinterpret_cast<uint4*>(kq + C::KQ_BYTES + r * 256 + (t % 2) * 128 + x * 16) = z;
       }
       fence_proxy_async_shared();
       mbar_arrive(&bars.full[s]);
     };
-    load(0);
-    cp_async_wait_all();
-    publish(0, g_next, b_next);
-    if (chunks > 1) load(1);
+    publish(0);
     for (int c = 0; c < chunks; ++c) {
       const int s = c % C_STAGES, ts = c % 2;
       const int i = t & 63;       // this thread's step: row of K K^T (t < 64) or of Q K^T
@@ -526,50 +524,69 @@ __global__ void __launch_bounds__(C_THREADS, 1) gdn_rule_chunked(const RuleParam
       tc_fence_before();
       mbar_arrive(&bars.g_read);
       if (c >= 2) wait(&bars.tp_freed[ts], (c / 2) - 1);
-      // all threads' g and beta of this stage were published before g_full
       const float* gs = g_of(s);
-      const float beta = b_of(s)[i];
       uint8_t* tp = smem + C::TP_OFF + ts * C::TP_BYTES;
       float* am = reinterpret_cast<float*>(tp);
-      float d = 0.f;
+      // D_ij along the row, from the diagonal to the left
+      const float beta = b_of(s)[i];
+      float d = 0.f, next = 1.f;
 #pragma unroll
-      for (int j4 = CH - 4; j4 >= 0; j4 -= 4) {
-        float o[4];
+      for (int j8 = CH - 8; j8 >= 0; j8 -= 8) {
+        const float4 glo = at4(gs + j8), ghi = at4(gs + j8 + 4);
+        const float gg[8] = {glo.x, glo.y, glo.z, glo.w, ghi.x, ghi.y, ghi.z, ghi.w};
+        float o[8];
 #pragma unroll
-        for (int e = 3; e >= 0; --e) {
-          const int j = j4 + e;
-          const float next = j + 1 < CH ? gs[(j + 1) & 63] : 1.f;
-          d = j == i ? 1.f : (j < i ? d * next : 0.f);
-          if (t == 63) until_of(ts)[j] = d;
-          const float x = __uint_as_float(gr[j / 32][j % 32]);
-          o[e] = t < 64 ? (j < i ? beta * (d * x) : 0.f) : (j <= i ? d * x : 0.f);
+        for (int e = 7; e >= 0; --e) {
+          const int j = j8 + e;
+          d = j < i ? d * next : (j == i ? 1.f : 0.f);
+          next = gg[e];
+          const float x = d * __uint_as_float(gr[j / 32][j % 32]);
+          o[e] = t < 64 ? (j < i ? beta * x : 0.f) : (j <= i ? x : 0.f);
         }
         if (t < 64) {
-          *reinterpret_cast<float4*>(am + i * CH + j4) = make_float4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<float4*>(am + i * INV_LD + j8) = make_float4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<float4*>(am + i * INV_LD + j8 + 4) = make_float4(o[4], o[5], o[6], o[7]);
         } else {
-          // parts of P: 8-byte halves of the row's 16-byte pieces
-          uint32_t h0 = take_part(o[0], o[1]), h1 = take_part(o[2], o[3]);
-          const int at = i * 128 + (((j4 / 8) ^ (i & 7)) * 16) + (j4 % 8) * 2;
-          *reinterpret_cast<uint2*>(tp + 2 * CH * 128 + at) = make_uint2(h0, h1);
-          h0 = take_part(o[0], o[1]);
-          h1 = take_part(o[2], o[3]);
-          *reinterpret_cast<uint2*>(tp + 3 * CH * 128 + at) = make_uint2(h0, h1);
+          uint8_t* at = tp + C::T_BYTES + i * 128 + (((j8 / 8) ^ (i & 7)) * 16);
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            uint4 u;
+            u.x = take_part(o[0], o[1]);
+            u.y = take_part(o[2], o[3]);
+            u.z = take_part(o[4], o[5]);
+            u.w = take_part(o[6], o[7]);
+            *reinterpret_cast<uint4*>(at + part * CH * 128) = u;
+          }
         }
       }
-      if (t < 64) cum_of(ts)[i] = d * gs[0];
+      if (t < 64) {
+        cum_of(ts)[i] = d * next;
+        __syncwarp();
+        invert_block16(am + (t / 16) * 16 * (INV_LD + 1), t % 16);
+      } else if (warp == 3) {
+        // D_63,j: products of the decays behind j, two j per lane
+        const float2 gg = *reinterpret_cast<const float2*>(gs + 2 * lane);
+        float x = gg.x * gg.y;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+          const float y = __shfl_down_sync(0xffffffffu, x, o);
+          if (lane + o < 32) x *= y;
+        }
+        x = __shfl_down_sync(0xffffffffu, x, 1);
+        if (lane == 31) x = 1.f;
+        *reinterpret_cast<float2*>(until_of(ts) + 2 * lane) = make_float2(x * gg.y, x);
+      }
       named_bar_sync(1, C_PREP);
-      invert_unit_lower(am, t);
-      // T - I in two parts over the same memory: half a row per thread
+      invert_join(am, t);
+      // T in two parts over the same memory: half a row per thread
       {
         const int r = t / 2, c0 = (t % 2) * 32;
         float x[32];
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-          const float4 y = *reinterpret_cast<const float4*>(am + r * CH + c0 + 4 * q);
+          const float4 y = at4(am + r * INV_LD + c0 + 4 * q);
           x[4 * q] = y.x; x[4 * q + 1] = y.y; x[4 * q + 2] = y.z; x[4 * q + 3] = y.w;
         }
-#pragma unroll
-        for (int q = 0; q < 32; ++q) x[q] = c0 + q < r ? x[q] : 0.f;
         named_bar_sync(1, C_PREP);
 #pragma unroll
         for (int part = 0; part < 2; ++part)
@@ -585,14 +602,7 @@ __global__ void __launch_bounds__(C_THREADS, 1) gdn_rule_chunked(const RuleParam
       }
       fence_proxy_async_shared();
       mbar_arrive(&bars.tp_full[ts]);
-      if (c + 1 < chunks) {
-        cp_async_wait_all();
-        publish(c + 1, g_next, b_next);
-      }
-      if (c + 2 < chunks) {
-        if (c >= 1) wait(&bars.freed[(c + 2) % C_STAGES], (c - 1) / C_STAGES);
-        load(c + 2);
-      }
+      if (c + 1 < chunks) publish(c + 1);
     }
   } else if (warp < 12) {
     // --------------------------------------------------------- the state rows
@@ -605,50 +615,69 @@ __global__ void __launch_bounds__(C_THREADS, 1) gdn_rule_chunked(const RuleParam
     const float* src = p.state_in + state_off + (size_t)row * DK + h * NS;
 #pragma unroll
     for (int i = 0; i < NS; i += 4) {
-      const float4 x = live ? *reinterpret_cast<const float4*>(src + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 x = live ? at4(src + i) : make_float4(0.f, 0.f, 0.f, 0.f);
       s[i] = x.x; s[i + 1] = x.y; s[i + 2] = x.z; s[i + 3] = x.w;
     }
-    store_parts<3>(ta + C::COL_S + h * (NS / 2), C::S_PART, s);
+    const uint32_t s_col = ta + C::COL_S + h * (NS / 2);
+    auto store_state = [&](int b) {          // columns 16 b .. 16 b + 15 of this thread
+      float x[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = s[16 * b + j];
+      store_parts<3>({s_col + 8 * b, s_col + C::S_PART + 8 * b, s_col + 2 * C::S_PART + 8 * b}, x);
+    };
+#pragma unroll
+    for (int b = 0; b < NS / 16; ++b) store_state(b);
     tmem_st_wait();
     tc_fence_before();
     mbar_arrive(&bars.s_ready);
+    const size_t y_step = (size_t)p.Hv * p.Dv;
+    __nv_bfloat16* out = p.y + ((first + h * 32) * p.Hv + hv) * p.Dv + dv0 + row;
     for (int c = 0; c < chunks; ++c) {
       const int st = c % C_STAGES, ts = c % 2;
+      uint32_t d[2][16];
       // R = beta (V - c K S^T)
       wait(&bars.tp_full[ts], c / 2);
-      wait(&bars.d1_done, c);
-      tc_fence_after();
-      uint32_t d[32];
-      tmem_ld_32x32b_x32(ta + C::COL_D + h * 32, d);
       const __nv_bfloat16* vt =
           reinterpret_cast<const __nv_bfloat16*>(smem + st * C::STAGE_BYTES + C::KQ_BYTES) + h * 32 * 128 + row;
       const float* bs = b_of(st) + h * 32;
       const float* cs = cum_of(ts) + h * 32;
-      tmem_ld_wait();
-      float r[32];
+      const float* us = until_of(ts) + h * 32;
+      wait(&bars.d1_done, c);
+      tc_fence_after();
+      tmem_ld_32x32b_x16(ta + C::COL_D + h * 32, d[0]);
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        r[j] = bs[j] * (__bfloat162float(vt[j * 128]) - cs[j] * __uint_as_float(d[j]));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.freed[st]);
-      store_parts<2>(ta + C::COL_R + h * 16, 32, r);
+      for (int b = 0; b < 2; ++b) {
+        tmem_ld_wait();
+        if (b == 0) tmem_ld_32x32b_x16(ta + C::COL_D + h * 32 + 16, d[1]);
+        float r[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int jj = 16 * b + j;
+          r[j] = bs[jj] * __fmaf_rn(-cs[jj], __uint_as_float(d[b][j]), __bfloat162float(vt[jj * 128]));
+        }
+        store_parts<3>({ta + C::COL_R + h * 16 + 8 * b, ta + C::COL_R + 32 + h * 16 + 8 * b,
+                        ta + C::COL_R3 + h * 16 + 8 * b}, r);
+      }
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&bars.r_ready);
-      // Delta = R + (T - I) R
+      // Delta = T R, as it is (for y) and weighed for the state
       wait(&bars.d3_done, c);
       tc_fence_after();
-      tmem_ld_32x32b_x32(ta + C::COL_D + h * 32, d);
-      const float* us = until_of(ts) + h * 32;
-      tmem_ld_wait();
-      float w[32];
+      tmem_ld_32x32b_x16(ta + C::COL_D + h * 32, d[0]);
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        r[j] += __uint_as_float(d[j]);
-        w[j] = us[j] * r[j];
+      for (int b = 0; b < 2; ++b) {
+        tmem_ld_wait();
+        if (b == 0) tmem_ld_32x32b_x16(ta + C::COL_D + h * 32 + 16, d[1]);
+        float x[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = us[16 * b + j] * __uint_as_float(d[b][j]);
+        store_parts<3>({ta + C::COL_S + h * 16 + 8 * b, ta + C::COL_S + 32 + h * 16 + 8 * b,
+                        ta + C::COL_S + 64 + h * 16 + 8 * b}, x);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = __uint_as_float(d[b][j]);
+        store_parts<2>({ta + C::COL_R + h * 16 + 8 * b, ta + C::COL_R + 32 + h * 16 + 8 * b}, x);
       }
-      store_parts<3>(ta + C::COL_S + h * 16, 32, w);
-      store_parts<2>(ta + C::COL_R + h * 16, 32, r);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&bars.delta_ready);
@@ -656,36 +685,41 @@ __global__ void __launch_bounds__(C_THREADS, 1) gdn_rule_chunked(const RuleParam
       const float keep = cum_of(ts)[CH - 1];
       wait(&bars.d4_done, c);
       tc_fence_after();
+      tmem_ld_32x32b_x16(ta + C::COL_D + h * NS, d[0]);
 #pragma unroll
-      for (int b = 0; b < NS / 32; ++b) {
-        tmem_ld_32x32b_x32(ta + C::COL_D + h * NS + 32 * b, d);
+      for (int b = 0; b < NS / 16; ++b) {
         tmem_ld_wait();
+        if (b + 1 < NS / 16) tmem_ld_32x32b_x16(ta + C::COL_D + h * NS + 16 * (b + 1), d[(b + 1) & 1]);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) s[32 * b + j] = __fmaf_rn(keep, s[32 * b + j], __uint_as_float(d[j]));
+        for (int j = 0; j < 16; ++j)
+          s[16 * b + j] = __fmaf_rn(keep, s[16 * b + j], __uint_as_float(d[b & 1][j]));
+        store_state(b);
       }
-      if (c + 1 < chunks) {
-        store_parts<3>(ta + C::COL_S + h * (NS / 2), C::S_PART, s);
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(&bars.s_ready);
-      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&bars.s_ready);
       // Y = c Q S^T + P Delta, while the next chunk's K S^T runs
       wait(&bars.y_done, c);
       tc_fence_after();
-      uint32_t e[32];
-      tmem_ld_32x32b_x32(ta + C::COL_SQ + h * 32, d);
-      tmem_ld_32x32b_x32(ta + C::COL_Y + h * 32, e);
-      tmem_ld_wait();
-      tc_fence_before();
-      mbar_arrive(&bars.y_read);
       const int rows = min(CH, len - c * CH) - h * 32;
-      __nv_bfloat16* out = p.y + ((first + (size_t)c * CH + h * 32) * p.Hv + hv) * p.Dv + dv0 + row;
-      const size_t step = (size_t)p.Hv * p.Dv;
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        const float y = __fmaf_rn(cs[j], __uint_as_float(d[j]), __uint_as_float(e[j]));
-        if (live && j < rows) out[j * step] = __float2bfloat16_rn(y);
+      for (int b = 0; b < 2; ++b) {
+        tmem_ld_32x32b_x16(ta + C::COL_SQ + h * 32 + 16 * b, d[0]);
+        tmem_ld_32x32b_x16(ta + C::COL_Y + h * 32 + 16 * b, d[1]);
+        tmem_ld_wait();
+        if (b == 1) {
+          tc_fence_before();
+          mbar_arrive(&bars.y_read);
+        }
+        __nv_bfloat16* o = out + 16 * b * y_step;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float y = __fmaf_rn(cs[16 * b + j], __uint_as_float(d[0][j]), __uint_as_float(d[1][j]));
+          if (live && 16 * b + j < rows) *o = __float2bfloat16_rn(y);
+          o += y_step;
+        }
       }
+      out += CH * y_step;
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.tp_freed[ts]);
     }
@@ -696,70 +730,97 @@ __global__ void __launch_bounds__(C_THREADS, 1) gdn_rule_chunked(const RuleParam
         *reinterpret_cast<float4*>(dst + i) = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
     }
   } else if (lane == 0) {
-    // ------------------------------------------------------------- products
+    // ----------------------------------------------------- loads and products
     constexpr uint32_t ID64 = make_idesc_bf16(128, 64);
     constexpr uint32_t IDK = make_idesc_bf16(128, DK) | kIdescBTransposed;
+    auto load = [&](int c) {
+      const int s = c % C_STAGES;
+      uint8_t* kq = smem + s * C::STAGE_BYTES;
+      const int tok = int(first) + c * CH;
+      mbar_arrive_expect_tx(&bars.loaded[s], C::STAGE_BYTES);
+      for (int a = 0; a < DK / 64; ++a) {
+        tma_load_2d(kq + a * C::ATOM, &tm_k, &bars.loaded[s], hk * DK + a * 64, tok);
+        tma_load_2d(kq + a * C::ATOM + 64 * 128, &tm_q, &bars.loaded[s], hk * DK + a * 64, tok);
+      }
+      tma_load_2d(kq + C::KQ_BYTES, &tm_v, &bars.loaded[s], hv * p.Dv + dv0, tok);
+    };
     auto kq_desc = [&](int s, int row, int k) {   // 16 columns from 16 k on
       return make_sw128_desc(smem_base + s * C::STAGE_BYTES + (k / 4) * C::ATOM + row * 128 + (k % 4) * 32);
     };
     auto grams = [&](int c) {   // [K; Q] K^T
       const int s = c % C_STAGES;
       wait(&bars.full[s], c / C_STAGES);
+#pragma unroll
       for (int k = 0; k < DK / 16; ++k)
         mma_bf16_ss(tmem + C::COL_G, kq_desc(s, 0, k), kq_desc(s, 0, k), ID64, k > 0);
       tc_commit(&bars.g_full);
     };
+    for (int c = 0; c < min(chunks, 2); ++c) load(c);
     grams(0);
     for (int c = 0; c < chunks; ++c) {
       const int s = c % C_STAGES, ts = c % 2;
       const uint32_t tp = smem_base + C::TP_OFF + ts * C::TP_BYTES;
       wait(&bars.s_ready, c);
-      if (c == 0) wait(&bars.g_read, 0);
       tc_fence_after();
+#pragma unroll
       for (int part = 0; part < 3; ++part)
+#pragma unroll
         for (int k = 0; k < DK / 16; ++k)
           mma_bf16_ts(tmem + C::COL_D, tmem + C::COL_S + part * C::S_PART + k * 8, kq_desc(s, 0, k), ID64,
                       part + k > 0);
       tc_commit(&bars.d1_done);
+      // chunk c - 1 is done with its stage: its products are complete and its
+      // values read (s_ready comes after both)
+      if (c + 2 < chunks) load(c + 2);
       if (c > 0) {
         wait(&bars.y_read, c - 1);
         tc_fence_after();
       }
+#pragma unroll
       for (int part = 0; part < 2; ++part)
+#pragma unroll
         for (int k = 0; k < DK / 16; ++k)
           mma_bf16_ts(tmem + C::COL_SQ, tmem + C::COL_S + part * C::S_PART + k * 8, kq_desc(s, 64, k), ID64,
                       part + k > 0);
       wait(&bars.tp_full[ts], c / 2);
       wait(&bars.r_ready, c);
       tc_fence_after();
-      // first parts, then second part x first part both ways round
-      for (int m = 0; m < 3; ++m)
+      // R's three parts with T's first, R's first with T's second
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+#pragma unroll
         for (int k = 0; k < CH / 16; ++k)
-          mma_bf16_ts(tmem + C::COL_D, tmem + C::COL_R + (m == 1 ? 32 : 0) + k * 8,
-                      make_sw128_desc(tp + (m == 2 ? CH * 128 : 0) + k * 32), ID64, m + k > 0);
+          mma_bf16_ts(tmem + C::COL_D, tmem + (m == 2 ? C::COL_R3 : C::COL_R + (m == 1 ? 32 : 0)) + k * 8,
+                      make_sw128_desc(tp + (m == 3 ? CH * 128 : 0) + k * 32), ID64, m + k > 0);
       tc_commit(&bars.d3_done);
       if (c + 1 < chunks) grams(c + 1);
       wait(&bars.delta_ready, c);
       if (c + 1 < chunks) wait(&bars.g_read, c + 1);
       tc_fence_after();
+#pragma unroll
       for (int part = 0; part < 3; ++part)
+#pragma unroll
         for (int k = 0; k < CH / 16; ++k)
           mma_bf16_ts(tmem + C::COL_D, tmem + C::COL_S + part * 32 + k * 8,
                       make_sw128_mn_desc(smem_base + s * C::STAGE_BYTES + k * 16 * 128, C::ATOM), IDK,
                       part + k > 0);
       tc_commit(&bars.d4_done);
-      tc_commit(&bars.freed[s]);
+#pragma unroll
       for (int m = 0; m < 3; ++m)
+#pragma unroll
         for (int k = 0; k < CH / 16; ++k)
           mma_bf16_ts(tmem + C::COL_Y, tmem + C::COL_R + (m == 1 ? 32 : 0) + k * 8,
-                      make_sw128_desc(tp + (m == 2 ? 3 : 2) * CH * 128 + k * 32), ID64, m + k > 0);
+                      make_sw128_desc(tp + C::T_BYTES + (m == 2 ? CH * 128 : 0) + k * 32), ID64, m + k > 0);
       tc_commit(&bars.y_done);
       tc_commit(&bars.tp_freed[ts]);
     }
     // every commit's arrival has landed before the CTA gives its memory back
-    wait(&bars.y_done, chunks - 1);
+    // (the other commits' were waited for by the state's threads)
     for (int c = max(0, chunks - 2); c < chunks; ++c) wait(&bars.tp_freed[c % 2], c / 2);
-    for (int c = max(0, chunks - C_STAGES); c < chunks; ++c) wait(&bars.freed[c % C_STAGES], c / C_STAGES);
+    if (abort_word) {
+      // a wait ran out: let the copies in flight land before the CTA leaves
+      for (int c = max(0, chunks - C_STAGES); c < chunks; ++c) mbar_wait(&bars.loaded[c % C_STAGES], (c / C_STAGES) & 1);
+    }
   }
   __syncwarp();
   tc_fence_before();
@@ -772,13 +833,30 @@ template <int DK>
 int launch_chunked(const RuleParams& p, cudaStream_t stream) {
   static std::atomic<uint64_t> done{0};
   const long long grid = (long long)p.B * p.Hv * ((p.Dv + 127) / 128);
-  if (grid > 0x7fffffffll) return DFL_ERR_BAD_SHAPE;
+  if (grid > 0x7fffffffll || (!p.cu && (long long)p.B * p.T > 0x7fffffffll)) return DFL_ERR_BAD_SHAPE;
   int dev, sms;
   int st = host::current_device(&dev, &sms);
   if (st != DFL_OK) return st;
   st = host::ensure_smem(gdn_rule_chunked<DK>, CCfg<DK>::SMEM_BYTES, dev, done);
   if (st != DFL_OK) return st;
-  gdn_rule_chunked<DK><<<int(grid), C_THREADS, CCfg<DK>::SMEM_BYTES, stream>>>(p);
+  const uint64_t tokens = p.cu ? uint64_t(p.T) : uint64_t(p.B) * p.T;
+  CUtensorMap tm_q, tm_k, tm_v;
+  if (tokens > 0) {
+    const uint64_t wk = uint64_t(p.Hk) * DK, wv = uint64_t(p.Hv) * p.Dv;
+    st = host::make_tmap_2d(&tm_q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.q, wk, tokens, uint64_t(p.ldq) * 2, 64, CH,
+                            CU_TENSOR_MAP_SWIZZLE_128B);
+    if (st != DFL_OK) return st;
+    st = host::make_tmap_2d(&tm_k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.k, wk, tokens, uint64_t(p.ldk) * 2, 64, CH,
+                            CU_TENSOR_MAP_SWIZZLE_128B);
+    if (st != DFL_OK) return st;
+    st = host::make_tmap_2d(&tm_v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.v, wv, tokens, uint64_t(p.ldv) * 2, 128, CH,
+                            CU_TENSOR_MAP_SWIZZLE_NONE);
+    if (st != DFL_OK) return st;
+  } else {
+    std::memset(&tm_q, 0, sizeof(tm_q));   // no step, no load
+    tm_k = tm_v = tm_q;
+  }
+  gdn_rule_chunked<DK><<<int(grid), C_THREADS, CCfg<DK>::SMEM_BYTES, stream>>>(tm_q, tm_k, tm_v, p);
   return host::launch_status();
 }
 
