@@ -234,19 +234,23 @@ int launch_recurrent(const RuleParams& p, cudaStream_t stream) {
 // products from TMEM, and only K, Q, T and P are read from shared memory, K
 // both as it is and transposed from the same tile.
 //
-// fp32 in bf16 products: K and Q are bf16 already.  The state, R and the update
-// go in as three bf16 parts (24 bits), so what is carried from chunk to chunk
-// keeps 32-bit accuracy; T as two (its unit diagonal is exact, what lies below
-// it is a correction), P, and the state's and Delta's share of y, which ends in
-// 8 bits, as two, each without the product of the two second parts.
+// fp32 in bf16 products: K and Q are bf16 already.  The state and the update
+// Delta K go in as three bf16 parts (24 bits), so what is carried from chunk to
+// chunk keeps 32-bit accuracy; R and T - I as two each (without the product of
+// the second parts): their product is a correction to R, which is added in
+// fp32.  In y, which ends in 8 bits, the state has two parts, P and Delta one.
 //
 // Warps: 0-3 prepare T and P of the next chunk (K K^T and Q K^T from one
 // product, inverse by blocks of 16, 32 and 64 in fp32) and put zeros over rows
 // of masked steps and behind the end; 4-11 (two threads per value row, half the
 // columns each) carry the state; 12 loads (TMA, two chunks ahead) and issues
-// the products.
+// the products (13-15 only lend their registers).
 constexpr int CH = 64;               // steps of a chunk
-constexpr int C_THREADS = 13 * 32;
+constexpr int C_THREADS = 16 * 32;
+// Registers of a thread after the split; the launch has 128 for each, and
+// 128 (preparation, as launched) + 2 x 168 + 48 = 4 x 128.
+constexpr int C_REGS_STATE = 168, C_REGS_ISSUE = 48;
+constexpr int C_ORDER = 256;         // packed sequences that are taken longest first
 constexpr int C_STAGES = 3;
 constexpr int C_PREP = 128, C_STATE = 256;
 constexpr int INV_LD = CH + 4;       // floats of a row of the inverse (no bank conflicts between rows)
@@ -258,20 +262,19 @@ struct CCfg {
   static constexpr int V_BYTES = CH * 256;               // 64 rows x 128 columns
   static constexpr int STAGE_BYTES = KQ_BYTES + V_BYTES;
   static constexpr int T_BYTES = INV_LD * CH * 4;        // fp32 inverse, then T's two parts
-  static constexpr int TP_BYTES = T_BYTES + 2 * CH * 128;  // ... and P's
+  static constexpr int TP_BYTES = T_BYTES + CH * 128;    // ... and P
   static constexpr int TP_OFF = C_STAGES * STAGE_BYTES;
   static constexpr int SMALL_OFF = TP_OFF + 2 * TP_BYTES;
-  static constexpr int SMALL_BYTES = (C_STAGES * 2 + 2 * 2) * CH * 4;
+  static constexpr int SMALL_BYTES = (C_STAGES * 2 + 2 * 3) * CH * 4;
   static constexpr int SMEM_BYTES = SMALL_OFF + SMALL_BYTES + 1024;
-  static_assert(T_BYTES % 1024 == 0 && T_BYTES >= 2 * CH * 128, "P's parts start on a swizzle atom");
+  static_assert(T_BYTES % 1024 == 0 && T_BYTES >= 2 * CH * 128, "P starts on a swizzle atom");
   // TMEM columns
   static constexpr int S_PART = DK / 2;                  // columns of one part of the state
   static constexpr int COL_S = 0;                        // state parts; later Delta K's three parts
   static constexpr int COL_D = 192;                      // S K^T, then R T^T, then Delta K
   static constexpr int COL_G = 256;                      // [K; Q] K^T, over Delta K's second half
-  static constexpr int COL_R3 = 256;                     // R's third part, before the next [K; Q] K^T
   static constexpr int COL_SQ = 320;                     // S Q^T
-  static constexpr int COL_R = 384;                      // R's first parts, then Delta's
+  static constexpr int COL_R = 384;                      // R's parts, then Delta
   static constexpr int COL_Y = 448;                      // Delta P^T
 };
 
@@ -288,6 +291,29 @@ __device__ __forceinline__ uint32_t take_part(float& a, float& b) {
       : "+f"(a), "+f"(b)
       : "f"(__uint_as_float(u << 16)), "f"(__uint_as_float(u & 0xffff0000u)));
   return u;
+}
+
+// (d0, d1) = (a0, a1) * (b0, b1) + (c0, c1), one packed instruction
+__device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, float b0, float b1, float c0,
+                                     float c1) {
+  asm("{\n\t.reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\t"
+      "mov.b64 y, {%4, %5};\n\t"
+      "mov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 z, x, y, z;\n\t"
+      "mov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+
+template <int REGS>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+
+template <int REGS>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
 }
 
 // The parts of 16 values into 8 TMEM columns each, at the given addresses.
@@ -309,22 +335,7 @@ struct ChunkBars {
   uint64_t s_ready, d1_done, r_ready, d3_done, delta_ready, d4_done, y_done, y_read;
 };
 
-// m += x . y over four j: x a row's four values, y rows j .. j + 3 at column c
-__device__ __forceinline__ void fma_4x4(float4& m, const float4& x, const float4& y0, const float4& y1,
-                                        const float4& y2, const float4& y3) {
-  m.x = __fmaf_rn(x.x, y0.x, m.x); m.y = __fmaf_rn(x.x, y0.y, m.y);
-  m.z = __fmaf_rn(x.x, y0.z, m.z); m.w = __fmaf_rn(x.x, y0.w, m.w);
-  m.x = __fmaf_rn(x.y, y1.x, m.x); m.y = __fmaf_rn(x.y, y1.y, m.y);
-  m.z = __fmaf_rn(x.y, y1.z, m.z); m.w = __fmaf_rn(x.y, y1.w, m.w);
-  m.x = __fmaf_rn(x.z, y2.x, m.x); m.y = __fmaf_rn(x.z, y2.y, m.y);
-  m.z = __fmaf_rn(x.z, y2.z, m.z); m.w = __fmaf_rn(x.z, y2.w, m.w);
-  m.x = __fmaf_rn(x.w, y3.x, m.x); m.y = __fmaf_rn(x.w, y3.y, m.y);
-  m.z = __fmaf_rn(x.w, y3.z, m.z); m.w = __fmaf_rn(x.w, y3.w, m.w);
-}
-
 __device__ __forceinline__ float4 at4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-
-__device__ __forceinline__ float4 neg4(const float4& x) { return make_float4(-x.x, -x.y, -x.z, -x.w); }
 
 // Inverse of the diagonal block of 16 rows of a unit lower triangular matrix
 // (strictly lower part used) by forward substitution, column c per lane, 16
@@ -349,61 +360,133 @@ __device__ __forceinline__ void invert_block16(float* blk, int c) {
   for (int i = 0; i < 16; ++i) blk[i * INV_LD + c] = x[i];
 }
 
-// The rest of the 64 x 64 inverse from its diagonal blocks, by the 128
-// preparing threads: T21 = -T22 (A21 T11) for blocks of 16, then of 32.
-__device__ __forceinline__ void invert_join(float* a, int t) {
-  constexpr int L = INV_LD;
-  {
-    const int pr = t / 64, i = (t % 64) / 4, c = (t % 4) * 4;   // 4 columns of one row
-    float* t11 = a + pr * 32 * (L + 1);
-    float* a21 = t11 + 16 * L;
-    const float* t22 = t11 + 16 * (L + 1);
-    float4 m = make_float4(0.f, 0.f, 0.f, 0.f);
+// Operands of mma.m16n8k16 in two bf16 parts, from fp32 rows of INV_LD floats
+// (or from an accumulator): X = part 0 + part 1 to 16 bits, which is what T is
+// stored in.  A product adds part 0 x part 0, 0 x 1 and 1 x 0.
+struct FragA { uint32_t p[2][4]; };
+struct FragB { uint32_t p[2][2]; };
+
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t* p0, uint32_t* p1) {
+  *p0 = take_part(x, y);
+  *p1 = take_part(x, y);
+}
+
+// 16 x 16 block at x: lane l holds rows l / 4 and + 8, columns 2 (l % 4) .. + 1 and + 8
+__device__ __forceinline__ FragA load_frag_a(const float* x, int lane) {
+  FragA f;
+  const float* at = x + (lane / 4) * INV_LD + 2 * (lane % 4);
 #pragma unroll
-    for (int j = 0; j < 16; j += 4)
-      fma_4x4(m, at4(a21 + i * L + j), at4(t11 + j * L + c), at4(t11 + (j + 1) * L + c),
-              at4(t11 + (j + 2) * L + c), at4(t11 + (j + 3) * L + c));
-    named_bar_sync(1, C_PREP);
-    *reinterpret_cast<float4*>(a21 + i * L + c) = m;
-    named_bar_sync(1, C_PREP);
-    m = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int j = 0; j < 16; j += 4)
-      fma_4x4(m, at4(t22 + i * L + j), at4(a21 + j * L + c), at4(a21 + (j + 1) * L + c),
-              at4(a21 + (j + 2) * L + c), at4(a21 + (j + 3) * L + c));
-    named_bar_sync(1, C_PREP);
-    *reinterpret_cast<float4*>(a21 + i * L + c) = neg4(m);
-    named_bar_sync(1, C_PREP);
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = *reinterpret_cast<const float2*>(at + (i & 1) * 8 * INV_LD + (i / 2) * 8);
+    split_pair(v.x, v.y, &f.p[0][i], &f.p[1][i]);
   }
-  {
-    const int i = (t / 8) * 2, c = (t % 8) * 4;   // 4 columns of two rows
-    float* a21 = a + 32 * L;
-    const float* t22 = a + 32 * (L + 1);
-    float4 m0 = make_float4(0.f, 0.f, 0.f, 0.f), m1 = m0;
+  return f;
+}
+
+// 16 rows (k) x 8 columns at x
+__device__ __forceinline__ FragB load_frag_b(const float* x, int lane) {
+  FragB f;
+  const float* at = x + 2 * (lane % 4) * INV_LD + lane / 4;
 #pragma unroll
-    for (int j = 0; j < 32; j += 4) {
-      const float4 y0 = at4(a + j * L + c), y1 = at4(a + (j + 1) * L + c), y2 = at4(a + (j + 2) * L + c),
-                   y3 = at4(a + (j + 3) * L + c);
-      fma_4x4(m0, at4(a21 + i * L + j), y0, y1, y2, y3);
-      fma_4x4(m1, at4(a21 + (i + 1) * L + j), y0, y1, y2, y3);
-    }
-    named_bar_sync(1, C_PREP);
-    *reinterpret_cast<float4*>(a21 + i * L + c) = m0;
-    *reinterpret_cast<float4*>(a21 + (i + 1) * L + c) = m1;
-    named_bar_sync(1, C_PREP);
-    m0 = make_float4(0.f, 0.f, 0.f, 0.f);
-    m1 = m0;
+  for (int i = 0; i < 2; ++i)
+    split_pair(at[i * 8 * INV_LD], at[(i * 8 + 1) * INV_LD], &f.p[0][i], &f.p[1][i]);
+  return f;
+}
+
+__device__ __forceinline__ void mma_m16n8k16(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+
+// acc (16 rows, NT tiles of 8 columns) += A B, the parts' products in turn over
+// the tiles, so that neighbouring instructions do not wait for one another
+template <int NT>
+__device__ __forceinline__ void mma_parts(float (&acc)[NT][4], const FragA& a, const FragB (&b)[NT]) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 4) {
-      const float4 y0 = at4(a21 + j * L + c), y1 = at4(a21 + (j + 1) * L + c), y2 = at4(a21 + (j + 2) * L + c),
-                   y3 = at4(a21 + (j + 3) * L + c);
-      fma_4x4(m0, at4(t22 + i * L + j), y0, y1, y2, y3);
-      fma_4x4(m1, at4(t22 + (i + 1) * L + j), y0, y1, y2, y3);
-    }
-    named_bar_sync(1, C_PREP);
-    *reinterpret_cast<float4*>(a21 + i * L + c) = neg4(m0);
-    *reinterpret_cast<float4*>(a21 + (i + 1) * L + c) = neg4(m1);
-    named_bar_sync(1, C_PREP);
+  for (int i = 0; i < NT; ++i) mma_m16n8k16(acc[i], a.p[0], b[i].p[0]);
+#pragma unroll
+  for (int i = 0; i < NT; ++i) mma_m16n8k16(acc[i], a.p[0], b[i].p[1]);
+#pragma unroll
+  for (int i = 0; i < NT; ++i) mma_m16n8k16(acc[i], a.p[1], b[i].p[0]);
+}
+
+// out (16 rows, N columns from c0 on) = -(T22 A21) T11 for N2 x N2 blocks, the 16
+// rows from r0 on: the first product's accumulators are the second one's left
+// operand in place, so nothing passes through shared memory between them.
+template <int N2, int N>
+__device__ __forceinline__ void join_rows(const float* t22, const float* a21, const float* t11, int r0, int c0,
+                                          int lane, float (&out)[N / 8][4]) {
+  float m[N2 / 8][4];
+#pragma unroll
+  for (int i = 0; i < N2 / 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m[i][e] = 0.f;
+#pragma unroll
+  for (int k = 0; k < N2 / 16; ++k) {
+    const FragA a = load_frag_a(t22 + r0 * INV_LD + 16 * k, lane);
+    FragB b[N2 / 8];
+#pragma unroll
+    for (int i = 0; i < N2 / 8; ++i) b[i] = load_frag_b(a21 + 16 * k * INV_LD + 8 * i, lane);
+    mma_parts(m, a, b);
+  }
+#pragma unroll
+  for (int i = 0; i < N / 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[i][e] = 0.f;
+#pragma unroll
+  for (int k = 0; k < N2 / 16; ++k) {
+    FragA a;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      split_pair(-m[2 * k + i / 2][2 * (i & 1)], -m[2 * k + i / 2][2 * (i & 1) + 1], &a.p[0][i], &a.p[1][i]);
+    FragB b[N / 8];
+#pragma unroll
+    for (int i = 0; i < N / 8; ++i) b[i] = load_frag_b(t11 + 16 * k * INV_LD + c0 + 8 * i, lane);
+    mma_parts(out, a, b);
+  }
+}
+
+template <int N>
+__device__ __forceinline__ void store_rows(float* x, int lane, const float (&m)[N / 8][4]) {
+  float* at = x + (lane / 4) * INV_LD + 2 * (lane % 4);
+#pragma unroll
+  for (int i = 0; i < N / 8; ++i) {
+    *reinterpret_cast<float2*>(at + 8 * i) = make_float2(m[i][0], m[i][1]);
+    *reinterpret_cast<float2*>(at + 8 * INV_LD + 8 * i) = make_float2(m[i][2], m[i][3]);
+  }
+}
+
+// The rest of the 64 x 64 inverse from its diagonal blocks of 16, by the 4
+// preparing warps: T21 = -(T22 A21) T11 for blocks of 16, then of 32.  On the
+// register form of the tensor instructions: at 16 and 32 rows a TMEM round
+// trip would cost more than the products, and fp32 FMAs fed from shared
+// memory (measured: 3300 cycles) held up the state's products, whose operands
+// come from there too.
+__device__ __forceinline__ void invert_join(float* a, int warp, int lane) {
+  constexpr int L = INV_LD;
+  if (warp < 2) {
+    float* t11 = a + warp * 32 * (L + 1);
+    float m[2][4];
+    join_rows<16, 16>(t11 + 16 * (L + 1), t11 + 16 * L, t11, 0, 0, lane, m);
+    __syncwarp();
+    store_rows<16>(t11 + 16 * L, lane, m);
+  }
+  named_bar_sync(1, C_PREP);
+  const int r0 = (warp / 2) * 16, c0 = (warp % 2) * 16;
+  float m[2][4];
+  join_rows<32, 16>(a + 32 * (L + 1), a + 32 * L, a, r0, c0, lane, m);
+  named_bar_sync(1, C_PREP);
+  store_rows<16>(a + (32 + r0) * L + c0, lane, m);
+  named_bar_sync(1, C_PREP);
+}
+
+__device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; i += 4) {
+    const float4 v = at4(p + i);
+    x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
   }
 }
 
@@ -416,12 +499,27 @@ __global__ void __launch_bounds__(C_THREADS, 1)
   __shared__ ChunkBars bars;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_word;
+  __shared__ int lens[C_ORDER], chosen;
 
   const int tiles = (p.Dv + 127) / 128;
-  const int nh = blockIdx.x / tiles;  // n * Hv + hv
-  const int dv0 = (blockIdx.x - nh * tiles) * 128;
-  const int n = nh / p.Hv;
-  const int hv = nh - n * p.Hv;
+  const int dv0 = (blockIdx.x % tiles) * 128;
+  const int hv = (blockIdx.x / tiles) % p.Hv;
+  int n = blockIdx.x / (tiles * p.Hv);
+  if (p.cu && p.B > 1 && p.B <= C_ORDER) {
+    // Longest sequences first: a CTA's time goes by its chunks, and a long one
+    // that starts late would run on alone.
+    const int t = threadIdx.x;
+    if (t < p.B) lens[t] = p.cu[t + 1] - p.cu[t];
+    __syncthreads();
+    if (t < p.B) {
+      int rank = 0;
+      for (int u = 0; u < p.B; ++u) rank += lens[u] > lens[t] || (lens[u] == lens[t] && u < t);
+      if (rank == n) chosen = t;
+    }
+    __syncthreads();
+    n = chosen;
+  }
+  const int nh = n * p.Hv + hv;
   const int hk = hv / (p.Hv / p.Hk);
   const int cols = min(128, p.Dv - dv0);  // value rows of this CTA
   size_t first;
@@ -441,11 +539,12 @@ __global__ void __launch_bounds__(C_THREADS, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t smem_base = smem_u32(smem);
   float* small = reinterpret_cast<float*>(smem + C::SMALL_OFF);
-  // g and beta of a stage; c_i and D_63,i of a prepared chunk
+  // g and beta of a stage; c_i, D_63,i and -beta_i c_i of a prepared chunk
   auto g_of = [&](int s) { return small + s * 2 * CH; };
   auto b_of = [&](int s) { return small + s * 2 * CH + CH; };
-  auto cum_of = [&](int s) { return small + C_STAGES * 2 * CH + s * 2 * CH; };
-  auto until_of = [&](int s) { return small + C_STAGES * 2 * CH + s * 2 * CH + CH; };
+  auto cum_of = [&](int s) { return small + C_STAGES * 2 * CH + s * 3 * CH; };
+  auto until_of = [&](int s) { return small + C_STAGES * 2 * CH + s * 3 * CH + CH; };
+  auto nbc_of = [&](int s) { return small + C_STAGES * 2 * CH + s * 3 * CH + 2 * CH; };
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -485,15 +584,19 @@ __global__ void __launch_bounds__(C_THREADS, 1)
     const int t = threadIdx.x;
     // Chunk c's tiles have landed: zeros over rows of no step, g and beta (1
     // and 0 there: a step that changes nothing) beside them.
+    bool on;
+    float gv, bv;
+    auto fetch = [&](int c) {   // step t / 2 of the chunk
+      const size_t tok = first + (size_t)c * CH + t / 2;
+      on = t / 2 < len - c * CH && (!p.mask || p.mask[tok] != 0);
+      gv = on ? p.g[tok * p.Hv + hv] : 1.f;
+      bv = on ? p.beta[tok * p.Hv + hv] : 0.f;
+    };
     auto publish = [&](int c) {
-      const int s = c % C_STAGES;
-      const size_t tok0 = first + (size_t)c * CH;
-      const int rows = min(CH, len - c * CH);
-      const int r = t / 2;
-      const bool on = r < rows && (!p.mask || p.mask[tok0 + r] != 0);
+      const int s = c % C_STAGES, r = t / 2;
       if (t % 2 == 0) {
-        g_of(s)[r] = on ? p.g[(tok0 + r) * p.Hv + hv] : 1.f;
-        b_of(s)[r] = on ? p.beta[(tok0 + r) * p.Hv + hv] : 0.f;
+        g_of(s)[r] = gv;
+        b_of(s)[r] = bv;
       }
       wait(&bars.loaded[s], c / C_STAGES);
       if (!on) {
@@ -510,7 +613,9 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       fence_proxy_async_shared();
       mbar_arrive(&bars.full[s]);
     };
+    fetch(0);
     publish(0);
+    if (chunks > 1) fetch(1);
     for (int c = 0; c < chunks; ++c) {
       const int s = c % C_STAGES, ts = c % 2;
       const int i = t & 63;       // this thread's step: row of K K^T (t < 64) or of Q K^T
@@ -527,58 +632,76 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       const float* gs = g_of(s);
       uint8_t* tp = smem + C::TP_OFF + ts * C::TP_BYTES;
       float* am = reinterpret_cast<float*>(tp);
-      // D_ij along the row, from the diagonal to the left
-      const float beta = b_of(s)[i];
-      float d = 0.f, next = 1.f;
+      // D_ij along the row, from the diagonal to the left, times beta_i in A's
+      // rows; right of the diagonal d is 0 (what A's diagonal holds is not read)
+      const float start = t < 64 ? b_of(s)[i] : 1.f;
+      float d = 0.f, next = 0.f;
+      float4 glo = at4(gs + CH - 8), ghi = at4(gs + CH - 4);
 #pragma unroll
       for (int j8 = CH - 8; j8 >= 0; j8 -= 8) {
-        const float4 glo = at4(gs + j8), ghi = at4(gs + j8 + 4);
         const float gg[8] = {glo.x, glo.y, glo.z, glo.w, ghi.x, ghi.y, ghi.z, ghi.w};
         float o[8];
 #pragma unroll
         for (int e = 7; e >= 0; --e) {
           const int j = j8 + e;
-          d = j < i ? d * next : (j == i ? 1.f : 0.f);
+          d = j == i ? start : d * next;
           next = gg[e];
-          const float x = d * __uint_as_float(gr[j / 32][j % 32]);
-          o[e] = t < 64 ? (j < i ? beta * x : 0.f) : (j <= i ? x : 0.f);
+          o[e] = d * __uint_as_float(gr[j / 32][j % 32]);
+        }
+        if (j8 > 0) {   // before the stores, which it must not wait for
+          glo = at4(gs + j8 - 8);
+          ghi = at4(gs + j8 - 4);
         }
         if (t < 64) {
           *reinterpret_cast<float4*>(am + i * INV_LD + j8) = make_float4(o[0], o[1], o[2], o[3]);
           *reinterpret_cast<float4*>(am + i * INV_LD + j8 + 4) = make_float4(o[4], o[5], o[6], o[7]);
         } else {
-          uint8_t* at = tp + C::T_BYTES + i * 128 + (((j8 / 8) ^ (i & 7)) * 16);
-#pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            uint4 u;
-            u.x = take_part(o[0], o[1]);
-            u.y = take_part(o[2], o[3]);
-            u.z = take_part(o[4], o[5]);
-            u.w = take_part(o[6], o[7]);
-            *reinterpret_cast<uint4*>(at + part * CH * 128) = u;
-          }
+          uint4 u;
+          u.x = take_part(o[0], o[1]);
+          u.y = take_part(o[2], o[3]);
+          u.z = take_part(o[4], o[5]);
+          u.w = take_part(o[6], o[7]);
+          *reinterpret_cast<uint4*>(tp + C::T_BYTES + i * 128 + (((j8 / 8) ^ (i & 7)) * 16)) = u;
         }
       }
       if (t < 64) {
-        cum_of(ts)[i] = d * next;
         __syncwarp();
         invert_block16(am + (t / 16) * 16 * (INV_LD + 1), t % 16);
-      } else if (warp == 3) {
-        // D_63,j: products of the decays behind j, two j per lane
+      } else {
+        // c_i (warp 2) and D_63,j (warp 3): products of the decays up to a step
+        // and behind it, two steps per lane
         const float2 gg = *reinterpret_cast<const float2*>(gs + 2 * lane);
         float x = gg.x * gg.y;
+        if (warp == 2) {
 #pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-          const float y = __shfl_down_sync(0xffffffffu, x, o);
-          if (lane + o < 32) x *= y;
+          for (int o = 1; o < 32; o *= 2) {
+            const float y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x *= y;
+          }
+          float before = __shfl_up_sync(0xffffffffu, x, 1);
+          if (lane == 0) before = 1.f;
+          before *= gg.x;
+          const float2 bb = *reinterpret_cast<const float2*>(b_of(s) + 2 * lane);
+          *reinterpret_cast<float2*>(cum_of(ts) + 2 * lane) = make_float2(before, x);
+          *reinterpret_cast<float2*>(nbc_of(ts) + 2 * lane) = make_float2(-bb.x * before, -bb.y * x);
+        } else {
+#pragma unroll
+          for (int o = 1; o < 32; o *= 2) {
+            const float y = __shfl_down_sync(0xffffffffu, x, o);
+            if (lane + o < 32) x *= y;
+          }
+          x = __shfl_down_sync(0xffffffffu, x, 1);
+          if (lane == 31) x = 1.f;
+          *reinterpret_cast<float2*>(until_of(ts) + 2 * lane) = make_float2(x * gg.y, x);
         }
-        x = __shfl_down_sync(0xffffffffu, x, 1);
-        if (lane == 31) x = 1.f;
-        *reinterpret_cast<float2*>(until_of(ts) + 2 * lane) = make_float2(x * gg.y, x);
       }
+      // halfway: the next chunk's tiles have had the time to land, and its
+      // [K; Q] K^T is there when this chunk's T is done
+      if (c + 1 < chunks) publish(c + 1);
+      if (c + 2 < chunks) fetch(c + 2);
       named_bar_sync(1, C_PREP);
-      invert_join(am, t);
-      // T in two parts over the same memory: half a row per thread
+      invert_join(am, warp, lane);
+      // T - I in two parts over the same memory: half a row per thread
       {
         const int r = t / 2, c0 = (t % 2) * 32;
         float x[32];
@@ -587,6 +710,8 @@ __global__ void __launch_bounds__(C_THREADS, 1)
           const float4 y = at4(am + r * INV_LD + c0 + 4 * q);
           x[4 * q] = y.x; x[4 * q + 1] = y.y; x[4 * q + 2] = y.z; x[4 * q + 3] = y.w;
         }
+#pragma unroll
+        for (int q = 0; q < 32; ++q) x[q] = c0 + q == r ? 0.f : x[q];
         named_bar_sync(1, C_PREP);
 #pragma unroll
         for (int part = 0; part < 2; ++part)
@@ -602,10 +727,10 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       }
       fence_proxy_async_shared();
       mbar_arrive(&bars.tp_full[ts]);
-      if (c + 1 < chunks) publish(c + 1);
     }
   } else if (warp < 12) {
     // --------------------------------------------------------- the state rows
+    more_registers<C_REGS_STATE>();
     const int h = (warp - 4) / 4;            // which half of the columns
     const int row = (warp % 4) * 32 + lane;  // TMEM lane, value row dv0 + row
     const bool live = row < cols;
@@ -635,34 +760,27 @@ __global__ void __launch_bounds__(C_THREADS, 1)
     for (int c = 0; c < chunks; ++c) {
       const int st = c % C_STAGES, ts = c % 2;
       uint32_t d[2][16];
-      // R = beta (V - c K S^T)
+      // R = beta (V - c K S^T); beta V while the product runs.  Coefficients
+      // come 16 at a time, ahead of the stores that the compiler keeps loads behind.
       wait(&bars.tp_full[ts], c / 2);
       const __nv_bfloat16* vt =
           reinterpret_cast<const __nv_bfloat16*>(smem + st * C::STAGE_BYTES + C::KQ_BYTES) + h * 32 * 128 + row;
       const float* bs = b_of(st) + h * 32;
       const float* cs = cum_of(ts) + h * 32;
       const float* us = until_of(ts) + h * 32;
-      wait(&bars.d1_done, c);
-      tc_fence_after();
-      tmem_ld_32x32b_x16(ta + C::COL_D + h * 32, d[0]);
+      const float* nbc = nbc_of(ts) + h * 32;
+      float r[32];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        tmem_ld_wait();
-        if (b == 0) tmem_ld_32x32b_x16(ta + C::COL_D + h * 32 + 16, d[1]);
-        float r[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int jj = 16 * b + j;
-          r[j] = bs[jj] * __fmaf_rn(-cs[jj], __uint_as_float(d[b][j]), __bfloat162float(vt[jj * 128]));
-        }
-        store_parts<3>({ta + C::COL_R + h * 16 + 8 * b, ta + C::COL_R + 32 + h * 16 + 8 * b,
-                        ta + C::COL_R3 + h * 16 + 8 * b}, r);
+      for (int j = 0; j < 32; j += 4) {
+        const float4 be = at4(bs + j);
+        r[j] = be.x * __bfloat162float(vt[j * 128]);
+        r[j + 1] = be.y * __bfloat162float(vt[(j + 1) * 128]);
+        r[j + 2] = be.z * __bfloat162float(vt[(j + 2) * 128]);
+        r[j + 3] = be.w * __bfloat162float(vt[(j + 3) * 128]);
       }
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(&bars.r_ready);
-      // Delta = T R, as it is (for y) and weighed for the state
-      wait(&bars.d3_done, c);
+      float co[16];
+      load16(nbc, co);
+      wait(&bars.d1_done, c);
       tc_fence_after();
       tmem_ld_32x32b_x16(ta + C::COL_D + h * 32, d[0]);
 #pragma unroll
@@ -671,12 +789,39 @@ __global__ void __launch_bounds__(C_THREADS, 1)
         if (b == 0) tmem_ld_32x32b_x16(ta + C::COL_D + h * 32 + 16, d[1]);
         float x[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = us[16 * b + j] * __uint_as_float(d[b][j]);
-        store_parts<3>({ta + C::COL_S + h * 16 + 8 * b, ta + C::COL_S + 32 + h * 16 + 8 * b,
-                        ta + C::COL_S + 64 + h * 16 + 8 * b}, x);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = __uint_as_float(d[b][j]);
+        for (int j = 0; j < 16; j += 2) {
+          const int jj = 16 * b + j;
+          fma2(r[jj], r[jj + 1], co[j], co[j + 1], __uint_as_float(d[b][j]), __uint_as_float(d[b][j + 1]), r[jj],
+               r[jj + 1]);
+          x[j] = r[jj];
+          x[j + 1] = r[jj + 1];
+        }
+        if (b == 0) load16(nbc + 16, co);
         store_parts<2>({ta + C::COL_R + h * 16 + 8 * b, ta + C::COL_R + 32 + h * 16 + 8 * b}, x);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&bars.r_ready);
+      // Delta = R + (T - I) R, as it is (for y) and weighed for the state
+      load16(us, co);
+      wait(&bars.d3_done, c);
+      tc_fence_after();
+      tmem_ld_32x32b_x16(ta + C::COL_D + h * 32, d[0]);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        tmem_ld_wait();
+        if (b == 0) tmem_ld_32x32b_x16(ta + C::COL_D + h * 32 + 16, d[1]);
+        float x[16], w[16];
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+          const int jj = 16 * b + j;
+          fma2(x[j], x[j + 1], 1.f, 1.f, __uint_as_float(d[b][j]), __uint_as_float(d[b][j + 1]), r[jj], r[jj + 1]);
+          fma2(w[j], w[j + 1], co[j], co[j + 1], x[j], x[j + 1], 0.f, 0.f);
+        }
+        if (b == 0) load16(us + 16, co);
+        store_parts<3>({ta + C::COL_S + h * 16 + 8 * b, ta + C::COL_S + 32 + h * 16 + 8 * b,
+                        ta + C::COL_S + 64 + h * 16 + 8 * b}, w);
+        store_parts<1>({ta + C::COL_R + h * 16 + 8 * b}, x);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -691,8 +836,9 @@ __global__ void __launch_bounds__(C_THREADS, 1)
         tmem_ld_wait();
         if (b + 1 < NS / 16) tmem_ld_32x32b_x16(ta + C::COL_D + h * NS + 16 * (b + 1), d[(b + 1) & 1]);
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          s[16 * b + j] = __fmaf_rn(keep, s[16 * b + j], __uint_as_float(d[b & 1][j]));
+        for (int j = 0; j < 16; j += 2)
+          fma2(s[16 * b + j], s[16 * b + j + 1], keep, keep, s[16 * b + j], s[16 * b + j + 1],
+               __uint_as_float(d[b & 1][j]), __uint_as_float(d[b & 1][j + 1]));
         store_state(b);
       }
       tmem_st_wait();
@@ -706,17 +852,24 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       for (int b = 0; b < 2; ++b) {
         tmem_ld_32x32b_x16(ta + C::COL_SQ + h * 32 + 16 * b, d[0]);
         tmem_ld_32x32b_x16(ta + C::COL_Y + h * 32 + 16 * b, d[1]);
+        load16(cs + 16 * b, co);
         tmem_ld_wait();
         if (b == 1) {
           tc_fence_before();
           mbar_arrive(&bars.y_read);
         }
         __nv_bfloat16* o = out + 16 * b * y_step;
+        __nv_bfloat16 y[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float y = __fmaf_rn(cs[16 * b + j], __uint_as_float(d[0][j]), __uint_as_float(d[1][j]));
-          if (live && 16 * b + j < rows) *o = __float2bfloat16_rn(y);
-          o += y_step;
+        for (int j = 0; j < 16; ++j)
+          y[j] = __float2bfloat16_rn(__fmaf_rn(co[j], __uint_as_float(d[0][j]), __uint_as_float(d[1][j])));
+        if (live && rows >= 16 * b + 16) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[j * y_step] = y[j];
+        } else if (live) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (16 * b + j < rows) o[j * y_step] = y[j];
         }
       }
       out += CH * y_step;
@@ -729,14 +882,17 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       for (int i = 0; i < NS; i += 4)
         *reinterpret_cast<float4*>(dst + i) = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
     }
-  } else if (lane == 0) {
+  } else {
     // ----------------------------------------------------- loads and products
+    fewer_registers<C_REGS_ISSUE>();
+    if (warp == 12) {   // the whole warp walks along, one elected lane issues
     constexpr uint32_t ID64 = make_idesc_bf16(128, 64);
     constexpr uint32_t IDK = make_idesc_bf16(128, DK) | kIdescBTransposed;
     auto load = [&](int c) {
       const int s = c % C_STAGES;
       uint8_t* kq = smem + s * C::STAGE_BYTES;
       const int tok = int(first) + c * CH;
+      if (lane != 0) return;
       mbar_arrive_expect_tx(&bars.loaded[s], C::STAGE_BYTES);
       for (int a = 0; a < DK / 64; ++a) {
         tma_load_2d(kq + a * C::ATOM, &tm_k, &bars.loaded[s], hk * DK + a * 64, tok);
@@ -752,10 +908,11 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       wait(&bars.full[s], c / C_STAGES);
 #pragma unroll
       for (int k = 0; k < DK / 16; ++k)
-        mma_bf16_ss(tmem + C::COL_G, kq_desc(s, 0, k), kq_desc(s, 0, k), ID64, k > 0);
-      tc_commit(&bars.g_full);
+        mma_bf16_ss_warp(tmem + C::COL_G, kq_desc(s, 0, k), kq_desc(s, 0, k), ID64, k > 0);
+      tc_commit_warp(&bars.g_full);
     };
     for (int c = 0; c < min(chunks, 2); ++c) load(c);
+    __syncwarp();
     grams(0);
     for (int c = 0; c < chunks; ++c) {
       const int s = c % C_STAGES, ts = c % 2;
@@ -766,12 +923,18 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       for (int part = 0; part < 3; ++part)
 #pragma unroll
         for (int k = 0; k < DK / 16; ++k)
-          mma_bf16_ts(tmem + C::COL_D, tmem + C::COL_S + part * C::S_PART + k * 8, kq_desc(s, 0, k), ID64,
+          mma_bf16_ts_warp(tmem + C::COL_D, tmem + C::COL_S + part * C::S_PART + k * 8, kq_desc(s, 0, k), ID64,
                       part + k > 0);
-      tc_commit(&bars.d1_done);
+      tc_commit_warp(&bars.d1_done);
+      // the second half of Delta K's columns is free until this chunk's Delta K
+      if (c + 1 < chunks) {
+        if (c == 0) wait(&bars.g_read, 0);   // later ones were waited for before the last Delta K
+        grams(c + 1);
+      }
       // chunk c - 1 is done with its stage: its products are complete and its
       // values read (s_ready comes after both)
       if (c + 2 < chunks) load(c + 2);
+      __syncwarp();
       if (c > 0) {
         wait(&bars.y_read, c - 1);
         tc_fence_after();
@@ -780,20 +943,19 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       for (int part = 0; part < 2; ++part)
 #pragma unroll
         for (int k = 0; k < DK / 16; ++k)
-          mma_bf16_ts(tmem + C::COL_SQ, tmem + C::COL_S + part * C::S_PART + k * 8, kq_desc(s, 64, k), ID64,
+          mma_bf16_ts_warp(tmem + C::COL_SQ, tmem + C::COL_S + part * C::S_PART + k * 8, kq_desc(s, 64, k), ID64,
                       part + k > 0);
       wait(&bars.tp_full[ts], c / 2);
       wait(&bars.r_ready, c);
       tc_fence_after();
-      // R's three parts with T's first, R's first with T's second
+      // first parts, then second part x first part both ways round
 #pragma unroll
-      for (int m = 0; m < 4; ++m)
+      for (int m = 0; m < 3; ++m)
 #pragma unroll
         for (int k = 0; k < CH / 16; ++k)
-          mma_bf16_ts(tmem + C::COL_D, tmem + (m == 2 ? C::COL_R3 : C::COL_R + (m == 1 ? 32 : 0)) + k * 8,
-                      make_sw128_desc(tp + (m == 3 ? CH * 128 : 0) + k * 32), ID64, m + k > 0);
-      tc_commit(&bars.d3_done);
-      if (c + 1 < chunks) grams(c + 1);
+          mma_bf16_ts_warp(tmem + C::COL_D, tmem + C::COL_R + (m == 1 ? 32 : 0) + k * 8,
+                      make_sw128_desc(tp + (m == 2 ? CH * 128 : 0) + k * 32), ID64, m + k > 0);
+      tc_commit_warp(&bars.d3_done);
       wait(&bars.delta_ready, c);
       if (c + 1 < chunks) wait(&bars.g_read, c + 1);
       tc_fence_after();
@@ -801,18 +963,15 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       for (int part = 0; part < 3; ++part)
 #pragma unroll
         for (int k = 0; k < CH / 16; ++k)
-          mma_bf16_ts(tmem + C::COL_D, tmem + C::COL_S + part * 32 + k * 8,
+          mma_bf16_ts_warp(tmem + C::COL_D, tmem + C::COL_S + part * 32 + k * 8,
                       make_sw128_mn_desc(smem_base + s * C::STAGE_BYTES + k * 16 * 128, C::ATOM), IDK,
                       part + k > 0);
-      tc_commit(&bars.d4_done);
+      tc_commit_warp(&bars.d4_done);
 #pragma unroll
-      for (int m = 0; m < 3; ++m)
-#pragma unroll
-        for (int k = 0; k < CH / 16; ++k)
-          mma_bf16_ts(tmem + C::COL_Y, tmem + C::COL_R + (m == 1 ? 32 : 0) + k * 8,
-                      make_sw128_desc(tp + C::T_BYTES + (m == 2 ? CH * 128 : 0) + k * 32), ID64, m + k > 0);
-      tc_commit(&bars.y_done);
-      tc_commit(&bars.tp_freed[ts]);
+      for (int k = 0; k < CH / 16; ++k)
+        mma_bf16_ts_warp(tmem + C::COL_Y, tmem + C::COL_R + k * 8, make_sw128_desc(tp + C::T_BYTES + k * 32), ID64, k > 0);
+      tc_commit_warp(&bars.y_done);
+      tc_commit_warp(&bars.tp_freed[ts]);
     }
     // every commit's arrival has landed before the CTA gives its memory back
     // (the other commits' were waited for by the state's threads)
@@ -820,6 +979,7 @@ __global__ void __launch_bounds__(C_THREADS, 1)
     if (abort_word) {
       // a wait ran out: let the copies in flight land before the CTA leaves
       for (int c = max(0, chunks - C_STAGES); c < chunks; ++c) mbar_wait(&bars.loaded[c % C_STAGES], (c / C_STAGES) & 1);
+    }
     }
   }
   __syncwarp();
