@@ -243,8 +243,8 @@ int launch_recurrent(const RuleParams& p, cudaStream_t stream) {
 // Warps: 0-3 prepare T and P of the next chunk (K K^T and Q K^T from one
 // product, inverse by blocks of 16, 32 and 64 in fp32) and put zeros over rows
 // of masked steps and behind the end; 4-11 (two threads per value row, half the
-// columns each) carry the state; 12 loads (TMA, two chunks ahead) and issues
-// the products (13-15 only lend their registers).
+// columns each) carry the state; 12 and 14 issue the products and 13
+// the loads (TMA, two chunks ahead); 15 only lends its registers.
 constexpr int CH = 64;               // steps of a chunk
 constexpr int C_THREADS = 16 * 32;
 // Registers of a thread after the split; the launch has 128 for each, and
@@ -253,7 +253,8 @@ constexpr int C_REGS_STATE = 168, C_REGS_ISSUE = 48;
 constexpr int C_ORDER = 256;         // packed sequences that are taken longest first
 constexpr int C_STAGES = 3;
 constexpr int C_PREP = 128, C_STATE = 256;
-constexpr int INV_LD = CH + 4;       // floats of a row of the inverse (no bank conflicts between rows)
+constexpr int DIAG_LD = 20, DIAG_BLK = 16 * DIAG_LD + 4;   // floats: a row and a block of A's diagonal blocks
+constexpr int PART = CH * 128;       // bytes of one bf16 part of a 64 x 64 matrix, 128-byte swizzle
 
 template <int DK>
 struct CCfg {
@@ -261,13 +262,12 @@ struct CCfg {
   static constexpr int KQ_BYTES = (DK / 64) * ATOM;
   static constexpr int V_BYTES = CH * 256;               // 64 rows x 128 columns
   static constexpr int STAGE_BYTES = KQ_BYTES + V_BYTES;
-  static constexpr int T_BYTES = INV_LD * CH * 4;        // fp32 inverse, then T's two parts
-  static constexpr int TP_BYTES = T_BYTES + CH * 128;    // ... and P
+  static constexpr int TP_BYTES = 3 * PART;              // T's two parts and P
   static constexpr int TP_OFF = C_STAGES * STAGE_BYTES;
-  static constexpr int SMALL_OFF = TP_OFF + 2 * TP_BYTES;
+  static constexpr int A_OFF = TP_OFF + 2 * TP_BYTES;    // A's two parts, its diagonal blocks in fp32, a place for stores to nowhere
+  static constexpr int SMALL_OFF = A_OFF + 2 * PART + 4 * DIAG_BLK * 4 + 1024;
   static constexpr int SMALL_BYTES = (C_STAGES * 2 + 2 * 3) * CH * 4;
   static constexpr int SMEM_BYTES = SMALL_OFF + SMALL_BYTES + 1024;
-  static_assert(T_BYTES % 1024 == 0 && T_BYTES >= 2 * CH * 128, "P starts on a swizzle atom");
   // TMEM columns
   static constexpr int S_PART = DK / 2;                  // columns of one part of the state
   static constexpr int COL_S = 0;                        // state parts; later Delta K's three parts
@@ -290,6 +290,16 @@ __device__ __forceinline__ uint32_t take_part(float& a, float& b) {
       "mov.b64 {%0, %1}, y;\n\t}"
       : "+f"(a), "+f"(b)
       : "f"(__uint_as_float(u << 16)), "f"(__uint_as_float(u & 0xffff0000u)));
+  return u;
+}
+
+// The leading parts of eight values, as the 16 bytes that they take in a part.
+__device__ __forceinline__ uint4 take_part8(float* x) {
+  uint4 u;
+  u.x = take_part(x[0], x[1]);
+  u.y = take_part(x[2], x[3]);
+  u.z = take_part(x[4], x[5]);
+  u.w = take_part(x[6], x[7]);
   return u;
 }
 
@@ -332,22 +342,25 @@ struct ChunkBars {
   uint64_t loaded[C_STAGES], full[C_STAGES];
   uint64_t tp_full[2], tp_freed[2];
   uint64_t g_full, g_read;
-  uint64_t s_ready, d1_done, r_ready, d3_done, delta_ready, d4_done, y_done, y_read;
+  uint64_t s_ready, d1_done, r_ready, d3_done, delta_ready, d4_done, q_done, y_done, y_read;
 };
 
 __device__ __forceinline__ float4 at4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
-// Inverse of the diagonal block of 16 rows of a unit lower triangular matrix
-// (strictly lower part used) by forward substitution, column c per lane, 16
-// lanes of one warp a block.
-__device__ __forceinline__ void invert_block16(float* blk, int c) {
+// Byte offset of element (r, c) in a part of a 64 x 64 matrix.
+__device__ __forceinline__ int part_at(int r, int c) { return r * 128 + (((c / 8) ^ (r & 7)) * 16) + (c % 8) * 2; }
+
+// Inverse of a unit lower triangular block of 16 rows (strictly lower part
+// used) by forward substitution, column c per lane, 16 lanes of one warp a
+// block; then row c of it in parts to row 16 b + c, columns 16 b .. of t.
+__device__ __forceinline__ void invert_block16(float* blk, uint8_t* t, int b, int c) {
   float x[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     float s0 = i == c ? 1.f : 0.f, s1 = 0.f;
 #pragma unroll
     for (int j = 0; j < i; j += 4) {
-      const float4 m = at4(blk + i * INV_LD + j);
+      const float4 m = at4(blk + i * DIAG_LD + j);
       s0 = __fmaf_rn(-m.x, x[j], s0);
       if (j + 1 < i) s1 = __fmaf_rn(-m.y, x[j + 1], s1);
       if (j + 2 < i) s0 = __fmaf_rn(-m.z, x[j + 2], s0);
@@ -357,129 +370,106 @@ __device__ __forceinline__ void invert_block16(float* blk, int c) {
   }
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 16; ++i) blk[i * INV_LD + c] = x[i];
-}
-
-// Operands of mma.m16n8k16 in two bf16 parts, from fp32 rows of INV_LD floats
-// (or from an accumulator): X = part 0 + part 1 to 16 bits, which is what T is
-// stored in.  A product adds part 0 x part 0, 0 x 1 and 1 x 0.
-struct FragA { uint32_t p[2][4]; };
-struct FragB { uint32_t p[2][2]; };
-
-__device__ __forceinline__ void split_pair(float x, float y, uint32_t* p0, uint32_t* p1) {
-  *p0 = take_part(x, y);
-  *p1 = take_part(x, y);
-}
-
-// 16 x 16 block at x: lane l holds rows l / 4 and + 8, columns 2 (l % 4) .. + 1 and + 8
-__device__ __forceinline__ FragA load_frag_a(const float* x, int lane) {
-  FragA f;
-  const float* at = x + (lane / 4) * INV_LD + 2 * (lane % 4);
+  for (int i = 0; i < 16; ++i) blk[i * DIAG_LD + c] = x[i];
+  __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 v = *reinterpret_cast<const float2*>(at + (i & 1) * 8 * INV_LD + (i / 2) * 8);
-    split_pair(v.x, v.y, &f.p[0][i], &f.p[1][i]);
+  for (int i = 0; i < 16; i += 4) {
+    const float4 y = at4(blk + c * DIAG_LD + i);
+    x[i] = y.x; x[i + 1] = y.y; x[i + 2] = y.z; x[i + 3] = y.w;
   }
-  return f;
-}
-
-// 16 rows (k) x 8 columns at x
-__device__ __forceinline__ FragB load_frag_b(const float* x, int lane) {
-  FragB f;
-  const float* at = x + 2 * (lane % 4) * INV_LD + lane / 4;
+  uint8_t* at0 = t + part_at(16 * b + c, 16 * b);
+  uint8_t* at1 = t + part_at(16 * b + c, 16 * b + 8);
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    split_pair(at[i * 8 * INV_LD], at[(i * 8 + 1) * INV_LD], &f.p[0][i], &f.p[1][i]);
-  return f;
+  for (int part = 0; part < 2; ++part) {
+    *reinterpret_cast<uint4*>(at0 + part * PART) = take_part8(x);
+    *reinterpret_cast<uint4*>(at1 + part * PART) = take_part8(x + 8);
+  }
 }
 
-__device__ __forceinline__ void mma_m16n8k16(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+// Four 8 x 8 blocks of a part: rows r .. r + 15, columns c .. c + 15, in the order
+// of a left operand (as they are) or of two right operands' k x n (transposed).
+template <bool TRANS>
+__device__ __forceinline__ void load_blocks(uint32_t part, int r, int c, int lane, uint32_t (&f)[4]) {
+  const uint32_t at = part + part_at(r + (lane & 15), c + (lane >> 4) * 8);
+  if constexpr (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3]) : "r"(at) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3]) : "r"(at) : "memory");
+}
+
+__device__ __forceinline__ void mma_m16n8k16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// acc (16 rows, NT tiles of 8 columns) += A B, the parts' products in turn over
-// the tiles, so that neighbouring instructions do not wait for one another
-template <int NT>
-__device__ __forceinline__ void mma_parts(float (&acc)[NT][4], const FragA& a, const FragB (&b)[NT]) {
+// acc (16 rows, NP pairs of 8 columns) += A B with B's rows k .. k + 15, columns
+// c .. of a matrix in two parts: first x first, first x second, second x first,
+// each over the tiles in turn, so that neighbours do not wait for one another.
+template <int NP>
+__device__ __forceinline__ void mma_parts(float (&acc)[2 * NP][4], const uint32_t (&a)[2][4], uint32_t b, int k,
+                                          int c, int lane) {
+  uint32_t f[2][NP][4];
 #pragma unroll
-  for (int i = 0; i < NT; ++i) mma_m16n8k16(acc[i], a.p[0], b[i].p[0]);
+  for (int part = 0; part < 2; ++part)
 #pragma unroll
-  for (int i = 0; i < NT; ++i) mma_m16n8k16(acc[i], a.p[0], b[i].p[1]);
+    for (int i = 0; i < NP; ++i) load_blocks<true>(b + part * PART, k, c + 16 * i, lane, f[part][i]);
 #pragma unroll
-  for (int i = 0; i < NT; ++i) mma_m16n8k16(acc[i], a.p[1], b[i].p[0]);
+  for (int m = 0; m < 3; ++m)
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      mma_m16n8k16(acc[2 * i], a[m == 2], f[m == 1][i][0], f[m == 1][i][1]);
+      mma_m16n8k16(acc[2 * i + 1], a[m == 2], f[m == 1][i][2], f[m == 1][i][3]);
+    }
 }
 
-// out (16 rows, N columns from c0 on) = -(T22 A21) T11 for N2 x N2 blocks, the 16
-// rows from r0 on: the first product's accumulators are the second one's left
-// operand in place, so nothing passes through shared memory between them.
-template <int N2, int N>
-__device__ __forceinline__ void join_rows(const float* t22, const float* a21, const float* t11, int r0, int c0,
-                                          int lane, float (&out)[N / 8][4]) {
-  float m[N2 / 8][4];
-#pragma unroll
-  for (int i = 0; i < N2 / 8; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) m[i][e] = 0.f;
-#pragma unroll
-  for (int k = 0; k < N2 / 16; ++k) {
-    const FragA a = load_frag_a(t22 + r0 * INV_LD + 16 * k, lane);
-    FragB b[N2 / 8];
-#pragma unroll
-    for (int i = 0; i < N2 / 8; ++i) b[i] = load_frag_b(a21 + 16 * k * INV_LD + 8 * i, lane);
-    mma_parts(m, a, b);
-  }
+// Rows R + r0 .. + 15, columns C + c0 .. + 15 of T = -(T22 A21) T11 for blocks of N
+// rows, T22 at (R, R), A21 at (R, C), T11 at (C, C): the first product's
+// accumulators are the second one's left operand in place, so nothing passes
+// through shared memory between them.
+template <int N>
+__device__ __forceinline__ void join_block(uint8_t* t, uint32_t t_at, uint32_t a_at, int R, int C, int r0, int c0,
+                                           int lane) {
+  float m[N / 8][4];
 #pragma unroll
   for (int i = 0; i < N / 8; ++i)
 #pragma unroll
+    for (int e = 0; e < 4; ++e) m[i][e] = 0.f;
+#pragma unroll
+  for (int k = 0; k < N / 16; ++k) {
+    uint32_t a[2][4];
+    load_blocks<false>(t_at, R + r0, R + 16 * k, lane, a[0]);
+    load_blocks<false>(t_at + PART, R + r0, R + 16 * k, lane, a[1]);
+    mma_parts<N / 16>(m, a, a_at, R + 16 * k, C, lane);
+  }
+  float out[2][4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
     for (int e = 0; e < 4; ++e) out[i][e] = 0.f;
 #pragma unroll
-  for (int k = 0; k < N2 / 16; ++k) {
-    FragA a;
+  for (int k = 0; k < N / 16; ++k) {
+    uint32_t a[2][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      split_pair(-m[2 * k + i / 2][2 * (i & 1)], -m[2 * k + i / 2][2 * (i & 1) + 1], &a.p[0][i], &a.p[1][i]);
-    FragB b[N / 8];
+    for (int i = 0; i < 4; ++i) {
+      float x = -m[2 * k + i / 2][2 * (i & 1)], y = -m[2 * k + i / 2][2 * (i & 1) + 1];
+      a[0][i] = take_part(x, y);
+      a[1][i] = take_part(x, y);
+    }
+    mma_parts<1>(out, a, t_at, C + 16 * k, C + c0, lane);
+  }
 #pragma unroll
-    for (int i = 0; i < N / 8; ++i) b[i] = load_frag_b(t11 + 16 * k * INV_LD + c0 + 8 * i, lane);
-    mma_parts(out, a, b);
-  }
-}
-
-template <int N>
-__device__ __forceinline__ void store_rows(float* x, int lane, const float (&m)[N / 8][4]) {
-  float* at = x + (lane / 4) * INV_LD + 2 * (lane % 4);
+  for (int part = 0; part < 2; ++part)
 #pragma unroll
-  for (int i = 0; i < N / 8; ++i) {
-    *reinterpret_cast<float2*>(at + 8 * i) = make_float2(m[i][0], m[i][1]);
-    *reinterpret_cast<float2*>(at + 8 * INV_LD + 8 * i) = make_float2(m[i][2], m[i][3]);
-  }
-}
-
-// The rest of the 64 x 64 inverse from its diagonal blocks of 16, by the 4
-// preparing warps: T21 = -(T22 A21) T11 for blocks of 16, then of 32.  On the
-// register form of the tensor instructions: at 16 and 32 rows a TMEM round
-// trip would cost more than the products, and fp32 FMAs fed from shared
-// memory (measured: 3300 cycles) held up the state's products, whose operands
-// come from there too.
-__device__ __forceinline__ void invert_join(float* a, int warp, int lane) {
-  constexpr int L = INV_LD;
-  if (warp < 2) {
-    float* t11 = a + warp * 32 * (L + 1);
-    float m[2][4];
-    join_rows<16, 16>(t11 + 16 * (L + 1), t11 + 16 * L, t11, 0, 0, lane, m);
-    __syncwarp();
-    store_rows<16>(t11 + 16 * L, lane, m);
-  }
-  named_bar_sync(1, C_PREP);
-  const int r0 = (warp / 2) * 16, c0 = (warp % 2) * 16;
-  float m[2][4];
-  join_rows<32, 16>(a + 32 * (L + 1), a + 32 * L, a, r0, c0, lane, m);
-  named_bar_sync(1, C_PREP);
-  store_rows<16>(a + (32 + r0) * L + c0, lane, m);
-  named_bar_sync(1, C_PREP);
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; e += 2)
+        *reinterpret_cast<uint32_t*>(t + part * PART +
+                                     part_at(R + r0 + lane / 4 + 4 * e, C + c0 + 8 * i + 2 * (lane % 4))) =
+            take_part(out[i][e], out[i][e + 1]);
 }
 
 __device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
@@ -564,11 +554,17 @@ __global__ void __launch_bounds__(C_THREADS, 1)
     mbar_init(&bars.d3_done, 1);
     mbar_init(&bars.delta_ready, C_STATE);
     mbar_init(&bars.d4_done, 1);
+    mbar_init(&bars.q_done, 1);
     mbar_init(&bars.y_done, 1);
     mbar_init(&bars.y_read, C_STATE);
     abort_word = 0;
     fence_barrier_init();
   }
+  // T above its diagonal blocks stays 0; everything else is written per chunk
+  for (int i = threadIdx.x; i < 2 * 2 * PART / 16; i += C_THREADS)
+    *reinterpret_cast<uint4*>(smem + C::TP_OFF + (i / (2 * PART / 16)) * C::TP_BYTES + (i % (2 * PART / 16)) * 16) =
+        make_uint4(0, 0, 0, 0);
+  fence_proxy_async_shared();
   if (warp == 12) {
     tmem_alloc(&tmem_slot, 512);
     tmem_relinquish();
@@ -631,7 +627,9 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       if (c >= 2) wait(&bars.tp_freed[ts], (c / 2) - 1);
       const float* gs = g_of(s);
       uint8_t* tp = smem + C::TP_OFF + ts * C::TP_BYTES;
-      float* am = reinterpret_cast<float*>(tp);
+      uint8_t* ap = smem + C::A_OFF;
+      float* diag = reinterpret_cast<float*>(ap + 2 * PART);
+      float* nowhere = diag + 4 * DIAG_BLK + lane * 8;
       // D_ij along the row, from the diagonal to the left, times beta_i in A's
       // rows; right of the diagonal d is 0 (what A's diagonal holds is not read)
       const float start = t < 64 ? b_of(s)[i] : 1.f;
@@ -653,20 +651,24 @@ __global__ void __launch_bounds__(C_THREADS, 1)
           ghi = at4(gs + j8 - 4);
         }
         if (t < 64) {
-          *reinterpret_cast<float4*>(am + i * INV_LD + j8) = make_float4(o[0], o[1], o[2], o[3]);
-          *reinterpret_cast<float4*>(am + i * INV_LD + j8 + 4) = make_float4(o[4], o[5], o[6], o[7]);
-        } else {
-          uint4 u;
-          u.x = take_part(o[0], o[1]);
-          u.y = take_part(o[2], o[3]);
-          u.z = take_part(o[4], o[5]);
-          u.w = take_part(o[6], o[7]);
-          *reinterpret_cast<uint4*>(tp + C::T_BYTES + i * 128 + (((j8 / 8) ^ (i & 7)) * 16)) = u;
+          // A's block on the diagonal in fp32, what lies left of it in parts.
+          // Lanes of a warp differ in which of the two a column is: each store
+          // has a place for lanes that it is not for, so that no branch splits
+          // the warp.
+          float* at = j8 / 16 == i / 16 ? diag + (i / 16) * DIAG_BLK + (i % 16) * DIAG_LD + j8 % 16 : nowhere;
+          *reinterpret_cast<float4*>(at) = make_float4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<float4*>(at + 4) = make_float4(o[4], o[5], o[6], o[7]);
+        }
+        if (t >= 64 || j8 < 48) {
+          uint8_t* at = t >= 64 ? tp + 2 * PART + part_at(i, j8)
+                                : (j8 / 16 < i / 16 ? ap + part_at(i, j8) : reinterpret_cast<uint8_t*>(nowhere));
+          *reinterpret_cast<uint4*>(at) = take_part8(o);
+          if (t < 64) *reinterpret_cast<uint4*>(j8 / 16 < i / 16 ? at + PART : at) = take_part8(o);
         }
       }
       if (t < 64) {
         __syncwarp();
-        invert_block16(am + (t / 16) * 16 * (INV_LD + 1), t % 16);
+        invert_block16(diag + (t / 16) * DIAG_BLK, tp, t / 16, t % 16);
       } else {
         // c_i (warp 2) and D_63,j (warp 3): products of the decays up to a step
         // and behind it, two steps per lane
@@ -700,31 +702,16 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       if (c + 1 < chunks) publish(c + 1);
       if (c + 2 < chunks) fetch(c + 2);
       named_bar_sync(1, C_PREP);
-      invert_join(am, warp, lane);
-      // T - I in two parts over the same memory: half a row per thread
-      {
-        const int r = t / 2, c0 = (t % 2) * 32;
-        float x[32];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const float4 y = at4(am + r * INV_LD + c0 + 4 * q);
-          x[4 * q] = y.x; x[4 * q + 1] = y.y; x[4 * q + 2] = y.z; x[4 * q + 3] = y.w;
-        }
-#pragma unroll
-        for (int q = 0; q < 32; ++q) x[q] = c0 + q == r ? 0.f : x[q];
-        named_bar_sync(1, C_PREP);
-#pragma unroll
-        for (int part = 0; part < 2; ++part)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint4 u;
-            u.x = take_part(x[8 * q], x[8 * q + 1]);
-            u.y = take_part(x[8 * q + 2], x[8 * q + 3]);
-            u.z = take_part(x[8 * q + 4], x[8 * q + 5]);
-            u.w = take_part(x[8 * q + 6], x[8 * q + 7]);
-            *reinterpret_cast<uint4*>(tp + part * CH * 128 + r * 128 + (((c0 / 8 + q) ^ (r & 7)) * 16)) = u;
-          }
-      }
+      // The rest of the inverse from its diagonal blocks: blocks of 16, then of
+      // 32.  On the register form of the tensor instructions: at these sizes a
+      // TMEM round trip would cost more than the products.
+      const uint32_t t_at = smem_u32(tp), a_at = smem_u32(ap);
+      if (warp < 2) join_block<16>(tp, t_at, a_at, 32 * warp + 16, 32 * warp, 0, 0, lane);
+      named_bar_sync(1, C_PREP);
+      join_block<32>(tp, t_at, a_at, 32, 0, (warp / 2) * 16, (warp % 2) * 16, lane);
+      named_bar_sync(1, C_PREP);
+      // T - I goes into the products
+      if (t < 64) *reinterpret_cast<uint16_t*>(tp + part_at(t, t)) = 0;
       fence_proxy_async_shared();
       mbar_arrive(&bars.tp_full[ts]);
     }
@@ -755,21 +742,13 @@ __global__ void __launch_bounds__(C_THREADS, 1)
     tmem_st_wait();
     tc_fence_before();
     mbar_arrive(&bars.s_ready);
-    const size_t y_step = (size_t)p.Hv * p.Dv;
-    __nv_bfloat16* out = p.y + ((first + h * 32) * p.Hv + hv) * p.Dv + dv0 + row;
-    for (int c = 0; c < chunks; ++c) {
-      const int st = c % C_STAGES, ts = c % 2;
-      uint32_t d[2][16];
-      // R = beta (V - c K S^T); beta V while the product runs.  Coefficients
-      // come 16 at a time, ahead of the stores that the compiler keeps loads behind.
-      wait(&bars.tp_full[ts], c / 2);
+    float r[32];
+    auto beta_v = [&](int c) {               // r = beta V of chunk c
+      const int st = c % C_STAGES;
+      wait(&bars.full[st], c / C_STAGES);
       const __nv_bfloat16* vt =
           reinterpret_cast<const __nv_bfloat16*>(smem + st * C::STAGE_BYTES + C::KQ_BYTES) + h * 32 * 128 + row;
       const float* bs = b_of(st) + h * 32;
-      const float* cs = cum_of(ts) + h * 32;
-      const float* us = until_of(ts) + h * 32;
-      const float* nbc = nbc_of(ts) + h * 32;
-      float r[32];
 #pragma unroll
       for (int j = 0; j < 32; j += 4) {
         const float4 be = at4(bs + j);
@@ -778,6 +757,19 @@ __global__ void __launch_bounds__(C_THREADS, 1)
         r[j + 2] = be.z * __bfloat162float(vt[(j + 2) * 128]);
         r[j + 3] = be.w * __bfloat162float(vt[(j + 3) * 128]);
       }
+    };
+    beta_v(0);
+    const size_t y_step = (size_t)p.Hv * p.Dv;
+    __nv_bfloat16* out = p.y + ((first + h * 32) * p.Hv + hv) * p.Dv + dv0 + row;
+    for (int c = 0; c < chunks; ++c) {
+      const int ts = c % 2;
+      uint32_t d[2][16];
+      // R = beta V - beta c K S^T.  Coefficients come 16 at a time, ahead of the
+      // stores that the compiler keeps loads behind.
+      wait(&bars.tp_full[ts], c / 2);
+      const float* cs = cum_of(ts) + h * 32;
+      const float* us = until_of(ts) + h * 32;
+      const float* nbc = nbc_of(ts) + h * 32;
       float co[16];
       load16(nbc, co);
       wait(&bars.d1_done, c);
@@ -804,6 +796,7 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       mbar_arrive(&bars.r_ready);
       // Delta = R + (T - I) R, as it is (for y) and weighed for the state
       load16(us, co);
+      wait(&bars.q_done, c);                 // S Q^T has read the state that the parts of Delta go over
       wait(&bars.d3_done, c);
       tc_fence_after();
       tmem_ld_32x32b_x16(ta + C::COL_D + h * 32, d[0]);
@@ -828,6 +821,7 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       mbar_arrive(&bars.delta_ready);
       // S <- c_63 S + Delta K
       const float keep = cum_of(ts)[CH - 1];
+      if (c + 1 < chunks) beta_v(c + 1);     // while the product runs
       wait(&bars.d4_done, c);
       tc_fence_after();
       tmem_ld_32x32b_x16(ta + C::COL_D + h * NS, d[0]);
@@ -885,101 +879,107 @@ __global__ void __launch_bounds__(C_THREADS, 1)
   } else {
     // ----------------------------------------------------- loads and products
     fewer_registers<C_REGS_ISSUE>();
-    if (warp == 12) {   // the whole warp walks along, one elected lane issues
+    // The whole warp walks along, one elected lane issues.  The chain from one
+    // state to the next and what only has to be done beside it are issued by
+    // two warps; a product that reads what the other's wrote, or writes what it
+    // read, comes after a wait that covers it.
     constexpr uint32_t ID64 = make_idesc_bf16(128, 64);
     constexpr uint32_t IDK = make_idesc_bf16(128, DK) | kIdescBTransposed;
-    auto load = [&](int c) {
-      const int s = c % C_STAGES;
-      uint8_t* kq = smem + s * C::STAGE_BYTES;
-      const int tok = int(first) + c * CH;
-      if (lane != 0) return;
-      mbar_arrive_expect_tx(&bars.loaded[s], C::STAGE_BYTES);
-      for (int a = 0; a < DK / 64; ++a) {
-        tma_load_2d(kq + a * C::ATOM, &tm_k, &bars.loaded[s], hk * DK + a * 64, tok);
-        tma_load_2d(kq + a * C::ATOM + 64 * 128, &tm_q, &bars.loaded[s], hk * DK + a * 64, tok);
-      }
-      tma_load_2d(kq + C::KQ_BYTES, &tm_v, &bars.loaded[s], hv * p.Dv + dv0, tok);
-    };
-    auto kq_desc = [&](int s, int row, int k) {   // 16 columns from 16 k on
-      return make_sw128_desc(smem_base + s * C::STAGE_BYTES + (k / 4) * C::ATOM + row * 128 + (k % 4) * 32);
-    };
-    auto grams = [&](int c) {   // [K; Q] K^T
-      const int s = c % C_STAGES;
-      wait(&bars.full[s], c / C_STAGES);
-#pragma unroll
-      for (int k = 0; k < DK / 16; ++k)
-        mma_bf16_ss_warp(tmem + C::COL_G, kq_desc(s, 0, k), kq_desc(s, 0, k), ID64, k > 0);
-      tc_commit_warp(&bars.g_full);
-    };
-    for (int c = 0; c < min(chunks, 2); ++c) load(c);
-    __syncwarp();
-    grams(0);
-    for (int c = 0; c < chunks; ++c) {
-      const int s = c % C_STAGES, ts = c % 2;
-      const uint32_t tp = smem_base + C::TP_OFF + ts * C::TP_BYTES;
-      wait(&bars.s_ready, c);
-      tc_fence_after();
-#pragma unroll
-      for (int part = 0; part < 3; ++part)
-#pragma unroll
-        for (int k = 0; k < DK / 16; ++k)
-          mma_bf16_ts_warp(tmem + C::COL_D, tmem + C::COL_S + part * C::S_PART + k * 8, kq_desc(s, 0, k), ID64,
-                      part + k > 0);
-      tc_commit_warp(&bars.d1_done);
-      // the second half of Delta K's columns is free until this chunk's Delta K
-      if (c + 1 < chunks) {
-        if (c == 0) wait(&bars.g_read, 0);   // later ones were waited for before the last Delta K
-        grams(c + 1);
-      }
-      // chunk c - 1 is done with its stage: its products are complete and its
-      // values read (s_ready comes after both)
-      if (c + 2 < chunks) load(c + 2);
-      __syncwarp();
-      if (c > 0) {
-        wait(&bars.y_read, c - 1);
+    if (warp == 12) {
+      for (int c = 0; c < chunks; ++c) {
+        const int ts = c % 2;
+        const uint32_t kq = smem_base + (c % C_STAGES) * C::STAGE_BYTES;
+        const uint32_t tp = smem_base + C::TP_OFF + ts * C::TP_BYTES;
+        wait(&bars.full[c % C_STAGES], c / C_STAGES);
+        wait(&bars.s_ready, c);
         tc_fence_after();
+#pragma unroll
+        for (int part = 0; part < 3; ++part)
+#pragma unroll
+          for (int a = 0; a < DK / 64; ++a)
+            mma_bf16_ts_warp_x4<2>(tmem + C::COL_D, tmem + C::COL_S + part * C::S_PART + a * 32,
+                                   make_sw128_desc(kq + a * C::ATOM), ID64, part + a > 0);
+        tc_commit_warp(&bars.d1_done);
+        wait(&bars.tp_full[ts], c / 2);
+        wait(&bars.r_ready, c);
+        tc_fence_after();
+        // first parts, then second part x first part both ways round
+#pragma unroll
+        for (int m = 0; m < 3; ++m)
+          mma_bf16_ts_warp_x4<2>(tmem + C::COL_D, tmem + C::COL_R + (m == 1 ? 32 : 0),
+                                 make_sw128_desc(tp + (m == 2 ? PART : 0)), ID64, m > 0);
+        tc_commit_warp(&bars.d3_done);
+        wait(&bars.delta_ready, c);
+        // [K; Q] K^T of the next chunk has left the second half of these columns
+        if (c + 1 < chunks) wait(&bars.g_read, c + 1);
+        tc_fence_after();
+#pragma unroll
+        for (int part = 0; part < 3; ++part)
+          mma_bf16_ts_warp_x4<128>(tmem + C::COL_D, tmem + C::COL_S + part * 32, make_sw128_mn_desc(kq, C::ATOM), IDK,
+                                   part > 0);
+        tc_commit_warp(&bars.d4_done);
       }
+    } else if (warp == 14) {
+      auto grams = [&](int c) {   // [K; Q] K^T
+        const uint32_t kq = smem_base + (c % C_STAGES) * C::STAGE_BYTES;
+        wait(&bars.full[c % C_STAGES], c / C_STAGES);
 #pragma unroll
-      for (int part = 0; part < 2; ++part)
+        for (int a = 0; a < DK / 64; ++a)
+          mma_bf16_ss_warp_x4(tmem + C::COL_G, make_sw128_desc(kq + a * C::ATOM), make_sw128_desc(kq + a * C::ATOM), ID64,
+                              a > 0);
+        tc_commit_warp(&bars.g_full);
+      };
+      grams(0);
+      wait(&bars.g_read, 0);
+      for (int c = 0; c < chunks; ++c) {
+        const int ts = c % 2;
+        const uint32_t kq = smem_base + (c % C_STAGES) * C::STAGE_BYTES;
+        const uint32_t tp = smem_base + C::TP_OFF + ts * C::TP_BYTES;
+        wait(&bars.s_ready, c);
+        // the last chunk's Delta K has been read, its second half is free until
+        // this chunk's
+        tc_fence_after();
+        if (c + 1 < chunks) grams(c + 1);
+        if (c > 0) wait(&bars.y_read, c - 1);
+        tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < DK / 16; ++k)
-          mma_bf16_ts_warp(tmem + C::COL_SQ, tmem + C::COL_S + part * C::S_PART + k * 8, kq_desc(s, 64, k), ID64,
-                      part + k > 0);
-      wait(&bars.tp_full[ts], c / 2);
-      wait(&bars.r_ready, c);
-      tc_fence_after();
-      // first parts, then second part x first part both ways round
+        for (int part = 0; part < 2; ++part)
 #pragma unroll
-      for (int m = 0; m < 3; ++m)
-#pragma unroll
-        for (int k = 0; k < CH / 16; ++k)
-          mma_bf16_ts_warp(tmem + C::COL_D, tmem + C::COL_R + (m == 1 ? 32 : 0) + k * 8,
-                      make_sw128_desc(tp + (m == 2 ? CH * 128 : 0) + k * 32), ID64, m + k > 0);
-      tc_commit_warp(&bars.d3_done);
-      wait(&bars.delta_ready, c);
-      if (c + 1 < chunks) wait(&bars.g_read, c + 1);
-      tc_fence_after();
-#pragma unroll
-      for (int part = 0; part < 3; ++part)
-#pragma unroll
-        for (int k = 0; k < CH / 16; ++k)
-          mma_bf16_ts_warp(tmem + C::COL_D, tmem + C::COL_S + part * 32 + k * 8,
-                      make_sw128_mn_desc(smem_base + s * C::STAGE_BYTES + k * 16 * 128, C::ATOM), IDK,
-                      part + k > 0);
-      tc_commit_warp(&bars.d4_done);
-#pragma unroll
-      for (int k = 0; k < CH / 16; ++k)
-        mma_bf16_ts_warp(tmem + C::COL_Y, tmem + C::COL_R + k * 8, make_sw128_desc(tp + C::T_BYTES + k * 32), ID64, k > 0);
-      tc_commit_warp(&bars.y_done);
-      tc_commit_warp(&bars.tp_freed[ts]);
-    }
-    // every commit's arrival has landed before the CTA gives its memory back
-    // (the other commits' were waited for by the state's threads)
-    for (int c = max(0, chunks - 2); c < chunks; ++c) wait(&bars.tp_freed[c % 2], c / 2);
-    if (abort_word) {
-      // a wait ran out: let the copies in flight land before the CTA leaves
-      for (int c = max(0, chunks - C_STAGES); c < chunks; ++c) mbar_wait(&bars.loaded[c % C_STAGES], (c / C_STAGES) & 1);
-    }
+          for (int a = 0; a < DK / 64; ++a)
+            mma_bf16_ts_warp_x4<2>(tmem + C::COL_SQ, tmem + C::COL_S + part * C::S_PART + a * 32,
+                                   make_sw128_desc(kq + 64 * 128 + a * C::ATOM), ID64, part + a > 0);
+        tc_commit_warp(&bars.q_done);
+        wait(&bars.delta_ready, c);
+        tc_fence_after();
+        mma_bf16_ts_warp_x4<2>(tmem + C::COL_Y, tmem + C::COL_R, make_sw128_desc(tp + 2 * PART), ID64, 0);
+        tc_commit_warp(&bars.y_done);
+        tc_commit_warp(&bars.tp_freed[ts]);
+      }
+      // the last arrivals land before the CTA gives its memory back (the other
+      // commits' were waited for by the state's threads)
+      for (int c = max(0, chunks - 2); c < chunks; ++c) wait(&bars.tp_freed[c % 2], c / 2);
+    } else if (warp == 13 && lane == 0) {
+      // loads, on a thread of their own: issuing a chunk's five takes about as
+      // long (2000 cycles) as a round of products
+      for (int c = 0; c < chunks; ++c) {
+        // chunk c - 3 is done with the stage: its products are complete and its
+        // values read (the next state came after both).  Every phase is waited
+        // for in turn: a parity alone does not tell phase 1 from none.
+        if (c == C_STAGES) wait(&bars.s_ready, 0);
+        if (c >= C_STAGES) wait(&bars.s_ready, c - C_STAGES + 1);
+        uint8_t* kq = smem + (c % C_STAGES) * C::STAGE_BYTES;
+        uint64_t* bar = &bars.loaded[c % C_STAGES];
+        const int tok = int(first) + c * CH;
+        mbar_arrive_expect_tx(bar, C::STAGE_BYTES);
+        for (int a = 0; a < DK / 64; ++a) {
+          tma_load_2d(kq + a * C::ATOM, &tm_k, bar, hk * DK + a * 64, tok);
+          tma_load_2d(kq + a * C::ATOM + 64 * 128, &tm_q, bar, hk * DK + a * 64, tok);
+        }
+        tma_load_2d(kq + C::KQ_BYTES, &tm_v, bar, hv * p.Dv + dv0, tok);
+      }
+      // whatever went wrong elsewhere, no copy is in flight when the CTA leaves
+      for (int c = max(0, chunks - C_STAGES); c < chunks; ++c)
+        mbar_wait(&bars.loaded[c % C_STAGES], (c / C_STAGES) & 1);
     }
   }
   __syncwarp();
