@@ -253,7 +253,10 @@ constexpr int C_REGS_STATE = 168, C_REGS_ISSUE = 48;
 constexpr int C_ORDER = 256;         // packed sequences that are taken longest first
 constexpr int C_STAGES = 3;
 constexpr int C_PREP = 128, C_STATE = 256;
-constexpr int DIAG_LD = 20, DIAG_BLK = 16 * DIAG_LD + 4;   // floats: a row and a block of A's diagonal blocks
+// A in fp32, floats of a row and of a block: blocks 0-3 on the diagonal (16 x
+// 16), 4 and 5 left of blocks 1 and 3, then the 32 x 32 block at (32, 0).
+constexpr int DIAG_LD = 20, DIAG_BLK = 16 * DIAG_LD + 4, OFF_LD = 36;
+constexpr int A32_FLOATS = 6 * DIAG_BLK + 32 * OFF_LD;
 constexpr int PART = CH * 128;       // bytes of one bf16 part of a 64 x 64 matrix, 128-byte swizzle
 
 template <int DK>
@@ -264,10 +267,11 @@ struct CCfg {
   static constexpr int STAGE_BYTES = KQ_BYTES + V_BYTES;
   static constexpr int TP_BYTES = 3 * PART;              // T's two parts and P
   static constexpr int TP_OFF = C_STAGES * STAGE_BYTES;
-  static constexpr int A_OFF = TP_OFF + 2 * TP_BYTES;    // A's two parts, its diagonal blocks in fp32, a place for stores to nowhere
-  static constexpr int SMALL_OFF = A_OFF + 2 * PART + 4 * DIAG_BLK * 4 + 1024;
+  static constexpr int A_OFF = TP_OFF + 2 * TP_BYTES;    // A's two parts, A in fp32, a place for stores to nowhere
+  static constexpr int SMALL_OFF = A_OFF + 2 * PART + A32_FLOATS * 4 + 1024;
   static constexpr int SMALL_BYTES = (C_STAGES * 2 + 2 * 3) * CH * 4;
   static constexpr int SMEM_BYTES = SMALL_OFF + SMALL_BYTES + 1024;
+  static_assert(SMEM_BYTES + 1024 <= 227 * 1024, "with the barriers, what a CTA can have");
   // TMEM columns
   static constexpr int S_PART = DK / 2;                  // columns of one part of the state
   static constexpr int COL_S = 0;                        // state parts; later Delta K's three parts
@@ -489,7 +493,7 @@ __global__ void __launch_bounds__(C_THREADS, 1)
   __shared__ ChunkBars bars;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_word;
-  __shared__ int lens[C_ORDER], chosen;
+  __shared__ int chosen;
 
   const int tiles = (p.Dv + 127) / 128;
   const int dv0 = (blockIdx.x % tiles) * 128;
@@ -499,6 +503,7 @@ __global__ void __launch_bounds__(C_THREADS, 1)
     // Longest sequences first: a CTA's time goes by its chunks, and a long one
     // that starts late would run on alone.
     const int t = threadIdx.x;
+    int* lens = reinterpret_cast<int*>(smem_raw);
     if (t < p.B) lens[t] = p.cu[t + 1] - p.cu[t];
     __syncthreads();
     if (t < p.B) {
@@ -560,10 +565,9 @@ __global__ void __launch_bounds__(C_THREADS, 1)
     abort_word = 0;
     fence_barrier_init();
   }
-  // T above its diagonal blocks stays 0; everything else is written per chunk
-  for (int i = threadIdx.x; i < 2 * 2 * PART / 16; i += C_THREADS)
-    *reinterpret_cast<uint4*>(smem + C::TP_OFF + (i / (2 * PART / 16)) * C::TP_BYTES + (i % (2 * PART / 16)) * 16) =
-        make_uint4(0, 0, 0, 0);
+  // T and P above their diagonal blocks stay 0; the rest is written per chunk
+  for (int i = threadIdx.x; i < 2 * C::TP_BYTES / 16; i += C_THREADS)
+    *reinterpret_cast<uint4*>(smem + C::TP_OFF + i * 16) = make_uint4(0, 0, 0, 0);
   fence_proxy_async_shared();
   if (warp == 12) {
     tmem_alloc(&tmem_slot, 512);
@@ -629,47 +633,72 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       uint8_t* tp = smem + C::TP_OFF + ts * C::TP_BYTES;
       uint8_t* ap = smem + C::A_OFF;
       float* diag = reinterpret_cast<float*>(ap + 2 * PART);
-      float* nowhere = diag + 4 * DIAG_BLK + lane * 8;
+      float* off32 = diag + 6 * DIAG_BLK;
+      float* nowhere = off32 + 32 * OFF_LD + lane * 8;
       // D_ij along the row, from the diagonal to the left, times beta_i in A's
       // rows; right of the diagonal d is 0 (what A's diagonal holds is not read)
       const float start = t < 64 ? b_of(s)[i] : 1.f;
+      // A's row in fp32: lanes of a warp differ in which block a column is in,
+      // and lanes that a store is not for have a place for it, so that no
+      // branch splits the warp
+      const int blk = i / 16;
+      float* row_diag = diag + blk * DIAG_BLK + (i % 16) * DIAG_LD;
+      float* row_odd = blk & 1 ? row_diag : nowhere;                                  // columns of block 1 or 3
+      float* row_even = blk & 1 ? row_diag + (4 + blk / 2 - blk) * DIAG_BLK : row_diag;  // of block 0 or 2
       float d = 0.f, next = 0.f;
       float4 glo = at4(gs + CH - 8), ghi = at4(gs + CH - 4);
 #pragma unroll
       for (int j8 = CH - 8; j8 >= 0; j8 -= 8) {
-        const float gg[8] = {glo.x, glo.y, glo.z, glo.w, ghi.x, ghi.y, ghi.z, ghi.w};
-        float o[8];
+        if (j8 < 32 || (warp & 1)) {   // the first 32 rows end with column 31
+          const float gg[8] = {glo.x, glo.y, glo.z, glo.w, ghi.x, ghi.y, ghi.z, ghi.w};
+          float o[8];
 #pragma unroll
-        for (int e = 7; e >= 0; --e) {
-          const int j = j8 + e;
-          d = j == i ? start : d * next;
-          next = gg[e];
-          o[e] = d * __uint_as_float(gr[j / 32][j % 32]);
-        }
-        if (j8 > 0) {   // before the stores, which it must not wait for
-          glo = at4(gs + j8 - 8);
-          ghi = at4(gs + j8 - 4);
-        }
-        if (t < 64) {
-          // A's block on the diagonal in fp32, what lies left of it in parts.
-          // Lanes of a warp differ in which of the two a column is: each store
-          // has a place for lanes that it is not for, so that no branch splits
-          // the warp.
-          float* at = j8 / 16 == i / 16 ? diag + (i / 16) * DIAG_BLK + (i % 16) * DIAG_LD + j8 % 16 : nowhere;
-          *reinterpret_cast<float4*>(at) = make_float4(o[0], o[1], o[2], o[3]);
-          *reinterpret_cast<float4*>(at + 4) = make_float4(o[4], o[5], o[6], o[7]);
-        }
-        if (t >= 64 || j8 < 48) {
-          uint8_t* at = t >= 64 ? tp + 2 * PART + part_at(i, j8)
-                                : (j8 / 16 < i / 16 ? ap + part_at(i, j8) : reinterpret_cast<uint8_t*>(nowhere));
-          *reinterpret_cast<uint4*>(at) = take_part8(o);
-          if (t < 64) *reinterpret_cast<uint4*>(j8 / 16 < i / 16 ? at + PART : at) = take_part8(o);
+          for (int e = 7; e >= 0; --e) {
+            const int j = j8 + e;
+            d = j == i ? start : d * next;
+            next = gg[e];
+            o[e] = d * __uint_as_float(gr[j / 32][j % 32]);
+          }
+          if (j8 > 0) {   // before the stores, which it must not wait for
+            glo = at4(gs + j8 - 8);
+            ghi = at4(gs + j8 - 4);
+          }
+          if (t >= 64) {
+            *reinterpret_cast<uint4*>(tp + 2 * PART + part_at(i, j8)) = take_part8(o);
+          } else {
+            float* at = warp == 1 && j8 < 32 ? off32 + (i - 32) * OFF_LD + j8
+                                             : ((j8 / 16) & 1 ? row_odd : row_even) + (j8 % 16);
+            *reinterpret_cast<float4*>(at) = make_float4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<float4*>(at + 4) = make_float4(o[4], o[5], o[6], o[7]);
+          }
+        } else if (j8 == 32) {
+          glo = at4(gs + 24);
+          ghi = at4(gs + 28);
         }
       }
+      named_bar_sync(1, C_PREP);
       if (t < 64) {
-        __syncwarp();
         invert_block16(diag + (t / 16) * DIAG_BLK, tp, t / 16, t % 16);
       } else {
+        // what lies left of the diagonal blocks, in parts
+        {
+          const int r = (t - 64) / 2, c0 = (t % 2) * 16;
+          float x[16];
+          load16(off32 + r * OFF_LD + c0, x);
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            *reinterpret_cast<uint4*>(ap + part * PART + part_at(32 + r, c0)) = take_part8(x);
+            *reinterpret_cast<uint4*>(ap + part * PART + part_at(32 + r, c0 + 8)) = take_part8(x + 8);
+          }
+          const int b = (t - 64) / 32, rb = (t % 32) / 2, cb = (t % 2) * 8;
+          const float* src = diag + (4 + b) * DIAG_BLK + rb * DIAG_LD + cb;
+          const float4 lo = at4(src), hi = at4(src + 4);
+          x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w;
+          x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
+#pragma unroll
+          for (int part = 0; part < 2; ++part)
+            *reinterpret_cast<uint4*>(ap + part * PART + part_at(32 * b + 16 + rb, 32 * b + cb)) = take_part8(x);
+        }
         // c_i (warp 2) and D_63,j (warp 3): products of the decays up to a step
         // and behind it, two steps per lane
         const float2 gg = *reinterpret_cast<const float2*>(gs + 2 * lane);
@@ -760,7 +789,7 @@ __global__ void __launch_bounds__(C_THREADS, 1)
     };
     beta_v(0);
     const size_t y_step = (size_t)p.Hv * p.Dv;
-    __nv_bfloat16* out = p.y + ((first + h * 32) * p.Hv + hv) * p.Dv + dv0 + row;
+    __nv_bfloat16* out = p.y + ((first + h * 32) * p.Hv + hv) * p.Dv + dv0;
     for (int c = 0; c < chunks; ++c) {
       const int ts = c % 2;
       uint32_t d[2][16];
@@ -838,33 +867,44 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&bars.s_ready);
-      // Y = c Q S^T + P Delta, while the next chunk's K S^T runs
+      // Y = c Q S^T + P Delta, while the next chunk's K S^T runs.  Steps are rows
+      // of y and value rows its columns: the tile is turned in shared memory, so
+      // that y goes out 16 bytes a lane (2-byte stores straight from the lanes
+      // took 2700 cycles of a chunk's 10000 with every SM at work).  It lies
+      // over the next chunk's V, which every thread has read before s_ready.
       wait(&bars.y_done, c);
       tc_fence_after();
-      const int rows = min(CH, len - c * CH) - h * 32;
+      load16(cs, co);
+      tmem_ld_32x32b_x16(ta + C::COL_SQ + h * 32, d[0]);
+      tmem_ld_32x32b_x16(ta + C::COL_Y + h * 32, d[1]);
+      wait(&bars.s_ready, c + 1);
+      uint8_t* yt = smem + ((c + 1) % C_STAGES) * C::STAGE_BYTES + C::KQ_BYTES + h * 32 * 256;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        tmem_ld_32x32b_x16(ta + C::COL_SQ + h * 32 + 16 * b, d[0]);
-        tmem_ld_32x32b_x16(ta + C::COL_Y + h * 32 + 16 * b, d[1]);
-        load16(cs + 16 * b, co);
         tmem_ld_wait();
-        if (b == 1) {
-          tc_fence_before();
-          mbar_arrive(&bars.y_read);
-        }
-        __nv_bfloat16* o = out + 16 * b * y_step;
         __nv_bfloat16 y[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j)
           y[j] = __float2bfloat16_rn(__fmaf_rn(co[j], __uint_as_float(d[0][j]), __uint_as_float(d[1][j])));
-        if (live && rows >= 16 * b + 16) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) o[j * y_step] = y[j];
-        } else if (live) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (16 * b + j < rows) o[j * y_step] = y[j];
+        if (b == 0) {
+          load16(cs + 16, co);
+          tmem_ld_32x32b_x16(ta + C::COL_SQ + h * 32 + 16, d[0]);
+          tmem_ld_32x32b_x16(ta + C::COL_Y + h * 32 + 16, d[1]);
+        } else {
+          tc_fence_before();
+          mbar_arrive(&bars.y_read);
         }
+        __nv_bfloat16* at = reinterpret_cast<__nv_bfloat16*>(yt + 16 * b * 256) + row;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) at[j * 128] = y[j];
+      }
+      named_bar_sync(2 + h, C_STATE / 2);
+      const int rows = min(CH, len - c * CH) - h * 32;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int rr = (warp % 4) * 8 + 2 * i + lane / 16, x = lane % 16;
+        const uint4 u = *reinterpret_cast<const uint4*>(yt + rr * 256 + x * 16);
+        if (rr < rows && x * 8 < cols) *reinterpret_cast<uint4*>(out + rr * y_step + x * 8) = u;
       }
       out += CH * y_step;
       __syncwarp();
