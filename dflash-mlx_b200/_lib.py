@@ -120,6 +120,8 @@ class DflashError(RuntimeError):
 def load(path: Path | None = None) -> ctypes.CDLL:
     """Load (once) and return the library, with argtypes set for every symbol."""
     global _lib
+    if path is None and _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None and path is None:
             return _lib

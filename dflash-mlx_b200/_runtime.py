@@ -7,6 +7,7 @@ launch goes through libdflash_b200.so.
 
 from __future__ import annotations
 
+import contextlib
 import threading
 
 import torch
@@ -17,7 +18,16 @@ _workspaces: dict[tuple[int, int], torch.Tensor] = {}
 
 def stream_ptr(device: torch.device) -> int:
     """Raw cudaStream_t of torch's current stream on ``device``."""
-    return int(torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+_here = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context with ``device`` current; costs nothing where it already is."""
+    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
@@ -68,12 +78,12 @@ def require_cuda(t: torch.Tensor, name: str) -> None:
 
 def same_device(dev: torch.device, **tensors) -> None:
     """Every given tensor (None: left out) is a CUDA tensor on ``dev``."""
+    index = dev.index
     for name, t in tensors.items():
-        if t is None:
+        if t is None or (isinstance(t, torch.Tensor) and t.get_device() == index):
             continue
         require_cuda(t, name)
-        if t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, not on {dev}")
+        raise ValueError(f"{name} is on {t.device}, not on {dev}")
 
 
 def mask_bytes(mask: torch.Tensor, name: str) -> torch.Tensor:

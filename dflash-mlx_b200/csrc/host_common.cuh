@@ -132,11 +132,11 @@ inline int ensure_smem(Kernel kernel, int bytes, int dev, std::atomic<uint64_t>&
 // prologue and its weight loads) while the previous kernel in the stream is
 // still running; it calls griddep_wait() before touching that kernel's outputs.
 template <typename... KArgs, typename... Args>
-inline int launch_pdl(void (*kernel)(KArgs...), int grid, int block, size_t smem,
+inline int launch_pdl(void (*kernel)(KArgs...), dim3 grid, int block, size_t smem,
                       cudaStream_t stream, Args&&... args) {
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;

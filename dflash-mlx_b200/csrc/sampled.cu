@@ -138,10 +138,87 @@ __device__ __forceinline__ void take(Stat& a, float x, int id, float c) {
   a.s += x == INFINITY ? 1.f : exp_scaled(x - a.m, c);
 }
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 16 bytes of logits as floats
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void get(const uint4& u, float (&f)[4]) {
+    f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+  }
+};
+template <>
+struct Vec<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void get(const uint4& u, float (&f)[8]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
+template <>
+struct Vec<__half> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void get(const uint4& u, float (&f)[8]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = x.x;
+      f[2 * i + 1] = x.y;
+    }
+  }
+};
+
+constexpr int MAX_SEG = 32768;
+
+// One bit per id of [v0, v1), set where it is suppressed: 16 mask bytes at a
+// time where they lie on 16-byte borders (v0 does, being a multiple of 16).
+__device__ __forceinline__ void stage_mask(const uint8_t* sup, int v0, int v1, uint16_t* bits) {
+  const int words = (v1 - v0 + 15) / 16;
+  const bool wide = (reinterpret_cast<uintptr_t>(sup) & 15) == 0;
+  for (int i = threadIdx.x; i < words; i += THREADS) {
+    const int v = v0 + 16 * i;
+    uint32_t r = 0;
+    if (wide && v + 16 <= v1) {
+      const uint4 u = *reinterpret_cast<const uint4*>(sup + v);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      // a byte each to 0 or 1, then bits 0, 8, 16, 24 side by side at the top
+      for (int j = 0; j < 4; ++j) r |= ((__vsetne4(w[j], 0) * 0x10204080u) >> 28) << (4 * j);
+    } else {
+      for (int j = 0; j < 16 && v + j < v1; ++j) r |= uint32_t(sup[v + j] != 0) << j;
+    }
+    bits[i] = uint16_t(r);
+  }
+  // a word behind the last is read with it
+  if (threadIdx.x < 4) bits[words + threadIdx.x] = 0;
+}
+
 // Segment blockIdx.x of row blockIdx.y (target rows, then draft rows).
+//
+// Per id: widen, maximum, one FMA for (x - m) c with c = log2(e) / z, ex2, add --
+// 5 instructions; HBM leaves about 8 (measured: see the launch).  m c is rounded
+// once per maximum, a common factor of all terms that is taken out again at
+// the end.  The quick loop takes a vector of ids at a time and moves the
+// maximum rarely; a thread that met NaN or +inf, or nothing above the lowest
+// value, goes over its ids again one by one.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
   __shared__ Stat sh[WARPS];
+  __shared__ uint32_t bits[MAX_SEG / 32 + 4];
+  constexpr int N = Vec<T>::N, U = 4;
+  griddep_launch_dependents();
   const int row = blockIdx.y;
   const bool is_draft = row >= p.B * p.T;
   const int r = is_draft ? row - p.B * p.T : row;
@@ -157,11 +234,92 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
   const T* x = is_draft ? draft_row<T>(p, b, i) : target_row<T>(p, b, i);
   const uint8_t* sup = is_draft ? nullptr : p.suppress;
   const int v0 = blockIdx.x * p.seg, v1 = min(p.V, v0 + p.seg);
-  Stat a{-INFINITY, 0.f, 0x7fffffff};
-  for (int v = v0 + threadIdx.x; v < v1; v += THREADS) {
-    float f = to_f<T>(x[v]);
-    if (sup && sup[v]) f = -INFINITY;
-    take<T>(a, f, v, c);
+  if (sup) {
+    stage_mask(sup, v0, v1, reinterpret_cast<uint16_t*>(bits));
+    __syncthreads();
+  }
+  auto hidden = [&](int v) { return sup && ((bits[(v - v0) / 32] >> ((v - v0) & 31)) & 1u); };
+  // ids up to the first 16-byte border one by one, then vectors, then the rest
+  const int head = min(int((16 - (reinterpret_cast<uintptr_t>(x + v0) & 15)) & 15) / int(sizeof(T)), v1 - v0);
+  const int vecs = (v1 - v0 - head) / N;
+  const int body = v0 + head;
+  Stat a{-FLT_MAX, 0.f, 0x7fffffff};
+  float mc = -FLT_MAX * c;   // may be -inf: replaced before the first term that counts
+  auto raise = [&](float top) {
+    const float was = mc;
+    a.m = top;
+    mc = a.m * c;
+    a.s = a.s > 0.f ? a.s * ex2(was - mc) : 0.f;
+  };
+  for (int k0 = threadIdx.x; k0 < vecs; k0 += THREADS * U) {
+    uint4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k0 + u * THREADS < vecs)
+        raw[u] = __ldg(reinterpret_cast<const uint4*>(x + body) + k0 + u * THREADS);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (k0 + u * THREADS >= vecs) break;
+      const int v = body + (k0 + u * THREADS) * N;
+      float f[N];
+      Vec<T>::get(raw[u], f);
+      if (sup) {
+        const int o = v - v0;
+        const uint32_t off = __funnelshift_r(bits[o / 32], bits[o / 32 + 1], o & 31) & ((1u << N) - 1u);
+        if (off) {
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+            if ((off >> j) & 1u) f[j] = -INFINITY;
+        }
+      }
+      float top = f[0];
+#pragma unroll
+      for (int j = 1; j < N; ++j) top = fmaxf(top, f[j]);
+      if (top == -INFINITY) continue;   // masked whole (a NaN goes on, and into the sum)
+      if (top > a.m) {
+        raise(top);
+#pragma unroll
+        for (int j = N - 1; j >= 0; --j)
+          if (f[j] == top) a.id = v + j;
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) a.s += ex2(__fmaf_rn(f[j], c, -mc));
+    }
+  }
+  // the ragged ends, taken by the first threads
+  const int tail = body + vecs * N;
+  const bool in_head = threadIdx.x < head, in_tail = tail + int(threadIdx.x) < v1;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    if (!(e ? in_tail : in_head)) continue;
+    const int v = (e ? tail : v0) + int(threadIdx.x);
+    const float f = hidden(v) ? -INFINITY : to_f<T>(x[v]);
+    if (f > a.m) {
+      raise(f);
+      a.id = v;
+    } else if (f == a.m) {
+      a.id = min(a.id, v);
+    }
+    a.s += ex2(__fmaf_rn(f, c, -mc));
+  }
+  // the rounding of m c comes out of the sum: 2^d to second order
+  const float d = float(fma(-double(a.m), double(c), double(mc))) * 0.693147181f;
+  a.s = __fmaf_rn(a.s, __fmaf_rn(0.5f * d, d, d), a.s);
+  if (!(a.s > 0.f && fabsf(d) < 1e-3f) || a.id == 0x7fffffff) {
+    a = Stat{-INFINITY, 0.f, 0x7fffffff};
+    if (in_head) {
+      const int v = v0 + int(threadIdx.x);
+      take<T>(a, hidden(v) ? -INFINITY : to_f<T>(x[v]), v, c);
+    }
+    for (int k = threadIdx.x; k < vecs; k += THREADS)
+      for (int j = 0; j < N; ++j) {
+        const int v = body + k * N + j;
+        take<T>(a, hidden(v) ? -INFINITY : to_f<T>(x[v]), v, c);
+      }
+    if (in_tail) {
+      const int v = tail + int(threadIdx.x);
+      take<T>(a, hidden(v) ? -INFINITY : to_f<T>(x[v]), v, c);
+    }
   }
   a = warp_join(a, c);
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = a;
@@ -230,12 +388,32 @@ __device__ __forceinline__ double block_sum(double x, double* sh) {
   return r;
 }
 
+// Exclusive sum over the threads before this one, added in a fixed order.
+__device__ __forceinline__ double before_me(double x, double* sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double run = x;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const double y = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += y;
+  }
+  __syncthreads();
+  if (lane == 31) sh[warp] = run;
+  __syncthreads();
+  double base = 0.0;
+  for (int w = 0; w < warp; ++w) base += sh[w];
+  const double prev = __shfl_up_sync(0xffffffffu, run, 1);
+  return lane == 0 ? base : base + prev;
+}
+
 // Accept (every CTA of a request alike; CTA 0 writes), then the 64-bit sums of
 // segment blockIdx.x of the rows that the next token is drawn from.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) decide_kernel(const Params p) {
   __shared__ int first_bad;
   __shared__ double sh[WARPS];
+  griddep_launch_dependents();
+  griddep_wait();
   const int b = blockIdx.y;
   const int n = draft_len(p, b);
   const float z = clean_temperature(p.temperature[b]);
@@ -329,8 +507,9 @@ template <typename T>
 __global__ void __launch_bounds__(THREADS) pick_kernel(const Params p) {
   __shared__ double sh[WARPS];
   __shared__ int last;
-  __shared__ int found_seg, found_id, any_id;
+  __shared__ int found_seg, any_seg, found_id, any_id;
   __shared__ double before;
+  griddep_wait();
   const int b = blockIdx.y;
   const int n = draft_len(p, b);
   const float z = clean_temperature(p.temperature[b]);
@@ -394,26 +573,44 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const Params p) {
     if (threadIdx.x == 0) p.token[b] = -1;
     return;
   }
+  float u = p.sample_u[b];
+  u = u > 0.f ? u : 0.f;
+  const double border = (double)u * total;
   if (threadIdx.x == 0) {
-    float u = p.sample_u[b];
-    u = u > 0.f ? u : 0.f;
-    const double border = (double)u * total;
-    double run = 0.0, at = 0.0;
-    int g = -1;
-    for (int x = 0; x < p.psegs; ++x) {
-      if (!(ws[x] > 0.0)) continue;
-      g = x;       // the last segment that has any, should the sums round below the border
-      at = run;
-      run += ws[x];
-      if (run > border) break;
-    }
-    found_seg = g;
-    before = border - at;
-    found_id = 0x7fffffff;
-    any_id = -1;
+    found_seg = found_id = 0x7fffffff;
+    any_seg = any_id = -1;
   }
   __syncthreads();
-  // ids of the segment: each thread a contiguous piece, exclusive sums of the pieces in order
+  {
+    // each thread a run of segments; the first whose sum exceeds the border, or
+    // the last that has any, should the sums round below it
+    const int per = (p.psegs + THREADS - 1) / THREADS;
+    const int g0 = threadIdx.x * per, g1 = min(p.psegs, g0 + per);
+    double mine = 0.0;
+    for (int g = g0; g < g1; ++g) mine += ws[g];
+    const double base = before_me(mine, sh);
+    double run = base;
+    for (int g = g0; g < g1; ++g) {
+      run += ws[g];
+      if (!(ws[g] > 0.0)) continue;
+      atomicMax(&any_seg, g);
+      if (run > border) {
+        atomicMin(&found_seg, g);
+        break;
+      }
+    }
+    __syncthreads();
+    const int chosen = found_seg != 0x7fffffff ? found_seg : any_seg;
+    if (chosen >= g0 && chosen < g1) {
+      run = base;
+      for (int g = g0; g < chosen; ++g) run += ws[g];
+      before = border - run;   // what is left of the border inside the segment
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) found_seg = chosen;
+    __syncthreads();
+  }
+  // ids of the segment: each thread a contiguous piece, the pieces' sums in order
   constexpr int PER = PICK_SEG / THREADS;
   const int w0 = found_seg * PICK_SEG + threadIdx.x * PER;
   double mine = 0.0, piece[PER];
@@ -424,19 +621,7 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const Params p) {
     piece[j] = use_left ? l : w;
     mine += piece[j];
   }
-  __shared__ double pre[THREADS];
-  pre[threadIdx.x] = mine;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double run = 0.0;
-    for (int t = 0; t < THREADS; ++t) {
-      const double x = pre[t];
-      pre[t] = run;
-      run += x;
-    }
-  }
-  __syncthreads();
-  double run = pre[threadIdx.x];
+  double run = before_me(mine, sh);
   int hit = 0x7fffffff, any = -1;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
@@ -456,7 +641,7 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const Params p) {
 // beside its loads, short enough that a few rows still fill the card.
 inline void geometry(int B, int T, int V, bool draft, int sms, int* seg, int* segs, int* psegs) {
   const long long rows = (long long)B * T + (draft ? (long long)B * (T - 1) : 0);
-  int s = 32768;
+  int s = MAX_SEG;
   while (s > 4096 && rows * ((V + s - 1) / s) < 8ll * sms) s /= 2;
   *seg = s;
   *segs = (V + s - 1) / s;
@@ -488,11 +673,10 @@ int launch(const Params& p, cudaStream_t stream) {
   rows_kernel<T><<<dim3(p.segs, rows), THREADS, 0, stream>>>(p);
   int st = host::launch_status();
   if (st != DFL_OK) return st;
-  decide_kernel<T><<<dim3(p.psegs, p.B), THREADS, 0, stream>>>(p);
-  st = host::launch_status();
+  // without the draft's logits there are no sums to take again
+  st = host::launch_pdl(decide_kernel<T>, dim3(p.draft ? p.psegs : 1, p.B), THREADS, 0, stream, p);
   if (st != DFL_OK) return st;
-  pick_kernel<T><<<dim3(p.psegs, p.B), THREADS, 0, stream>>>(p);
-  return host::launch_status();
+  return host::launch_pdl(pick_kernel<T>, dim3(p.psegs, p.B), THREADS, 0, stream, p);
 }
 
 // rows <= 65535: the grid's y dimension

@@ -36,7 +36,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._runtime import mask_bytes, require_cuda, same_device, stream_ptr
+from ._runtime import mask_bytes, on_device, require_cuda, same_device, stream_ptr
 
 
 def _check(tape, k, g, state, steps=None, mask=None):
@@ -160,17 +160,20 @@ def gated_delta_kernel_with_tape(q: torch.Tensor, k: torch.Tensor, v: torch.Tens
 
 
 # ------------------------------------------------- whole sequences, no tape
-def _token_rows(x: torch.Tensor):
+def _token_rows(x: torch.Tensor, b: int, t: int, h: int, d: int):
     """``x [B, T, H, D]`` as tokens one fixed stride apart: ``(tensor, stride)``.
     Views of a wider projection (heads and values next to each other, tokens
     further apart) are read in place when their rows are 16-byte aligned;
     everything else is copied."""
-    b, t, h, d = x.shape
-    step = x.stride(1) if t > 1 else (x.stride(0) if b > 1 else h * d)
-    fits = ((d == 1 or x.stride(3) == 1) and (h == 1 or x.stride(2) == d) and step >= h * d
-            and (b == 1 or t == 1 or x.stride(0) == t * step) and step % 8 == 0 and step < 2**31
-            and x.data_ptr() % 16 == 0)
-    return (x, step) if fits else (x.contiguous(), h * d)
+    if x.data_ptr() % 16 == 0:
+        if x.is_contiguous():
+            return x, h * d
+        s0, s1, s2, s3 = x.stride()
+        step = s1 if t > 1 else (s0 if b > 1 else h * d)
+        if (s3 == 1 and (h == 1 or s2 == d) and step >= h * d and (b == 1 or t == 1 or s0 == t * step)
+                and step % 8 == 0 and step < 2**31):
+            return x, step
+    return _aligned(x), h * d
 
 
 def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor,
@@ -199,80 +202,80 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     dev = state.device
     same_device(dev, q=q, k=k, v=v, g=g, beta=beta, mask=mask, cu_seqlens=cu_seqlens, out=out,
                 out_state=out_state)
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        if t.dtype != torch.bfloat16:
-            raise NotImplementedError(f"{name} must be bfloat16, got {t.dtype}")
-        if t.dim() != 4:
-            raise ValueError(f"{name} must be [B, T, heads, dim], got {tuple(t.shape)}")
-    if g.dtype != torch.float32 or beta.dtype != torch.float32:
-        raise NotImplementedError("g and beta must be float32")
-    if state.dtype != torch.float32:
-        raise NotImplementedError(f"state must be float32, got {state.dtype}")
+    bf16, f32 = torch.bfloat16, torch.float32
+    if q.dtype != bf16 or k.dtype != bf16 or v.dtype != bf16:
+        raise NotImplementedError(f"q, k and v must be bfloat16, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if g.dtype != f32 or beta.dtype != f32 or state.dtype != f32:
+        raise NotImplementedError(f"g, beta and state must be float32, got {g.dtype}, {beta.dtype}, {state.dtype}")
+    if k.dim() != 4 or v.dim() != 4:
+        raise ValueError(f"q, k and v must be [B, T, heads, dim], got {tuple(k.shape)} and {tuple(v.shape)}")
     b, t_steps, hk, dk = k.shape
-    hv, dv = v.shape[2:]
+    bv, tv, hv, dv = v.shape
     if q.shape != k.shape:
         raise ValueError("q and k must have the same shape")
     if hk < 1 or hv < 1 or hv % hk != 0:
         raise ValueError(f"Cannot align K heads {hk} to V heads {hv}")
     if dk not in (32, 64, 128, 256) or dv < 32 or dv % 32 != 0:
         raise ValueError(f"Dk must be 32, 64, 128 or 256 and Dv a multiple of 32, got {dk} and {dv}")
-    if v.shape[:2] != (b, t_steps) or beta.shape != (b, t_steps, hv):
+    tokens = (b, t_steps, hv)
+    if bv != b or tv != t_steps or beta.shape != tokens:
         raise ValueError("v must be [B, T, Hv, Dv] and beta [B, T, Hv]")
-    if g.shape not in ((b, t_steps, hv), (b, t_steps, hv, dk)):
+    vector = g.dim() == 4
+    if g.shape != ((b, t_steps, hv, dk) if vector else tokens):
         raise ValueError(f"Unsupported gating shape {tuple(g.shape)}")
-    seqs = b
+    seqs, steps, cu_ptr, mask_ptr = b, t_steps, None, None
     if cu_seqlens is not None:
         if b != 1:
             raise ValueError(f"packed sequences take B = 1, got {b}")
         if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
             raise ValueError("cu_seqlens must be int32 [sequences + 1]")
-        seqs = cu_seqlens.numel() - 1
         cu_seqlens = cu_seqlens.contiguous()
-    if state.shape != (seqs, hv, dv, dk):
-        raise ValueError(f"state must be [B, Hv, Dv, Dk] = {(seqs, hv, dv, dk)}, got {tuple(state.shape)}")
+        cu_ptr = cu_seqlens.data_ptr()
+        seqs = cu_seqlens.numel() - 1
+        steps = t_steps // max(seqs, 1)
+    shape = (seqs, hv, dv, dk)
+    if state.shape != shape:
+        raise ValueError(f"state must be [B, Hv, Dv, Dk] = {shape}, got {tuple(state.shape)}")
     if mask is not None:
         if mask.shape != (b, t_steps):
             raise ValueError(f"mask must be [B, T] = {(b, t_steps)}, got {tuple(mask.shape)}")
         mask = mask_bytes(mask, "mask")
+        mask_ptr = mask.data_ptr()
     zero_gaps = out is None
     if out is None:
         new = torch.zeros if seqs == 0 else torch.empty
-        out = new((b, t_steps, hv, dv), dtype=torch.bfloat16, device=dev)
-    elif (out.dtype != torch.bfloat16 or out.shape != (b, t_steps, hv, dv) or not out.is_contiguous()
+        out = new((b, t_steps, hv, dv), dtype=bf16, device=dev)
+    elif (out.dtype != bf16 or out.shape != (b, t_steps, hv, dv) or not out.is_contiguous()
           or out.data_ptr() % 16 != 0):
         raise ValueError(f"out must be contiguous, 16-byte aligned bf16 {(b, t_steps, hv, dv)}")
     if out_state is None:
-        out_state = torch.empty((seqs, hv, dv, dk), dtype=torch.float32, device=dev)
+        out_state = torch.empty(shape, dtype=f32, device=dev)
         state = _aligned(state)
     else:
-        if (out_state.dtype != torch.float32 or out_state.shape != state.shape
-                or not out_state.is_contiguous() or out_state.data_ptr() % 16 != 0):
-            raise ValueError(f"out_state must be contiguous, 16-byte aligned fp32 {tuple(state.shape)}")
+        if (out_state.dtype != f32 or out_state.shape != shape or not out_state.is_contiguous()
+                or out_state.data_ptr() % 16 != 0):
+            raise ValueError(f"out_state must be contiguous, 16-byte aligned fp32 {shape}")
         if out_state.data_ptr() == state.data_ptr() and state.is_contiguous():
             pass   # in place
         elif out_state.untyped_storage().data_ptr() == state.untyped_storage().data_ptr():
             state = state.clone(memory_format=torch.contiguous_format)   # may overlap in part
         else:
             state = _aligned(state)
-    q, ldq = _token_rows(q)
-    k, ldk = _token_rows(k)
-    v, ldv = _token_rows(v)
+    q, ldq = _token_rows(q, b, t_steps, hk, dk)
+    k, ldk = _token_rows(k, b, t_steps, hk, dk)
+    v, ldv = _token_rows(v, b, t_steps, hv, dv)
     g, beta = g.contiguous(), beta.contiguous()
-    mask_ptr = None if mask is None else mask.data_ptr()
-    cu_ptr = None if cu_seqlens is None else cu_seqlens.data_ptr()
-    steps = t_steps if cu_seqlens is None else t_steps // max(seqs, 1)
-    # bytes that both entries address alike: q, k, v rows, then the rest
+    lib = _lib.load()
     head = (q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, g.data_ptr())
     tail = (beta.data_ptr(), mask_ptr, cu_ptr, state.data_ptr(), out_state.data_ptr(), out.data_ptr(),
-            1 if zero_gaps else 0, seqs, t_steps, hv, hk, dv, dk)
-    with torch.cuda.device(dev):
-        if g.dim() == 3 and dk in (64, 128) and steps >= _CHUNKED_STEPS:
-            entry = "dfl_gdn_rule_chunked"
-            st = _lib.load().dfl_gdn_rule_chunked(*head, *tail, stream_ptr(dev))
+            1 if zero_gaps else 0, seqs, t_steps, hv, hk, dv, dk, stream_ptr(dev))
+    with on_device(dev):
+        if not vector and (dk == 128 or dk == 64) and steps >= _CHUNKED_STEPS:
+            entry, st = "dfl_gdn_rule_chunked", lib.dfl_gdn_rule_chunked(*head, *tail)
         else:
-            entry = "dfl_gdn_rule_recurrent"
-            st = _lib.load().dfl_gdn_rule_recurrent(*head, 1 if g.dim() == 4 else 0, *tail, stream_ptr(dev))
-    _lib.check(entry, st)
+            entry, st = "dfl_gdn_rule_recurrent", lib.dfl_gdn_rule_recurrent(*head, 1 if vector else 0, *tail)
+    if st:
+        _lib.check(entry, st)
     return out, out_state
 
 

@@ -27,7 +27,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._runtime import mask_bytes, require_cuda, same_device, stream_ptr, workspace
+from ._runtime import mask_bytes, on_device, require_cuda, same_device, stream_ptr, workspace
 
 
 def workspace_bytes(rows: int, dim: int, vocab: int) -> int:
@@ -135,7 +135,8 @@ def _logit_rows(x: torch.Tensor):
     buffer's rows costs no copy)."""
     if x.shape[2] > 1 and x.stride(2) != 1:
         x = x.contiguous()
-    return x, int(x.stride(1)), int(x.stride(0))
+    bs, ld, _ = x.stride()
+    return x, ld, bs
 
 
 def verify_accept_sampled(logits: torch.Tensor, verify_ids: torch.Tensor, accept_u: torch.Tensor,
@@ -171,61 +172,63 @@ def verify_accept_sampled(logits: torch.Tensor, verify_ids: torch.Tensor, accept
         raise NotImplementedError(f"logits must be bfloat16, float16 or float32, got {logits.dtype}")
     if logits.dim() != 3 or logits.shape[1] < 1 or logits.shape[2] < 1:
         raise ValueError(f"logits must be [B, T, V], got {tuple(logits.shape)}")
-    b, t, v = (int(x) for x in logits.shape)
+    b, t, v = logits.shape
     same_device(dev, verify_ids=verify_ids, accept_u=accept_u, sample_u=sample_u,
                 draft_logits=draft_logits, draft_lens=draft_lens, suppress_token_mask=suppress_token_mask)
-    if tuple(verify_ids.shape) != (b, t) or verify_ids.dtype not in (torch.int32, torch.int64):
+    i32, f32 = torch.int32, torch.float32
+    if verify_ids.shape != (b, t) or verify_ids.dtype not in (i32, torch.int64):
         raise ValueError(f"verify_ids must be int32 or int64 {(b, t)}")
-    if tuple(accept_u.shape) != (b, t - 1) or tuple(sample_u.shape) != (b,):
+    if accept_u.shape != (b, t - 1) or sample_u.shape != (b,):
         raise ValueError(f"accept_u must be {(b, t - 1)} and sample_u {(b,)}")
-    if accept_u.dtype != torch.float32 or sample_u.dtype != torch.float32:
+    if accept_u.dtype != f32 or sample_u.dtype != f32:
         raise ValueError("accept_u and sample_u must be float32")
+    logits, ld, bs = _logit_rows(logits)
+    draft_ptr, ldd, bsd = None, 0, 0
     if draft_logits is not None:
-        if tuple(draft_logits.shape) != (b, t - 1, v) or draft_logits.dtype != logits.dtype:
+        if draft_logits.shape != (b, t - 1, v) or draft_logits.dtype != logits.dtype:
             raise ValueError(f"draft_logits must be {logits.dtype} {(b, t - 1, v)}")
-        if t == 1:
-            draft_logits = None
+        if t > 1:
+            draft_logits, ldd, bsd = _logit_rows(draft_logits)
+            draft_ptr = draft_logits.data_ptr()
     if isinstance(temperature, torch.Tensor):
         same_device(dev, temperature=temperature)
-        if temperature.dtype != torch.float32 or tuple(temperature.shape) != (b,):
+        if temperature.dtype != f32 or temperature.shape != (b,):
             raise ValueError(f"temperature must be a number or float32 {(b,)}")
         temperature = temperature.contiguous()
     else:
         if not float(temperature) >= 0.0:
             raise ValueError(f"temperature must be >= 0, got {temperature}")
-        temperature = torch.full((b,), float(temperature), dtype=torch.float32, device=dev)
+        temperature = torch.full((b,), float(temperature), dtype=f32, device=dev)
+    lens_ptr = sup_ptr = None
     if draft_lens is not None:
-        if draft_lens.dtype != torch.int32 or tuple(draft_lens.shape) != (b,):
+        if draft_lens.dtype != i32 or draft_lens.shape != (b,):
             raise ValueError(f"draft_lens must be int32 {(b,)}")
         draft_lens = draft_lens.contiguous()
-    sup = None
+        lens_ptr = draft_lens.data_ptr()
     if suppress_token_mask is not None:
-        if tuple(suppress_token_mask.shape) != (v,):
+        if suppress_token_mask.shape != (v,):
             raise ValueError(f"suppress_token_mask must be {(v,)}")
-        sup = mask_bytes(suppress_token_mask, "suppress_token_mask")
-    logits, ld, bs = _logit_rows(logits)
-    ldd = bsd = 0
-    if draft_logits is not None:
-        draft_logits, ldd, bsd = _logit_rows(draft_logits)
-    ids = verify_ids.to(torch.int32).contiguous()
+        suppress_token_mask = mask_bytes(suppress_token_mask, "suppress_token_mask")
+        sup_ptr = suppress_token_mask.data_ptr()
+    ids = verify_ids.to(i32).contiguous()
     accept_u, sample_u = accept_u.contiguous(), sample_u.contiguous()
-    acc = torch.empty(b, dtype=torch.int32, device=dev)
-    nxt = torch.empty(b, dtype=torch.int32, device=dev)
-    prob = torch.empty((b, t - 1), dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
+    acc = torch.empty(b, dtype=i32, device=dev)
+    nxt = torch.empty(b, dtype=i32, device=dev)
+    prob = torch.empty((b, t - 1), dtype=f32, device=dev)
+    lib = _lib.load()
+    with on_device(dev):
         st = ctypes.c_int(0)
-        n = _lib.load().dfl_verify_sampled_workspace_bytes(b, t, v, 0 if draft_logits is None else 1,
-                                                           ctypes.byref(st))
-        _lib.check("dfl_verify_sampled_workspace_bytes", st.value)
+        n = lib.dfl_verify_sampled_workspace_bytes(b, t, v, 0 if draft_ptr is None else 1, ctypes.byref(st))
+        if st.value:
+            _lib.check("dfl_verify_sampled_workspace_bytes", st.value)
         # scratch of this call alone (any content), not one of the zero-filled workspaces
-        ws = torch.empty(max(int(n), 16), dtype=torch.uint8, device=dev)
-        status = _lib.load().dfl_verify_accept_sampled(
-            logits.data_ptr(), None if draft_logits is None else draft_logits.data_ptr(),
-            _LOGIT_TYPES[logits.dtype], ids.data_ptr(), accept_u.data_ptr(), sample_u.data_ptr(),
-            temperature.data_ptr(), None if draft_lens is None else draft_lens.data_ptr(),
-            None if sup is None else sup.data_ptr(), acc.data_ptr(), nxt.data_ptr(), prob.data_ptr(),
-            ld, bs, ldd, bsd, b, t, v, ws.data_ptr(), ws.numel(), stream_ptr(dev))
-    _lib.check("dfl_verify_accept_sampled", status)
+        ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
+        status = lib.dfl_verify_accept_sampled(
+            logits.data_ptr(), draft_ptr, _LOGIT_TYPES[logits.dtype], ids.data_ptr(), accept_u.data_ptr(),
+            sample_u.data_ptr(), temperature.data_ptr(), lens_ptr, sup_ptr, acc.data_ptr(), nxt.data_ptr(),
+            prob.data_ptr(), ld, bs, ldd, bsd, b, t, v, ws.data_ptr(), ws.numel(), stream_ptr(dev))
+    if status:
+        _lib.check("dfl_verify_accept_sampled", status)
     return acc, nxt, prob
 
 

@@ -26,7 +26,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._runtime import require_cuda, same_device, stream_ptr, workspace
+from ._runtime import on_device, require_cuda, same_device, stream_ptr, workspace
 from .verify_qmm import qmm_w4g64
 
 
@@ -119,35 +119,40 @@ def route_experts(router_logits: torch.Tensor, top_k: int, *, score: str = "soft
         raise NotImplementedError(f"router_logits must be bfloat16, float16 or float32, got {lg.dtype}")
     if lg.dim() != 2 or lg.shape[1] < 1:
         raise ValueError(f"router_logits must be [T, E], got {tuple(lg.shape)}")
-    t, e = (int(x) for x in lg.shape)
+    t, e = lg.shape
     if score not in ("softmax", "sigmoid"):
         raise ValueError(f"score must be softmax or sigmoid, got {score!r}")
     group_score = group_score or ("top2" if score == "sigmoid" else "max")
     if group_score not in ("top2", "max"):
         raise ValueError(f"group_score must be top2 or max, got {group_score!r}")
-    groups = int(n_groups)
+    k, groups = int(top_k), int(n_groups)
     kept = groups if topk_groups is None else int(topk_groups)
     if groups < 1 or e % groups != 0 or not 1 <= kept <= groups:
         raise ValueError(f"{e} experts in {groups} groups, {kept} of them kept")
-    if not 1 <= int(top_k) <= min(32, kept * (e // groups)):
-        raise ValueError(f"top_k = {top_k}: 1 to 32, and at most the {kept * (e // groups)} experts of the kept groups")
+    if not 1 <= k <= min(32, kept * (e // groups)):
+        raise ValueError(f"top_k = {k}: 1 to 32, and at most the {kept * (e // groups)} experts of the kept groups")
+    bias_ptr = None
     if bias is not None:
         same_device(dev, bias=bias)
-        if bias.dtype != torch.float32 or tuple(bias.shape) != (e,):
+        if bias.dtype != torch.float32 or bias.shape != (e,):
             raise ValueError(f"bias must be float32 {(e,)}")
         bias = bias.contiguous()
-    if (e > 1 and lg.stride(1) != 1) or (t > 1 and lg.stride(0) < e):
+        bias_ptr = bias.data_ptr()
+    ld, step = lg.stride()
+    if (e > 1 and step != 1) or (t > 1 and ld < e):
         lg = lg.contiguous()
-    w = torch.empty((t, int(top_k)), dtype=torch.float32, device=dev)
-    ids = torch.empty((t, int(top_k)), dtype=torch.int32, device=dev)
+        ld = e
+    w = torch.empty((t, k), dtype=torch.float32, device=dev)
+    ids = torch.empty((t, k), dtype=torch.int32, device=dev)
     flags = ((_ROUTE_SIGMOID if score == "sigmoid" else 0) | (_ROUTE_GROUP_TOP2 if group_score == "top2" else 0)
              | (_ROUTE_RENORM if renormalize else 0))
-    with torch.cuda.device(dev):
-        st = _lib.load().dfl_moe_route_experts(
-            lg.data_ptr(), _LOGIT_TYPES[lg.dtype], int(lg.stride(0)) if t > 1 else e,
-            None if bias is None else bias.data_ptr(), t, e, int(top_k), groups, kept, flags, float(scale),
-            w.data_ptr(), ids.data_ptr(), stream_ptr(dev))
-    _lib.check("dfl_moe_route_experts", st)
+    lib = _lib.load()
+    with on_device(dev):
+        st = lib.dfl_moe_route_experts(lg.data_ptr(), _LOGIT_TYPES[lg.dtype], ld if t > 1 else e, bias_ptr, t, e, k,
+                                       groups, kept, flags, float(scale), w.data_ptr(), ids.data_ptr(),
+                                       stream_ptr(dev))
+    if st:
+        _lib.check("dfl_moe_route_experts", st)
     return w, ids
 
 
