@@ -11,12 +11,12 @@
 // The committed tokens are then distributed as samples of the target alone.
 // z = 0 (or below, or NaN) is greedy: p_i is all on the largest logit's id.
 //
-// Three launches.  rows_kernel reads every row once (the one pass that is bound
+// Three or four launches.  rows_kernel reads every row once (the one pass that is bound
 // by HBM): maximum, its id and sum of exponentials of each segment, in 32 bits.
-// decide_kernel joins a request's segments, accepts, and, where the next token
-// comes from a difference of two softmaxes, adds the two rows' exponentials
-// again in 64 bits.  pick_kernel adds the weights of that one row's segments in
-// 64 bits, and the last CTA of a request finds the segment and the id.  The 64
+// decide_kernel joins a request's segments and accepts.  Where the next token
+// comes from a difference of two softmaxes, norm_kernel adds the two rows'
+// exponentials again in 64 bits.  pick_kernel adds the weights of that one
+// row's segments in 64 bits, and the last CTA of a request finds the segment and the id.  The 64
 // bits are for the id: with 2^18 ids a weight is 2^-18 of the total, and a sum
 // in 32 bits would move a border by a sizeable part of it.
 //
@@ -57,7 +57,7 @@ struct Params {
   int* part_id;          // [B * T][segs] lowest id of the maximum
   double* zsum;          // [2][B][psegs]
   double* wsum;          // [2][B][psegs]
-  int* sel;              // [B] accepted
+  struct Chosen* chosen; // [B]
   int* ticket;           // [B]
 };
 
@@ -144,7 +144,8 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// 16 bytes of logits as floats
+// 16 bytes of logits: as floats, their largest (NaN only if all are), and -inf
+// put over those with a bit in `off`.
 template <typename T>
 struct Vec;
 template <>
@@ -153,7 +154,28 @@ struct Vec<float> {
   static __device__ __forceinline__ void get(const uint4& u, float (&f)[4]) {
     f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
   }
+  static __device__ __forceinline__ float top(const uint4& u) {
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  }
+  static __device__ __forceinline__ void hide(uint4& u, uint32_t off) {
+    if (off & 1u) u.x = 0xff800000u;
+    if (off & 2u) u.y = 0xff800000u;
+    if (off & 4u) u.z = 0xff800000u;
+    if (off & 8u) u.w = 0xff800000u;
+  }
 };
+
+template <uint32_t NEG_INF>
+__device__ __forceinline__ void hide16(uint4& u, uint32_t off) {
+  uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((off >> (2 * i)) & 1u) w[i] = (w[i] & 0xffff0000u) | NEG_INF;
+    if ((off >> (2 * i + 1)) & 1u) w[i] = (w[i] & 0xffffu) | (NEG_INF << 16);
+  }
+  u = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 template <>
 struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
@@ -165,19 +187,31 @@ struct Vec<__nv_bfloat16> {
       f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
   }
+  static __device__ __forceinline__ float top(const uint4& u) {
+    const __nv_bfloat162* w = reinterpret_cast<const __nv_bfloat162*>(&u);
+    const float2 m = __bfloat1622float2(__hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3])));
+    return fmaxf(m.x, m.y);
+  }
+  static __device__ __forceinline__ void hide(uint4& u, uint32_t off) { hide16<0xff80u>(u, off); }
 };
 template <>
 struct Vec<__half> {
   static constexpr int N = 8;
   static __device__ __forceinline__ void get(const uint4& u, float (&f)[8]) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    const __half2* w = reinterpret_cast<const __half2*>(&u);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      const float2 x = __half22float2(w[i]);
       f[2 * i] = x.x;
       f[2 * i + 1] = x.y;
     }
   }
+  static __device__ __forceinline__ float top(const uint4& u) {
+    const __half2* w = reinterpret_cast<const __half2*>(&u);
+    const float2 m = __half22float2(__hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3])));
+    return fmaxf(m.x, m.y);
+  }
+  static __device__ __forceinline__ void hide(uint4& u, uint32_t off) { hide16<0xfc00u>(u, off); }
 };
 
 constexpr int MAX_SEG = 32768;
@@ -207,12 +241,11 @@ __device__ __forceinline__ void stage_mask(const uint8_t* sup, int v0, int v1, u
 
 // Segment blockIdx.x of row blockIdx.y (target rows, then draft rows).
 //
-// Per id: widen, maximum, one FMA for (x - m) c with c = log2(e) / z, ex2, add --
-// 5 instructions; HBM leaves about 8 (measured: see the launch).  m c is rounded
-// once per maximum, a common factor of all terms that is taken out again at
-// the end.  The quick loop takes a vector of ids at a time and moves the
-// maximum rarely; a thread that met NaN or +inf, or nothing above the lowest
-// value, goes over its ids again one by one.
+// Per id: widen, half a packed maximum, one FMA for (x - m) c with c = log2(e) / z,
+// ex2, add.  m c is rounded once per maximum, a common factor of all terms that
+// is taken out again at the end.  The quick loop moves the maximum at most
+// once in U vectors; a thread that met NaN or +inf, or nothing above the
+// lowest value, goes over its ids again one by one.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
   __shared__ Stat sh[WARPS];
@@ -234,58 +267,76 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
   const T* x = is_draft ? draft_row<T>(p, b, i) : target_row<T>(p, b, i);
   const uint8_t* sup = is_draft ? nullptr : p.suppress;
   const int v0 = blockIdx.x * p.seg, v1 = min(p.V, v0 + p.seg);
-  if (sup) {
-    stage_mask(sup, v0, v1, reinterpret_cast<uint16_t*>(bits));
-    __syncthreads();
-  }
   auto hidden = [&](int v) { return sup && ((bits[(v - v0) / 32] >> ((v - v0) & 31)) & 1u); };
   // ids up to the first 16-byte border one by one, then vectors, then the rest
   const int head = min(int((16 - (reinterpret_cast<uintptr_t>(x + v0) & 15)) & 15) / int(sizeof(T)), v1 - v0);
   const int vecs = (v1 - v0 - head) / N;
   const int body = v0 + head;
   Stat a{-FLT_MAX, 0.f, 0x7fffffff};
-  float mc = -FLT_MAX * c;   // may be -inf: replaced before the first term that counts
+  float mc = -FLT_MAX * c;   // may be -inf
+  float part[U] = {};        // the sum, in parts that do not wait for one another
   auto raise = [&](float top) {
     const float was = mc;
     a.m = top;
     mc = a.m * c;
-    a.s = a.s > 0.f ? a.s * ex2(was - mc) : 0.f;
-  };
-  for (int k0 = threadIdx.x; k0 < vecs; k0 += THREADS * U) {
-    uint4 raw[U];
+    const float f = was > -INFINITY ? ex2(was - mc) : 0.f;
+    a.s *= f;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (k0 + u * THREADS < vecs)
-        raw[u] = __ldg(reinterpret_cast<const uint4*>(x + body) + k0 + u * THREADS);
+    for (int u = 0; u < U; ++u) part[u] *= f;
+  };
+  // the next vectors are on their way while these are worked on
+  const uint4* src = reinterpret_cast<const uint4*>(x + body);
+  uint4 raw[U], ahead[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (int(threadIdx.x) + u * THREADS < vecs) ahead[u] = __ldg(src + threadIdx.x + u * THREADS);
+  if (sup) {
+    stage_mask(sup, v0, v1, reinterpret_cast<uint16_t*>(bits));
+    __syncthreads();
+  }
+  for (int k0 = threadIdx.x; k0 < vecs; k0 += THREADS * U) {
+    float top = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (k0 + u * THREADS >= vecs) break;
-      const int v = body + (k0 + u * THREADS) * N;
-      float f[N];
-      Vec<T>::get(raw[u], f);
-      if (sup) {
-        const int o = v - v0;
-        const uint32_t off = __funnelshift_r(bits[o / 32], bits[o / 32 + 1], o & 31) & ((1u << N) - 1u);
-        if (off) {
+      const int k = k0 + u * THREADS;
+      raw[u] = ahead[u];
+      if (k + U * THREADS < vecs) ahead[u] = __ldg(src + k + U * THREADS);
+      if (k < vecs) {
+        if (sup) {
+          const int o = head + k * N;
+          const uint32_t off = __funnelshift_r(bits[o / 32], bits[o / 32 + 1], o & 31) & ((1u << N) - 1u);
+          if (off) Vec<T>::hide(raw[u], off);
+        }
+      } else {
+        Vec<T>::hide(raw[u], (1u << N) - 1u);
+      }
+      top = fmaxf(top, Vec<T>::top(raw[u]));
+    }
+    if (top > a.m) {
+      raise(top);
+      a.id = 0;        // which one it is, a greedy row finds below
+      if (z == 0.f) {
+        a.id = 0x7fffffff;
 #pragma unroll
-          for (int j = 0; j < N; ++j)
-            if ((off >> j) & 1u) f[j] = -INFINITY;
+        for (int u = U - 1; u >= 0; --u) {
+          float f[N];
+          Vec<T>::get(raw[u], f);
+#pragma unroll
+          for (int j = N - 1; j >= 0; --j)
+            if (f[j] == top) a.id = body + (k0 + u * THREADS) * N + j;
         }
       }
-      float top = f[0];
+    }
 #pragma unroll
-      for (int j = 1; j < N; ++j) top = fmaxf(top, f[j]);
-      if (top == -INFINITY) continue;   // masked whole (a NaN goes on, and into the sum)
-      if (top > a.m) {
-        raise(top);
+    for (int u = 0; u < U; ++u) {
+      float f[N];
+      Vec<T>::get(raw[u], f);
 #pragma unroll
-        for (int j = N - 1; j >= 0; --j)
-          if (f[j] == top) a.id = v + j;
-      }
-#pragma unroll
-      for (int j = 0; j < N; ++j) a.s += ex2(__fmaf_rn(f[j], c, -mc));
+      for (int j = 0; j < N; ++j) part[u] += ex2(__fmaf_rn(f[j], c, -mc));
     }
   }
+#pragma unroll
+  for (int u = 0; u < U; ++u) a.s += part[u];
   // the ragged ends, taken by the first threads
   const int tail = body + vecs * N;
   const bool in_head = threadIdx.x < head, in_tail = tail + int(threadIdx.x) < v1;
@@ -376,6 +427,48 @@ __device__ __forceinline__ double weight(float x, float m, double inv_z) {
   return d < 0.0 ? exp(d * inv_z) : 0.0;   // NaN compares false; -inf gives exp(-inf) = 0
 }
 
+// The same for many ids: 2^t, t = (x - m) c with c = log2(e) / z, as 2^e T[i] 2^r with
+// t = e + i / 256 + r, |r| <= 2^-9: the 256 powers of 2^(1/256) from a table in shared
+// memory, 2^r by its Taylor series to r^3 (the next term is 1.4e-13 of the
+// result).  10 operations in 64 bits; the sums of a row then err by less than
+// 1e-13 of their total, where exponentials in 32 bits would leave 1e-9 and with
+// 2^18 ids move one border in some thousands over a uniform.
+constexpr int POWERS = 256;
+
+__device__ __forceinline__ void fill_powers(double* table) {
+  for (int i = threadIdx.x; i < POWERS; i += THREADS) table[i] = exp2(double(i) / POWERS);
+}
+
+__device__ __forceinline__ double weight_table(float x, float m, double c, const double* table) {
+  const double t = ((double)x - (double)m) * c;
+  const double big = 6755399441055744.0 / POWERS;       // 1.5 * 2^52: t rounds to a multiple of 2^-8
+  const double s = t + big;
+  const int k = __double2loint(s);
+  const double r = t - (s - big);
+  constexpr double l1 = 0.69314718055994530942, l2 = l1 * l1 / 2.0, l3 = l1 * l1 * l1 / 6.0;   // ln 2
+  const double p = fma(fma(fma(l3, r, l2), r, l1), r, 1.0);
+  const double w = table[k & (POWERS - 1)] * p;
+  const double v = __hiloint2double(__double2hiint(w) + ((k >> 8) << 20), __double2loint(w));
+  if (x == m) return 1.0;
+  return t > -1000.0 ? v : 0.0;                          // NaN compares false
+}
+
+// Logits of ids v, v + THREADS, .. (8 of them) below v1, -inf where there is none
+// or it is suppressed; every load is issued before the first is waited for.
+template <typename T>
+__device__ __forceinline__ void load_ids(const T* row, const uint8_t* sup, int v, int v1, float (&x)[8]) {
+  uint32_t off = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int at = min(v + j * THREADS, v1 - 1);
+    x[j] = to_f<T>(row[at]);
+    off |= uint32_t(at != v + j * THREADS || (sup != nullptr && sup[at] != 0)) << j;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if ((off >> j) & 1u) x[j] = -INFINITY;
+}
+
 __device__ __forceinline__ double block_sum(double x, double* sh) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
@@ -406,15 +499,19 @@ __device__ __forceinline__ double before_me(double x, double* sh) {
   return lane == 0 ? base : base + prev;
 }
 
-// Accept (every CTA of a request alike; CTA 0 writes), then the 64-bit sums of
-// segment blockIdx.x of the rows that the next token is drawn from.
+// What a request's next token is drawn from, as decide_kernel leaves it.
+struct Chosen {
+  int row;        // accepted drafts
+  float mp, mq;   // maxima of the target's and of the draft's row (-inf: empty, or not used)
+};
+
+// Accept: a CTA per request, a warp per draft.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) decide_kernel(const Params p) {
   __shared__ int first_bad;
-  __shared__ double sh[WARPS];
   griddep_launch_dependents();
   griddep_wait();
-  const int b = blockIdx.y;
+  const int b = blockIdx.x;
   const int n = draft_len(p, b);
   const float z = clean_temperature(p.temperature[b]);
   const float c = z == 0.f ? 1.f : 1.44269504f / z;
@@ -427,16 +524,17 @@ __global__ void __launch_bounds__(THREADS) decide_kernel(const Params p) {
     if (i < n) {
       const int x = p.ids[(size_t)b * p.T + i + 1];
       const bool in = x >= 0 && x < p.V;
+      const int at = in ? x : 0;
+      const bool hidden = !in || (p.suppress && p.suppress[at]);
+      const float lx = to_f<T>(target_row<T>(p, b, i)[at]);
+      const float dx = p.draft ? to_f<T>(draft_row<T>(p, b, i)[at]) : 0.f;
       float m;
       double s;
       int id;
       row_stat(p, b * p.T + i, true, c, &m, &s, &id);
-      const bool open = in && !(p.suppress && p.suppress[x]);
-      const float lx = open ? to_f<T>(target_row<T>(p, b, i)[x]) : -INFINITY;
-      if (m > -INFINITY && open) px = z == 0.f ? (x == id ? 1.0 : 0.0) : weight(lx, m, inv_z) / s;
+      if (m > -INFINITY && !hidden) px = z == 0.f ? (x == id ? 1.0 : 0.0) : weight(lx, m, inv_z) / s;
       if (p.draft && z != 0.f) {
         row_stat(p, p.B * p.T + b * (p.T - 1) + i, false, c, &m, &s, &id);
-        const float dx = in ? to_f<T>(draft_row<T>(p, b, i)[x]) : -INFINITY;
         qx = m > -INFINITY && in ? weight(dx, m, inv_z) / s : 0.0;
       }
       if (lane == 0) {
@@ -444,29 +542,56 @@ __global__ void __launch_bounds__(THREADS) decide_kernel(const Params p) {
         if (!(u * qx < px)) atomicMin(&first_bad, i);
       }
     }
-    if (lane == 0 && blockIdx.x == 0) p.draft_prob[(size_t)b * (p.T - 1) + i] = float(px);
+    if (lane == 0) p.draft_prob[(size_t)b * (p.T - 1) + i] = float(px);
   }
   __syncthreads();
+  if (warp != 0) return;
   const int a = first_bad;
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    p.accepted[b] = a;
-    p.sel[b] = a;
-  }
-  if (!(p.draft && a < n && z != 0.f)) return;
-  // normalisers of p_a and q_a
-  const int v0 = blockIdx.x * PICK_SEG, v1 = min(p.V, v0 + PICK_SEG);
-  float mp, mq;
+  Chosen ch{a, -INFINITY, -INFINITY};
   double s;
-  int id;
-  row_stat(p, b * p.T + a, false, c, &mp, &s, &id);
-  row_stat(p, p.B * p.T + b * (p.T - 1) + a, false, c, &mq, &s, &id);
-  const T* lp = target_row<T>(p, b, a);
-  const T* lq = draft_row<T>(p, b, a);
-  double sp = 0.0, sq = 0.0;
-  for (int v = v0 + threadIdx.x; v < v1; v += THREADS) {
-    if (!(p.suppress && p.suppress[v])) sp += mp > -INFINITY ? weight(to_f<T>(lp[v]), mp, inv_z) : 0.0;
-    sq += mq > -INFINITY ? weight(to_f<T>(lq[v]), mq, inv_z) : 0.0;
+  int id, unused;
+  row_stat(p, b * p.T + a, true, c, &ch.mp, &s, &id);
+  if (p.draft && a < n && z != 0.f) row_stat(p, p.B * p.T + b * (p.T - 1) + a, false, c, &ch.mq, &s, &unused);
+  if (lane == 0) {
+    p.accepted[b] = a;
+    p.chosen[b] = ch;
+    if (z == 0.f) p.token[b] = ch.mp > -INFINITY ? id : -1;
   }
+}
+
+// The 64-bit sums of segment blockIdx.x of the two rows whose difference a
+// request draws from.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) norm_kernel(const Params p) {
+  __shared__ double sh[WARPS];
+  __shared__ double powers[POWERS];
+  griddep_launch_dependents();
+  fill_powers(powers);
+  griddep_wait();
+  __syncthreads();
+  const int b = blockIdx.y;
+  const int n = draft_len(p, b);
+  const float z = clean_temperature(p.temperature[b]);
+  const Chosen ch = p.chosen[b];
+  if (!(ch.row < n && z != 0.f)) return;
+  const int v0 = blockIdx.x * PICK_SEG, v1 = min(p.V, v0 + PICK_SEG);
+  const T* lp = target_row<T>(p, b, ch.row);
+  const T* lq = draft_row<T>(p, b, ch.row);
+  const double c64 = 1.44269504088896340736 / (double)z;   // log2(e) / z
+  double sp = 0.0, sq = 0.0;
+#pragma unroll
+  for (int j0 = 0; j0 < PICK_SEG / THREADS; j0 += 8) {
+    float x[8], y[8];
+    load_ids<T>(lp, p.suppress, v0 + j0 * THREADS + threadIdx.x, v1, x);
+    load_ids<T>(lq, nullptr, v0 + j0 * THREADS + threadIdx.x, v1, y);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      sp += weight_table(x[j], ch.mp, c64, powers);
+      sq += weight_table(y[j], ch.mq, c64, powers);
+    }
+  }
+  if (!(ch.mp > -INFINITY)) sp = 0.0;   // rows with nothing in them
+  if (!(ch.mq > -INFINITY)) sq = 0.0;
   sp = block_sum(sp, sh);
   sq = block_sum(sq, sh);
   if (threadIdx.x == 0) {
@@ -480,19 +605,18 @@ template <typename T>
 struct Pick {
   const T* lp;
   const T* lq;     // null: no draft row to take away
-  const uint8_t* sup;
   float mp, mq;
-  double inv_z, ip, iq;  // 1 / z, 1 / sums
+  double c64, ip, iq;    // log2(e) / z, 1 / sums
+  const double* powers;
   int hot;         // id that a greedy draft takes away whole, or -1
-  // weights of id v: left after the draft, and the target's own
-  __device__ __forceinline__ void at(int v, double* left, double* whole) const {
-    double w = 0.0;
-    // the two products rounded alike, not fused into the difference: equal rows leave exactly 0
-    if (mp > -INFINITY && !(sup && sup[v])) w = __dmul_rn(weight(to_f<T>(lp[v]), mp, inv_z), ip);
+  // weights of id v, target logit x (-inf: hidden) and draft logit y: left after
+  // the draft, and the target's own.  The two products are rounded alike, not
+  // fused into the difference: equal rows leave exactly 0.
+  __device__ __forceinline__ void at(int v, float x, float y, double* left, double* whole) const {
+    const double w = mp > -INFINITY && x > -INFINITY ? __dmul_rn(weight_table(x, mp, c64, powers), ip) : 0.0;
     *whole = w;
     double l = v == hot ? 0.0 : w;
-    if (lq && mq > -INFINITY)
-      l = fmax(w - __dmul_rn(weight(to_f<T>(lq[v]), mq, inv_z), iq), 0.0);
+    if (lq && mq > -INFINITY) l = fmax(w - __dmul_rn(weight_table(y, mq, c64, powers), iq), 0.0);
     *left = l;
   }
 };
@@ -509,33 +633,28 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const Params p) {
   __shared__ int last;
   __shared__ int found_seg, any_seg, found_id, any_id;
   __shared__ double before;
+  __shared__ double powers[POWERS];
+  fill_powers(powers);
   griddep_wait();
+  __syncthreads();
   const int b = blockIdx.y;
   const int n = draft_len(p, b);
   const float z = clean_temperature(p.temperature[b]);
-  const float c = z == 0.f ? 1.f : 1.44269504f / z;
-  const int a = p.sel[b];
-  float m;
-  double s;
-  int id;
-  row_stat(p, b * p.T + a, true, c, &m, &s, &id);
-  if (z == 0.f) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) p.token[b] = m > -INFINITY ? id : -1;
-    return;
-  }
+  if (z == 0.f) return;   // greedy: decide_kernel wrote the token
+  const Chosen ch = p.chosen[b];
+  const int a = ch.row;
   Pick<T> k;
   k.lp = target_row<T>(p, b, a);
   k.lq = nullptr;
-  k.sup = p.suppress;
-  k.mp = m;
-  k.mq = -INFINITY;
-  k.inv_z = 1.0 / (double)z;
+  k.mp = ch.mp;
+  k.mq = ch.mq;
+  k.c64 = 1.44269504088896340736 / (double)z;
+  k.powers = powers;
   k.ip = k.iq = 1.0;
   k.hot = -1;
   if (a < n) {
     if (p.draft) {
       k.lq = draft_row<T>(p, b, a);
-      row_stat(p, p.B * p.T + b * (p.T - 1) + a, false, c, &k.mq, &s, &id);
       const double sp = fixed_sum(p.zsum + (size_t)b * p.psegs, p.psegs, sh);
       const double sq = fixed_sum(p.zsum + (size_t)(p.B + b) * p.psegs, p.psegs, sh);
       k.ip = sp > 0.0 ? 1.0 / sp : 0.0;
@@ -546,11 +665,19 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const Params p) {
   }
   const int v0 = blockIdx.x * PICK_SEG, v1 = min(p.V, v0 + PICK_SEG);
   double left = 0.0, whole = 0.0;
-  for (int v = v0 + threadIdx.x; v < v1; v += THREADS) {
-    double l, w;
-    k.at(v, &l, &w);
-    left += l;
-    whole += w;
+#pragma unroll
+  for (int j0 = 0; j0 < PICK_SEG / THREADS; j0 += 8) {
+    const int v = v0 + j0 * THREADS + threadIdx.x;
+    float x[8], y[8];
+    load_ids<T>(k.lp, p.suppress, v, v1, x);
+    load_ids<T>(k.lq ? k.lq : k.lp, nullptr, v, v1, y);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      double l, w;
+      k.at(v + j * THREADS, x[j], y[j], &l, &w);
+      left += l;
+      whole += w;
+    }
   }
   left = block_sum(left, sh);
   whole = block_sum(whole, sh);
@@ -616,8 +743,12 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const Params p) {
   double mine = 0.0, piece[PER];
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    double l = 0.0, w = 0.0;
-    if (w0 + j < p.V) k.at(w0 + j, &l, &w);
+    const int v = min(w0 + j, p.V - 1);
+    float x = to_f<T>(k.lp[v]);
+    const float y = to_f<T>(k.lq ? k.lq[v] : k.lp[v]);
+    if (w0 + j >= p.V || (p.suppress && p.suppress[v])) x = -INFINITY;
+    double l, w;
+    k.at(v, x, y, &l, &w);
     piece[j] = use_left ? l : w;
     mine += piece[j];
   }
@@ -662,7 +793,7 @@ inline size_t layout(Params* p, uint8_t* base) {
   p->zsum = reinterpret_cast<double*>(put((size_t)2 * p->B * p->psegs * sizeof(double)));
   p->wsum = reinterpret_cast<double*>(put((size_t)2 * p->B * p->psegs * sizeof(double)));
   p->part_id = reinterpret_cast<int*>(put((size_t)p->B * p->T * p->segs * sizeof(int)));
-  p->sel = reinterpret_cast<int*>(put((size_t)p->B * sizeof(int)));
+  p->chosen = reinterpret_cast<Chosen*>(put((size_t)p->B * sizeof(Chosen)));
   p->ticket = reinterpret_cast<int*>(put((size_t)p->B * sizeof(int)));
   return at;
 }
@@ -673,9 +804,12 @@ int launch(const Params& p, cudaStream_t stream) {
   rows_kernel<T><<<dim3(p.segs, rows), THREADS, 0, stream>>>(p);
   int st = host::launch_status();
   if (st != DFL_OK) return st;
-  // without the draft's logits there are no sums to take again
-  st = host::launch_pdl(decide_kernel<T>, dim3(p.draft ? p.psegs : 1, p.B), THREADS, 0, stream, p);
+  st = host::launch_pdl(decide_kernel<T>, dim3(p.B), THREADS, 0, stream, p);
   if (st != DFL_OK) return st;
+  if (p.draft) {   // without the draft's logits there are no sums to take again
+    st = host::launch_pdl(norm_kernel<T>, dim3(p.psegs, p.B), THREADS, 0, stream, p);
+    if (st != DFL_OK) return st;
+  }
   return host::launch_pdl(pick_kernel<T>, dim3(p.psegs, p.B), THREADS, 0, stream, p);
 }
 
