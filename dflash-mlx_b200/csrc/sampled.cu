@@ -33,7 +33,7 @@ namespace smp {
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
 constexpr int MAX_BLOCK = 256;    // tokens of a block
-constexpr int PICK_SEG = 4096;    // ids of a segment of the picked row
+constexpr int PICK_SEG = 512;     // ids of a segment of the picked row, a warp's
 
 struct Params {
   const void* logits;    // [B, T] rows of V
@@ -51,12 +51,15 @@ struct Params {
   long long bs, bsd;     // elements from one request to the next
   int B, T, V;
   int segs, seg;         // segments of a row and their length (rows_kernel)
-  int psegs;             // segments of PICK_SEG ids (decide_kernel, pick_kernel)
+  int psegs;             // segments of PICK_SEG ids (pick_kernel)
+  int words;             // of the mask's bits
+  int group;             // segments of a warp (norm_kernel, pick_kernel)
   // workspace
+  uint32_t* bits;        // [words]
   float2* part;          // [B * T + B * (T - 1)][segs] (maximum, sum)
   int* part_id;          // [B * T][segs] lowest id of the maximum
-  double* zsum;          // [2][B][psegs]
-  double* wsum;          // [2][B][psegs]
+  double* zsum;          // [2][B][CTAs of norm_kernel]
+  double* wsum;          // [B][psegs]
   struct Chosen* chosen; // [B]
   int* ticket;           // [B]
 };
@@ -214,29 +217,33 @@ struct Vec<__half> {
   static __device__ __forceinline__ void hide(uint4& u, uint32_t off) { hide16<0xfc00u>(u, off); }
 };
 
-constexpr int MAX_SEG = 32768;
+constexpr int MAX_SEG = 65536;
 
-// One bit per id of [v0, v1), set where it is suppressed: 16 mask bytes at a
-// time where they lie on 16-byte borders (v0 does, being a multiple of 16).
-__device__ __forceinline__ void stage_mask(const uint8_t* sup, int v0, int v1, uint16_t* bits) {
-  const int words = (v1 - v0 + 15) / 16;
+// One bit per id, set where it is suppressed, a word per thread; 16 mask bytes at
+// a time where they lie on 16-byte borders.  Packed once per call: in every
+// row's pass the bytes would cost half of the row's own traffic, and packing
+// them there 2.5 instructions an id (measured).
+__global__ void __launch_bounds__(THREADS) mask_kernel(const Params p) {
+  griddep_launch_dependents();
+  const uint8_t* sup = p.suppress;
   const bool wide = (reinterpret_cast<uintptr_t>(sup) & 15) == 0;
-  for (int i = threadIdx.x; i < words; i += THREADS) {
-    const int v = v0 + 16 * i;
-    uint32_t r = 0;
-    if (wide && v + 16 <= v1) {
+  const int i = blockIdx.x * THREADS + threadIdx.x;
+  if (i >= p.words) return;
+  uint32_t r = 0;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int v = 32 * i + 16 * h;
+    if (wide && v + 16 <= p.V) {
       const uint4 u = *reinterpret_cast<const uint4*>(sup + v);
       const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
       // a byte each to 0 or 1, then bits 0, 8, 16, 24 side by side at the top
-      for (int j = 0; j < 4; ++j) r |= ((__vsetne4(w[j], 0) * 0x10204080u) >> 28) << (4 * j);
+      for (int j = 0; j < 4; ++j) r |= ((__vsetne4(w[j], 0) * 0x10204080u) >> 28) << (16 * h + 4 * j);
     } else {
-      for (int j = 0; j < 16 && v + j < v1; ++j) r |= uint32_t(sup[v + j] != 0) << j;
+      for (int j = 0; j < 16 && v + j < p.V; ++j) r |= uint32_t(sup[v + j] != 0) << (16 * h + j);
     }
-    bits[i] = uint16_t(r);
   }
-  // a word behind the last is read with it
-  if (threadIdx.x < 4) bits[words + threadIdx.x] = 0;
+  p.bits[i] = r;   // two words behind the last id are read with it: 0
 }
 
 // Segment blockIdx.x of row blockIdx.y (target rows, then draft rows).
@@ -249,7 +256,6 @@ __device__ __forceinline__ void stage_mask(const uint8_t* sup, int v0, int v1, u
 template <typename T>
 __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
   __shared__ Stat sh[WARPS];
-  __shared__ uint32_t bits[MAX_SEG / 32 + 4];
   constexpr int N = Vec<T>::N, U = 4;
   griddep_launch_dependents();
   const int row = blockIdx.y;
@@ -265,9 +271,10 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
   if (is_draft && z == 0.f) return;
   const float c = z == 0.f ? 1.f : 1.44269504f / z;
   const T* x = is_draft ? draft_row<T>(p, b, i) : target_row<T>(p, b, i);
-  const uint8_t* sup = is_draft ? nullptr : p.suppress;
+  const bool sup = !is_draft && p.suppress != nullptr;
+  const uint32_t* bits = p.bits;
   const int v0 = blockIdx.x * p.seg, v1 = min(p.V, v0 + p.seg);
-  auto hidden = [&](int v) { return sup && ((bits[(v - v0) / 32] >> ((v - v0) & 31)) & 1u); };
+  auto hidden = [&](int v) { return sup && ((bits[v / 32] >> (v & 31)) & 1u); };
   // ids up to the first 16-byte border one by one, then vectors, then the rest
   const int head = min(int((16 - (reinterpret_cast<uintptr_t>(x + v0) & 15)) & 15) / int(sizeof(T)), v1 - v0);
   const int vecs = (v1 - v0 - head) / N;
@@ -290,10 +297,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if (int(threadIdx.x) + u * THREADS < vecs) ahead[u] = __ldg(src + threadIdx.x + u * THREADS);
-  if (sup) {
-    stage_mask(sup, v0, v1, reinterpret_cast<uint16_t*>(bits));
-    __syncthreads();
-  }
+  if (sup) griddep_wait();   // the mask's bits
   for (int k0 = threadIdx.x; k0 < vecs; k0 += THREADS * U) {
     float top = -INFINITY;
 #pragma unroll
@@ -303,7 +307,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
       if (k + U * THREADS < vecs) ahead[u] = __ldg(src + k + U * THREADS);
       if (k < vecs) {
         if (sup) {
-          const int o = head + k * N;
+          const int o = body + k * N;
           const uint32_t off = __funnelshift_r(bits[o / 32], bits[o / 32 + 1], o & 31) & ((1u << N) - 1u);
           if (off) Vec<T>::hide(raw[u], off);
         }
@@ -394,9 +398,10 @@ __device__ __forceinline__ void row_stat(const Params& p, int row, bool with_id,
   int at = 0x7fffffff;
   for (int g = lane; g < p.segs; g += 32) {
     const float x = p.part[(size_t)row * p.segs + g].x;
+    const int i = with_id ? p.part_id[(size_t)row * p.segs + g] : 0;
     if (x > mx) {
       mx = x;
-      at = with_id ? p.part_id[(size_t)row * p.segs + g] : 0;
+      at = i;
     }
   }
 #pragma unroll
@@ -453,25 +458,61 @@ __device__ __forceinline__ double weight_table(float x, float m, double c, const
   return t > -1000.0 ? v : 0.0;                          // NaN compares false
 }
 
-// Logits of ids v, v + THREADS, .. (8 of them) below v1, -inf where there is none
-// or it is suppressed; every load is issued before the first is waited for.
+// A lane's 16 ids of a segment of PICK_SEG: N at a time next to each other (16
+// bytes), the lanes side by side.
 template <typename T>
-__device__ __forceinline__ void load_ids(const T* row, const uint8_t* sup, int v, int v1, float (&x)[8]) {
-  uint32_t off = 0;
+__device__ __forceinline__ int lane_id(int j) {
+  constexpr int N = Vec<T>::N;
+  return (j / N) * 32 * N + int(threadIdx.x & 31) * N + j % N;
+}
+
+// Their logits, -inf behind the vocabulary or where suppressed; every load is
+// issued before the first is waited for.
+template <typename T>
+__device__ __forceinline__ void load_ids(const T* row, const uint32_t* bits, int seg, int V, float (&x)[16]) {
+  constexpr int N = Vec<T>::N;
+  const int v0 = seg * PICK_SEG;
+  uint32_t off[16 / N];
+  if (v0 + PICK_SEG <= V && (reinterpret_cast<uintptr_t>(row) & 15) == 0) {
+    uint4 u[16 / N];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int at = min(v + j * THREADS, v1 - 1);
-    x[j] = to_f<T>(row[at]);
-    off |= uint32_t(at != v + j * THREADS || (sup != nullptr && sup[at] != 0)) << j;
+    for (int i = 0; i < 16 / N; ++i) {
+      const int v = v0 + lane_id<T>(i * N);
+      u[i] = __ldg(reinterpret_cast<const uint4*>(row + v));
+      off[i] = bits ? bits[v / 32] >> (v & 31) : 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < 16 / N; ++i) {
+      float f[N];
+      Vec<T>::get(u[i], f);
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[i * N + j] = f[j];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16 / N; ++i) {
+      off[i] = 0;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int v = v0 + lane_id<T>(i * N + j), at = min(v, V - 1);
+        x[i * N + j] = to_f<T>(row[at]);
+        if (v >= V || (bits && ((bits[at / 32] >> (at & 31)) & 1u))) off[i] |= 1u << j;
+      }
+    }
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if ((off >> j) & 1u) x[j] = -INFINITY;
+  for (int j = 0; j < 16; ++j)
+    if ((off[j / N] >> (j % N)) & 1u) x[j] = -INFINITY;
+}
+
+__device__ __forceinline__ double warp_sum(double x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
 }
 
 __device__ __forceinline__ double block_sum(double x, double* sh) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  x = warp_sum(x);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = x;
   __syncthreads();
@@ -506,8 +547,10 @@ struct Chosen {
 };
 
 // Accept: a CTA per request, a warp per draft.
+constexpr int DECIDE_WARPS = 16;
+
 template <typename T>
-__global__ void __launch_bounds__(THREADS) decide_kernel(const Params p) {
+__global__ void __launch_bounds__(32 * DECIDE_WARPS) decide_kernel(const Params p) {
   __shared__ int first_bad;
   griddep_launch_dependents();
   griddep_wait();
@@ -519,7 +562,7 @@ __global__ void __launch_bounds__(THREADS) decide_kernel(const Params p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) first_bad = n;
   __syncthreads();
-  for (int i = warp; i < p.T - 1; i += WARPS) {
+  for (int i = warp; i < p.T - 1; i += DECIDE_WARPS) {
     double px = 0.0, qx = 1.0;
     if (i < n) {
       const int x = p.ids[(size_t)b * p.T + i + 1];
@@ -574,18 +617,18 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(const Params p) {
   const float z = clean_temperature(p.temperature[b]);
   const Chosen ch = p.chosen[b];
   if (!(ch.row < n && z != 0.f)) return;
-  const int v0 = blockIdx.x * PICK_SEG, v1 = min(p.V, v0 + PICK_SEG);
   const T* lp = target_row<T>(p, b, ch.row);
   const T* lq = draft_row<T>(p, b, ch.row);
   const double c64 = 1.44269504088896340736 / (double)z;   // log2(e) / z
   double sp = 0.0, sq = 0.0;
+  for (int g = 0; g < p.group; ++g) {
+    const int seg = (blockIdx.x * p.group + g) * WARPS + int(threadIdx.x >> 5);
+    if (seg >= p.psegs) break;
+    float x[16], y[16];
+    load_ids<T>(lp, p.suppress ? p.bits : nullptr, seg, p.V, x);
+    load_ids<T>(lq, nullptr, seg, p.V, y);
 #pragma unroll
-  for (int j0 = 0; j0 < PICK_SEG / THREADS; j0 += 8) {
-    float x[8], y[8];
-    load_ids<T>(lp, p.suppress, v0 + j0 * THREADS + threadIdx.x, v1, x);
-    load_ids<T>(lq, nullptr, v0 + j0 * THREADS + threadIdx.x, v1, y);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < 16; ++j) {
       sp += weight_table(x[j], ch.mp, c64, powers);
       sq += weight_table(y[j], ch.mq, c64, powers);
     }
@@ -595,8 +638,8 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(const Params p) {
   sp = block_sum(sp, sh);
   sq = block_sum(sq, sh);
   if (threadIdx.x == 0) {
-    p.zsum[(size_t)b * p.psegs + blockIdx.x] = sp;
-    p.zsum[(size_t)(p.B + b) * p.psegs + blockIdx.x] = sq;
+    p.zsum[(size_t)b * gridDim.x + blockIdx.x] = sp;
+    p.zsum[(size_t)(p.B + b) * gridDim.x + blockIdx.x] = sq;
   }
 }
 
@@ -609,15 +652,23 @@ struct Pick {
   double c64, ip, iq;    // log2(e) / z, 1 / sums
   const double* powers;
   int hot;         // id that a greedy draft takes away whole, or -1
-  // weights of id v, target logit x (-inf: hidden) and draft logit y: left after
-  // the draft, and the target's own.  The two products are rounded alike, not
-  // fused into the difference: equal rows leave exactly 0.
-  __device__ __forceinline__ void at(int v, float x, float y, double* left, double* whole) const {
+  // weight of id v, target logit x (-inf: hidden) and draft logit y, left after
+  // the draft.  The two products are rounded alike, not fused into the
+  // difference: equal rows leave exactly 0.
+  __device__ __forceinline__ double left(int v, float x, float y) const {
     const double w = mp > -INFINITY && x > -INFINITY ? __dmul_rn(weight_table(x, mp, c64, powers), ip) : 0.0;
-    *whole = w;
-    double l = v == hot ? 0.0 : w;
-    if (lq && mq > -INFINITY) l = fmax(w - __dmul_rn(weight_table(y, mq, c64, powers), iq), 0.0);
-    *left = l;
+    if (lq && mq > -INFINITY) return fmax(w - __dmul_rn(weight_table(y, mq, c64, powers), iq), 0.0);
+    return v == hot ? 0.0 : w;
+  }
+  // sum of a segment, in every lane of the warp
+  __device__ __forceinline__ double segment(int seg, int V, const uint32_t* bits) const {
+    float x[16], y[16];
+    load_ids<T>(lp, bits, seg, V, x);
+    if (lq) load_ids<T>(lq, nullptr, seg, V, y);
+    double sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sum += left(seg * PICK_SEG + lane_id<T>(j), x[j], lq ? y[j] : 0.f);
+    return warp_sum(sum);
   }
 };
 
@@ -655,35 +706,27 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const Params p) {
   if (a < n) {
     if (p.draft) {
       k.lq = draft_row<T>(p, b, a);
-      const double sp = fixed_sum(p.zsum + (size_t)b * p.psegs, p.psegs, sh);
-      const double sq = fixed_sum(p.zsum + (size_t)(p.B + b) * p.psegs, p.psegs, sh);
+      const int parts = gridDim.x;   // norm_kernel's grid is this one's
+      const double sp = fixed_sum(p.zsum + (size_t)b * parts, parts, sh);
+      const double sq = fixed_sum(p.zsum + (size_t)(p.B + b) * parts, parts, sh);
       k.ip = sp > 0.0 ? 1.0 / sp : 0.0;
       k.iq = sq > 0.0 ? 1.0 / sq : 0.0;
     } else {
       k.hot = p.ids[(size_t)b * p.T + a + 1];
     }
   }
-  const int v0 = blockIdx.x * PICK_SEG, v1 = min(p.V, v0 + PICK_SEG);
-  double left = 0.0, whole = 0.0;
-#pragma unroll
-  for (int j0 = 0; j0 < PICK_SEG / THREADS; j0 += 8) {
-    const int v = v0 + j0 * THREADS + threadIdx.x;
-    float x[8], y[8];
-    load_ids<T>(k.lp, p.suppress, v, v1, x);
-    load_ids<T>(k.lq ? k.lq : k.lp, nullptr, v, v1, y);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      double l, w;
-      k.at(v + j * THREADS, x[j], y[j], &l, &w);
-      left += l;
-      whole += w;
-    }
+  const uint32_t* bits = p.suppress ? p.bits : nullptr;
+  double* ws = p.wsum + (size_t)b * p.psegs;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int g = 0; g < p.group; ++g) {
+    const int seg = (blockIdx.x * p.group + g) * WARPS + warp;
+    if (seg >= p.psegs) break;
+    const double sum = k.segment(seg, p.V, bits);
+    if (lane == 0) ws[seg] = sum;
   }
-  left = block_sum(left, sh);
-  whole = block_sum(whole, sh);
+  __threadfence();
+  __syncthreads();
   if (threadIdx.x == 0) {
-    p.wsum[(size_t)b * p.psegs + blockIdx.x] = left;
-    p.wsum[(size_t)(p.B + b) * p.psegs + blockIdx.x] = whole;
     __threadfence();
     last = atomicAdd(&p.ticket[b], 1) == int(gridDim.x) - 1;
   }
@@ -692,10 +735,20 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const Params p) {
   __threadfence();
   // The last CTA of the request: total, the segment that the border falls in,
   // then the id inside it.  Which CTA this is changes no sum.
-  double total = fixed_sum(p.wsum + (size_t)b * p.psegs, p.psegs, sh);
-  const bool use_left = total > 0.0;   // nothing left after the draft: the target's own weights
-  const double* ws = p.wsum + (size_t)(use_left ? b : p.B + b) * p.psegs;
-  if (!use_left) total = fixed_sum(ws, p.psegs, sh);
+  double total = fixed_sum(ws, p.psegs, sh);
+  if (!(total > 0.0)) {
+    // nothing left after the draft (equal rows, and a draft that q cannot give):
+    // the target's own weights
+    k.lq = nullptr;
+    k.hot = -1;
+    __syncthreads();
+    for (int seg = warp; seg < p.psegs; seg += WARPS) {
+      const double sum = k.segment(seg, p.V, bits);
+      if (lane == 0) ws[seg] = sum;
+    }
+    __syncthreads();
+    total = fixed_sum(ws, p.psegs, sh);
+  }
   if (!(total > 0.0)) {
     if (threadIdx.x == 0) p.token[b] = -1;
     return;
@@ -737,7 +790,7 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const Params p) {
     if (threadIdx.x == 0) found_seg = chosen;
     __syncthreads();
   }
-  // ids of the segment: each thread a contiguous piece, the pieces' sums in order
+  // ids of the segment: each thread two neighbours, the pairs' sums in order
   constexpr int PER = PICK_SEG / THREADS;
   const int w0 = found_seg * PICK_SEG + threadIdx.x * PER;
   double mine = 0.0, piece[PER];
@@ -745,11 +798,9 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const Params p) {
   for (int j = 0; j < PER; ++j) {
     const int v = min(w0 + j, p.V - 1);
     float x = to_f<T>(k.lp[v]);
-    const float y = to_f<T>(k.lq ? k.lq[v] : k.lp[v]);
-    if (w0 + j >= p.V || (p.suppress && p.suppress[v])) x = -INFINITY;
-    double l, w;
-    k.at(v, x, y, &l, &w);
-    piece[j] = use_left ? l : w;
+    const float y = k.lq ? to_f<T>(k.lq[v]) : 0.f;
+    if (bits && ((bits[v / 32] >> (v & 31)) & 1u)) x = -INFINITY;
+    piece[j] = w0 + j < p.V ? k.left(v, x, y) : 0.0;
     mine += piece[j];
   }
   double run = before_me(mine, sh);
@@ -770,13 +821,17 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const Params p) {
 
 // Segment length of rows_kernel: long enough that a CTA's start-up is small
 // beside its loads, short enough that a few rows still fill the card.
-inline void geometry(int B, int T, int V, bool draft, int sms, int* seg, int* segs, int* psegs) {
-  const long long rows = (long long)B * T + (draft ? (long long)B * (T - 1) : 0);
+inline void geometry(Params* p, int sms) {
+  const long long rows = (long long)p->B * p->T + (p->draft ? (long long)p->B * (p->T - 1) : 0);
   int s = MAX_SEG;
-  while (s > 4096 && rows * ((V + s - 1) / s) < 8ll * sms) s /= 2;
-  *seg = s;
-  *segs = (V + s - 1) / s;
-  *psegs = (V + PICK_SEG - 1) / PICK_SEG;
+  while (s > 4096 && rows * ((p->V + s - 1) / s) < 8ll * sms) s /= 2;
+  p->seg = s;
+  p->segs = (p->V + s - 1) / s;
+  p->psegs = (p->V + PICK_SEG - 1) / PICK_SEG;
+  p->words = (p->V + 31) / 32 + 2;
+  // likewise for the picked row: more than one segment a warp where there are many
+  p->group = 1;
+  while (p->group < 8 && (long long)p->B * p->psegs >= 16ll * WARPS * sms * p->group) p->group *= 2;
 }
 
 inline size_t round16(size_t x) { return (x + 15) & ~size_t(15); }
@@ -791,7 +846,8 @@ inline size_t layout(Params* p, uint8_t* base) {
   };
   p->part = reinterpret_cast<float2*>(put(rows * p->segs * sizeof(float2)));
   p->zsum = reinterpret_cast<double*>(put((size_t)2 * p->B * p->psegs * sizeof(double)));
-  p->wsum = reinterpret_cast<double*>(put((size_t)2 * p->B * p->psegs * sizeof(double)));
+  p->wsum = reinterpret_cast<double*>(put((size_t)p->B * p->psegs * sizeof(double)));
+  p->bits = reinterpret_cast<uint32_t*>(put((size_t)p->words * sizeof(uint32_t)));
   p->part_id = reinterpret_cast<int*>(put((size_t)p->B * p->T * p->segs * sizeof(int)));
   p->chosen = reinterpret_cast<Chosen*>(put((size_t)p->B * sizeof(Chosen)));
   p->ticket = reinterpret_cast<int*>(put((size_t)p->B * sizeof(int)));
@@ -801,16 +857,27 @@ inline size_t layout(Params* p, uint8_t* base) {
 template <typename T>
 int launch(const Params& p, cudaStream_t stream) {
   const int rows = p.B * p.T + (p.draft ? p.B * (p.T - 1) : 0);
-  rows_kernel<T><<<dim3(p.segs, rows), THREADS, 0, stream>>>(p);
-  int st = host::launch_status();
+  // The first launch waits for what is before it on the stream as any launch
+  // does; the later ones start early and wait for the one before them.
+  int st;
+  if (p.suppress) {
+    mask_kernel<<<(p.words + THREADS - 1) / THREADS, THREADS, 0, stream>>>(p);
+    st = host::launch_status();
+    if (st != DFL_OK) return st;
+    st = host::launch_pdl(rows_kernel<T>, dim3(p.segs, rows), THREADS, 0, stream, p);
+  } else {
+    rows_kernel<T><<<dim3(p.segs, rows), THREADS, 0, stream>>>(p);
+    st = host::launch_status();
+  }
   if (st != DFL_OK) return st;
-  st = host::launch_pdl(decide_kernel<T>, dim3(p.B), THREADS, 0, stream, p);
+  const int picks = (p.psegs + WARPS * p.group - 1) / (WARPS * p.group);
+  st = host::launch_pdl(decide_kernel<T>, dim3(p.B), 32 * DECIDE_WARPS, 0, stream, p);
   if (st != DFL_OK) return st;
   if (p.draft) {   // without the draft's logits there are no sums to take again
-    st = host::launch_pdl(norm_kernel<T>, dim3(p.psegs, p.B), THREADS, 0, stream, p);
+    st = host::launch_pdl(norm_kernel<T>, dim3(picks, p.B), THREADS, 0, stream, p);
     if (st != DFL_OK) return st;
   }
-  return host::launch_pdl(pick_kernel<T>, dim3(p.psegs, p.B), THREADS, 0, stream, p);
+  return host::launch_pdl(pick_kernel<T>, dim3(picks, p.B), THREADS, 0, stream, p);
 }
 
 // rows <= 65535: the grid's y dimension
@@ -838,7 +905,7 @@ extern "C" size_t dfl_verify_sampled_workspace_bytes(int B, int T, int V, int wi
   p.T = T;
   p.V = V;
   p.draft = with_draft ? &p : nullptr;
-  smp::geometry(B, T, V, with_draft != 0, sms, &p.seg, &p.segs, &p.psegs);
+  smp::geometry(&p, sms);
   return smp::layout(&p, nullptr);
 }
 
@@ -881,7 +948,7 @@ extern "C" int dfl_verify_accept_sampled(const void* logits, const void* draft_l
   p.B = B;
   p.T = T;
   p.V = V;
-  smp::geometry(B, T, V, draft_logits != nullptr, sms, &p.seg, &p.segs, &p.psegs);
+  smp::geometry(&p, sms);
   if (!workspace || !host::aligned(workspace, 16)) return workspace ? DFL_ERR_MISALIGNED : DFL_ERR_WORKSPACE;
   if (workspace_bytes < smp::layout(&p, reinterpret_cast<uint8_t*>(workspace))) return DFL_ERR_WORKSPACE;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
