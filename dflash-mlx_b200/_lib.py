@@ -62,7 +62,10 @@ SIGNATURES = {
                                         _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                         _c_int, _vp]),
     "dfl_gdn_rule_chunked": (_c_int, [_vp, _c_int, _vp, _c_int, _vp, _c_int, _vp, _vp, _vp, _vp, _vp, _vp,
-                                      _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _vp]),
+                                      _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _vp,
+                                      _c_size, _vp]),
+    "dfl_gdn_rule_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                               ctypes.POINTER(_c_int)]),
     "dfl_verify_sampled_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int,
                                                      ctypes.POINTER(_c_int)]),
     "dfl_verify_accept_sampled": (_c_int, [_vp, _vp, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,

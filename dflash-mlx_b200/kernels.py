@@ -31,6 +31,7 @@ which is the identity for fp32).
 
 from __future__ import annotations
 
+import ctypes
 from typing import Optional
 
 import torch
@@ -268,12 +269,19 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     lib = _lib.load()
     head = (q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, g.data_ptr())
     tail = (beta.data_ptr(), mask_ptr, cu_ptr, state.data_ptr(), out_state.data_ptr(), out.data_ptr(),
-            1 if zero_gaps else 0, seqs, t_steps, hv, hk, dv, dk, stream_ptr(dev))
+            1 if zero_gaps else 0, seqs, t_steps, hv, hk, dv, dk)
     with on_device(dev):
         if not vector and (dk == 128 or dk == 64) and steps >= _CHUNKED_STEPS:
-            entry, st = "dfl_gdn_rule_chunked", lib.dfl_gdn_rule_chunked(*head, *tail)
+            entry = "dfl_gdn_rule_chunked"
+            status = ctypes.c_int(0)
+            n = lib.dfl_gdn_rule_workspace_bytes(seqs, t_steps, 0 if cu_ptr is None else 1, hv, dv, dk,
+                                                 ctypes.byref(status))
+            _lib.check("dfl_gdn_rule_workspace_bytes", status.value)
+            ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+            st = lib.dfl_gdn_rule_chunked(*head, *tail, ws.data_ptr() if n else None, n, stream_ptr(dev))
         else:
-            entry, st = "dfl_gdn_rule_recurrent", lib.dfl_gdn_rule_recurrent(*head, 1 if vector else 0, *tail)
+            entry = "dfl_gdn_rule_recurrent"
+            st = lib.dfl_gdn_rule_recurrent(*head, 1 if vector else 0, *tail, stream_ptr(dev))
     if st:
         _lib.check(entry, st)
     return out, out_state

@@ -340,7 +340,9 @@ int dfl_gdn_forward_tape(const uint16_t* q, const uint16_t* k, const uint16_t* v
  * dfl_gdn_rule_chunked takes 64 steps at a time as products on the tensor
  * cores (same results up to the order of fp32 sums; Dk 64 or 128, one decay
  * per head, keys of about unit length as for any use of the rule; q, k and v
- * 16-byte aligned, ldq, ldk and ldv multiples of 8).
+ * 16-byte aligned, ldq, ldk and ldv multiples of 8).  workspace:
+ * dfl_gdn_rule_workspace_bytes bytes (0: none needed), 16-byte aligned, any
+ * content, for states between the pieces of few long sequences.
  * The reference reaches this step, for caches that record no tape, through
  * mlx-lm's gated_delta_update (third party) from the hook at
  * dflash_mlx/engine/target_qwen_gdn.py:551-651. */
@@ -352,7 +354,9 @@ int dfl_gdn_rule_recurrent(const uint16_t* q, int ldq, const uint16_t* k, int ld
 int dfl_gdn_rule_chunked(const uint16_t* q, int ldq, const uint16_t* k, int ldk, const uint16_t* v,
                          int ldv, const float* g, const float* beta, const uint8_t* mask,
                          const int32_t* cu_seqlens, const float* state_in, float* state_out, uint16_t* y,
-                         int zero_gaps, int B, int T, int Hv, int Hk, int Dv, int Dk, void* stream);
+                         int zero_gaps, int B, int T, int Hv, int Hk, int Dv, int Dk, void* workspace,
+                         size_t workspace_bytes, void* stream);
+size_t dfl_gdn_rule_workspace_bytes(int B, int T, int packed, int Hv, int Dv, int Dk, int* status);
 
 /* ------------------------------------------------------------------------
  * DDTree verify: the GDN recurrence over a token tree.

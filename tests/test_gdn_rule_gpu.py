@@ -72,6 +72,9 @@ def _check(y, s, ry, rs, arrays, steps):
     (2, 200, 1, 1, 128, 256, False),
     (1, 700, 1, 2, 128, 128, False),
     (1, 300, 1, 2, 64, 96, False),
+    (1, 1500, 1, 2, 128, 128, False),    # few heads: cut in pieces
+    (2, 1027, 1, 3, 64, 160, False),
+    (1, 3000, 2, 4, 128, 32, False),
 ])
 @pytest.mark.parametrize("slow", [False, True])
 def test_padded_batch(pkg, dev, b, t, hk, hv, dk, dv, vec, slow):
@@ -88,6 +91,8 @@ def test_padded_batch(pkg, dev, b, t, hk, hv, dk, dv, vec, slow):
     ([200, 7, 300], 1, 3, 64, 64),
     ([5, 131], 1, 1, 256, 64),
     ([90, 91, 300], 1, 1, 128, 160),
+    ([3, 2000, 0, 700, 1], 1, 2, 128, 128),   # pieces of very unlike sequences
+    ([64, 2500], 1, 1, 64, 64),
 ])
 def test_packed_sequences(pkg, dev, lens, hk, hv, dk, dv):
     """Lengths of zero and one, ends inside a tile, rows before the first and
@@ -115,7 +120,8 @@ def test_packed_sequences(pkg, dev, lens, hk, hv, dk, dv):
     assert torch.equal(out[:, cut], y[:, cut]) and torch.equal(s, s2)
 
 
-@pytest.mark.parametrize("t,dk,dv", [(1, 128, 128), (40, 128, 128), (150, 128, 128), (150, 64, 64), (40, 256, 32)])
+@pytest.mark.parametrize("t,dk,dv", [(1, 128, 128), (40, 128, 128), (150, 128, 128), (150, 64, 64), (40, 256, 32),
+                                      (1100, 128, 128)])
 def test_mask(pkg, dev, t, dk, dv):
     """Masked steps change nothing, whatever they hold; one sequence is masked whole."""
     b, hk, hv = 3, 2, 4
@@ -190,7 +196,7 @@ def test_views_of_a_wider_projection(pkg, dev, t):
     assert torch.equal(y, want[0]) and torch.equal(s, want[1])
 
 
-@pytest.mark.parametrize("t", [1, 100])
+@pytest.mark.parametrize("t", [1, 100, 1100])
 def test_in_place_and_overlapping_state(pkg, dev, t):
     arrays = _inputs(22, 2, t, 2, 4, 128, 128)
     ins = _dev(arrays, dev)
@@ -249,7 +255,7 @@ def test_bad_offsets_are_reported_and_stay_inside(pkg, dev):
     assert _lib.device_error() == 0
 
 
-@pytest.mark.parametrize("t", [1, 150])
+@pytest.mark.parametrize("t", [1, 150, 1100])
 def test_captured_and_on_another_stream(pkg, dev, t):
     arrays = _inputs(26, 2, t, 2, 4, 128, 128)
     ins = _dev(arrays, dev)

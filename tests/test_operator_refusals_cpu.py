@@ -16,7 +16,7 @@ def _rule(lib, **kw):
              zero=1, B=2, T=4, Hv=4, Hk=2, Dv=128, Dk=128)
     a.update(kw)
     chunked = {k: x for k, x in a.items() if k != "gv"}
-    return [lib.dfl_gdn_rule_recurrent(*a.values(), None), lib.dfl_gdn_rule_chunked(*chunked.values(), None)]
+    return [lib.dfl_gdn_rule_recurrent(*a.values(), None), lib.dfl_gdn_rule_chunked(*chunked.values(), None, 0, None)]
 
 
 @pytest.mark.parametrize("kw,status", [
