@@ -282,6 +282,24 @@ struct CCfg {
   static constexpr int COL_Y = 448;                      // Delta P^T
 };
 
+// mbar_wait_abortable in few instructions (32 bits of the clock): there are
+// thirty waits below, and with two SMs at work behind one instruction cache a
+// chunk's code has to stay small (unrolled all through, a third of the cycles
+// went on fetching it).
+__device__ __forceinline__ void wait_on(uint64_t* bar, uint32_t parity, volatile int* abort_word) {
+  if (mbar_try_wait(bar, parity)) return;
+  uint32_t t0, t1;
+  asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t0));
+#pragma unroll 1
+  while (!*abort_word && !mbar_try_wait(bar, parity)) {
+    asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t1));
+    if (t1 - t0 > uint32_t(kWaitLimitNs)) {
+      atomicExch(&g_device_error, kDevWaitTimeout);
+      *abort_word = 1;
+    }
+  }
+}
+
 // The leading bf16 parts of two values; what they leave stays in a, b (exact).
 __device__ __forceinline__ uint32_t take_part(float& a, float& b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
@@ -664,7 +682,9 @@ __global__ void __launch_bounds__(C_THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  auto wait = [&](uint64_t* bar, int parity) { mbar_wait_abortable(bar, uint32_t(parity & 1), &abort_word); };
+  auto wait = [&](uint64_t* bar, int parity) {
+    wait_on(bar, uint32_t(parity & 1), &abort_word);
+  };
 
   if (warp < 4) {
     // ---------------------------------------------------------- preparation
@@ -689,11 +709,10 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       if (!on) {
         uint8_t* kq = smem + s * C::STAGE_BYTES;
         const uint4 z = make_uint4(0, 0, 0, 0);
-        for (int a = 0; a < DK / 64; ++a)
-#pragma unroll
-          for (int x = 0; x < 8; ++x)   // one of the row's K and Q per thread
-            *reinterpret_cast<uint4*>(kq + a * C::ATOM + ((t % 2) * 64 + r) * 128 + x * 16) = z;
-#pragma unroll
+#pragma unroll 1
+        for (int x = 0; x < DK / 8; ++x)   // one of the row's K and Q per thread
+          *reinterpret_cast<uint4*>(kq + (x / 8) * C::ATOM + ((t % 2) * 64 + r) * 128 + (x % 8) * 16) = z;
+#pragma unroll 1
         for (int x = 0; x < 8; ++x)
           *reinterpret_cast<uint4*>(kq + C::KQ_BYTES + r * 256 + (t % 2) * 128 + x * 16) = z;
       }
@@ -708,13 +727,7 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       const int i = t & 63;       // this thread's step: row of K K^T (t < 64) or of Q K^T
       wait(&bars.g_full, c);
       tc_fence_after();
-      uint32_t gr[2][32];
       const uint32_t gaddr = tmem + (uint32_t(warp * 32) << 16) + C::COL_G;
-      tmem_ld_32x32b_x32(gaddr, gr[0]);
-      tmem_ld_32x32b_x32(gaddr + 32, gr[1]);
-      tmem_ld_wait();
-      tc_fence_before();
-      mbar_arrive(&bars.g_read);
       if (c >= 2) wait(&bars.tp_freed[ts], (c / 2) - 1);
       const float* gs = g_of(s);
       uint8_t* tp = smem + C::TP_OFF + ts * C::TP_BYTES;
@@ -733,36 +746,36 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       float* row_odd = blk & 1 ? row_diag : nowhere;                                  // columns of block 1 or 3
       float* row_even = blk & 1 ? row_diag + (4 + blk / 2 - blk) * DIAG_BLK : row_diag;  // of block 0 or 2
       float d = 0.f, next = 0.f;
-      float4 glo = at4(gs + CH - 8), ghi = at4(gs + CH - 4);
+      // the first 32 rows end with column 31
+      int j8 = warp & 1 ? CH - 8 : 24;
+      uint32_t gr[8];
+      tmem_ld_32x32b_x8(gaddr + j8, gr);
+#pragma unroll 1
+      for (; j8 >= 0; j8 -= 8) {
+        const float4 glo = at4(gs + j8), ghi = at4(gs + j8 + 4);
+        const float gg[8] = {glo.x, glo.y, glo.z, glo.w, ghi.x, ghi.y, ghi.z, ghi.w};
+        float o[8];
+        tmem_ld_wait();
 #pragma unroll
-      for (int j8 = CH - 8; j8 >= 0; j8 -= 8) {
-        if (j8 < 32 || (warp & 1)) {   // the first 32 rows end with column 31
-          const float gg[8] = {glo.x, glo.y, glo.z, glo.w, ghi.x, ghi.y, ghi.z, ghi.w};
-          float o[8];
+        for (int e = 0; e < 8; ++e) o[e] = __uint_as_float(gr[e]);
+        if (j8 > 0) tmem_ld_32x32b_x8(gaddr + j8 - 8, gr);
 #pragma unroll
-          for (int e = 7; e >= 0; --e) {
-            const int j = j8 + e;
-            d = j == i ? start : d * next;
-            next = gg[e];
-            o[e] = d * __uint_as_float(gr[j / 32][j % 32]);
-          }
-          if (j8 > 0) {   // before the stores, which it must not wait for
-            glo = at4(gs + j8 - 8);
-            ghi = at4(gs + j8 - 4);
-          }
-          if (t >= 64) {
-            *reinterpret_cast<uint4*>(tp + 2 * PART + part_at(i, j8)) = take_part8(o);
-          } else {
-            float* at = warp == 1 && j8 < 32 ? off32 + (i - 32) * OFF_LD + j8
-                                             : ((j8 / 16) & 1 ? row_odd : row_even) + (j8 % 16);
-            *reinterpret_cast<float4*>(at) = make_float4(o[0], o[1], o[2], o[3]);
-            *reinterpret_cast<float4*>(at + 4) = make_float4(o[4], o[5], o[6], o[7]);
-          }
-        } else if (j8 == 32) {
-          glo = at4(gs + 24);
-          ghi = at4(gs + 28);
+        for (int e = 7; e >= 0; --e) {
+          d = j8 + e == i ? start : d * next;
+          next = gg[e];
+          o[e] *= d;
+        }
+        if (t >= 64) {
+          *reinterpret_cast<uint4*>(tp + 2 * PART + part_at(i, j8)) = take_part8(o);
+        } else {
+          float* at = warp == 1 && j8 < 32 ? off32 + (i - 32) * OFF_LD + j8
+                                           : ((j8 / 16) & 1 ? row_odd : row_even) + (j8 % 16);
+          *reinterpret_cast<float4*>(at) = make_float4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<float4*>(at + 4) = make_float4(o[4], o[5], o[6], o[7]);
         }
       }
+      tc_fence_before();
+      mbar_arrive(&bars.g_read);
       named_bar_sync(1, C_PREP);
       if (t < 64) {
         invert_block16(diag + (t / 16) * DIAG_BLK, tp, t / 16, t % 16);
@@ -850,17 +863,6 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       for (int i = 0; i < NS; ++i) s[i] = row == h * NS + i ? 1.f : 0.f;
     }
     const uint32_t s_col = ta + C::COL_S + h * (NS / 2);
-    auto store_state = [&](int b) {          // columns 16 b .. 16 b + 15 of this thread
-      float x[16];
-#pragma unroll
-      for (int j = 0; j < 16; ++j) x[j] = s[16 * b + j];
-      store_parts<3>({s_col + 8 * b, s_col + C::S_PART + 8 * b, s_col + 2 * C::S_PART + 8 * b}, x);
-    };
-#pragma unroll
-    for (int b = 0; b < NS / 16; ++b) store_state(b);
-    tmem_st_wait();
-    tc_fence_before();
-    mbar_arrive(&bars.s_ready);
     float r[32];
     auto beta_v = [&](int c) {               // r = beta V of chunk c
       const int st = c % C_STAGES;
@@ -882,19 +884,97 @@ __global__ void __launch_bounds__(C_THREADS, 1)
         r[j + 3] = be.w * __bfloat162float(vt[(j + 3) * 128]);
       }
     };
-    beta_v(0);
     const size_t y_step = (size_t)p.Hv * p.Dv;
     __nv_bfloat16* out = p.y + ((first + h * 32) * p.Hv + hv) * p.Dv + dv0;
-    for (int c = 0; c < chunks; ++c) {
+    auto yt_of = [&](int c) { return smem + (c % C_STAGES) * C::STAGE_BYTES + C::KQ_BYTES + h * 32 * 256; };
+    uint32_t d[2][16];
+    float co[16];
+    // Turn c ends chunk c - 1 (its state, its y) and begins chunk c.
+#pragma unroll 1
+    for (int c = 0;; ++c) {
+      if (c < chunks) beta_v(c);               // while the last chunk's Delta K runs
+      // S <- c_63 S + Delta K, and its parts for the products
+      float keep = 0.f;
+      if (c > 0) {
+        keep = cum_of((c - 1) % 2)[CH - 1];
+        wait(&bars.d4_done, c - 1);
+        tc_fence_after();
+        tmem_ld_32x32b_x16(ta + C::COL_D + h * NS, d[0]);
+      }
+#pragma unroll
+      for (int b = 0; b < NS / 16; ++b) {
+        if (c > 0) {
+          tmem_ld_wait();
+          if (b + 1 < NS / 16) tmem_ld_32x32b_x16(ta + C::COL_D + h * NS + 16 * (b + 1), d[(b + 1) & 1]);
+#pragma unroll
+          for (int j = 0; j < 16; j += 2)
+            fma2(s[16 * b + j], s[16 * b + j + 1], keep, keep, s[16 * b + j], s[16 * b + j + 1],
+                 __uint_as_float(d[b & 1][j]), __uint_as_float(d[b & 1][j + 1]));
+        }
+        if (c < chunks) {
+          float x[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) x[j] = s[16 * b + j];
+          store_parts<3>({s_col + 8 * b, s_col + C::S_PART + 8 * b, s_col + 2 * C::S_PART + 8 * b}, x);
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&bars.s_ready);
+      if (c > 0) {
+        // Y = c Q S^T + P Delta of the last chunk, while this one's K S^T runs.
+        // Steps are rows of y and value rows its columns: the tile is turned in
+        // shared memory, so that y goes out 16 bytes a lane (2-byte stores
+        // straight from the lanes took 2700 cycles of a chunk's 10000 with every
+        // SM at work).  It lies over this chunk's V, which every thread has read
+        // before s_ready.
+        const int last = c - 1, ts = last % 2;
+        wait(&bars.y_done, last);
+        if (!partial) {
+          const float* cs = cum_of(ts) + h * 32;
+          tc_fence_after();
+          load16(cs, co);
+          tmem_ld_32x32b_x16(ta + C::COL_SQ + h * 32, d[0]);
+          tmem_ld_32x32b_x16(ta + C::COL_Y + h * 32, d[1]);
+          wait(&bars.s_ready, c);
+          __nv_bfloat16* at = reinterpret_cast<__nv_bfloat16*>(yt_of(c)) + row;
+#pragma unroll 1
+          for (int b = 0; b < 2; ++b) {
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              at[j * 128] = __float2bfloat16_rn(__fmaf_rn(co[j], __uint_as_float(d[0][j]), __uint_as_float(d[1][j])));
+            at += 16 * 128;
+            if (b == 0) {
+              load16(cs + 16, co);
+              tmem_ld_32x32b_x16(ta + C::COL_SQ + h * 32 + 16, d[0]);
+              tmem_ld_32x32b_x16(ta + C::COL_Y + h * 32 + 16, d[1]);
+            }
+          }
+          tc_fence_before();
+        }
+        mbar_arrive(&bars.y_read);
+        if (!partial) {
+          named_bar_sync(2 + h, C_STATE / 2);
+          const int rows = min(CH, len - last * CH) - h * 32;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int rr = (warp % 4) * 8 + 2 * i + lane / 16, x = lane % 16;
+            const uint4 u = *reinterpret_cast<const uint4*>(yt_of(c) + rr * 256 + x * 16);
+            if (rr < rows && x * 8 < cols) *reinterpret_cast<uint4*>(out + rr * y_step + x * 8) = u;
+          }
+          out += CH * y_step;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.tp_freed[ts]);
+      }
+      if (c == chunks) break;
       const int ts = c % 2;
-      uint32_t d[2][16];
       // R = beta V - beta c K S^T.  Coefficients come 16 at a time, ahead of the
       // stores that the compiler keeps loads behind.
       wait(&bars.tp_full[ts], c / 2);
-      const float* cs = cum_of(ts) + h * 32;
       const float* us = until_of(ts) + h * 32;
       const float* nbc = nbc_of(ts) + h * 32;
-      float co[16];
       load16(nbc, co);
       wait(&bars.d1_done, c);
       tc_fence_after();
@@ -943,73 +1023,6 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&bars.delta_ready);
-      // S <- c_63 S + Delta K
-      const float keep = cum_of(ts)[CH - 1];
-      if (c + 1 < chunks) beta_v(c + 1);     // while the product runs
-      wait(&bars.d4_done, c);
-      tc_fence_after();
-      tmem_ld_32x32b_x16(ta + C::COL_D + h * NS, d[0]);
-#pragma unroll
-      for (int b = 0; b < NS / 16; ++b) {
-        tmem_ld_wait();
-        if (b + 1 < NS / 16) tmem_ld_32x32b_x16(ta + C::COL_D + h * NS + 16 * (b + 1), d[(b + 1) & 1]);
-#pragma unroll
-        for (int j = 0; j < 16; j += 2)
-          fma2(s[16 * b + j], s[16 * b + j + 1], keep, keep, s[16 * b + j], s[16 * b + j + 1],
-               __uint_as_float(d[b & 1][j]), __uint_as_float(d[b & 1][j + 1]));
-        store_state(b);
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(&bars.s_ready);
-      // Y = c Q S^T + P Delta, while the next chunk's K S^T runs.  Steps are rows
-      // of y and value rows its columns: the tile is turned in shared memory, so
-      // that y goes out 16 bytes a lane (2-byte stores straight from the lanes
-      // took 2700 cycles of a chunk's 10000 with every SM at work).  It lies
-      // over the next chunk's V, which every thread has read before s_ready.
-      wait(&bars.y_done, c);
-      if (partial) {
-        mbar_arrive(&bars.y_read);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.tp_freed[ts]);
-        continue;
-      }
-      tc_fence_after();
-      load16(cs, co);
-      tmem_ld_32x32b_x16(ta + C::COL_SQ + h * 32, d[0]);
-      tmem_ld_32x32b_x16(ta + C::COL_Y + h * 32, d[1]);
-      wait(&bars.s_ready, c + 1);
-      uint8_t* yt = smem + ((c + 1) % C_STAGES) * C::STAGE_BYTES + C::KQ_BYTES + h * 32 * 256;
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        tmem_ld_wait();
-        __nv_bfloat16 y[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          y[j] = __float2bfloat16_rn(__fmaf_rn(co[j], __uint_as_float(d[0][j]), __uint_as_float(d[1][j])));
-        if (b == 0) {
-          load16(cs + 16, co);
-          tmem_ld_32x32b_x16(ta + C::COL_SQ + h * 32 + 16, d[0]);
-          tmem_ld_32x32b_x16(ta + C::COL_Y + h * 32 + 16, d[1]);
-        } else {
-          tc_fence_before();
-          mbar_arrive(&bars.y_read);
-        }
-        __nv_bfloat16* at = reinterpret_cast<__nv_bfloat16*>(yt + 16 * b * 256) + row;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) at[j * 128] = y[j];
-      }
-      named_bar_sync(2 + h, C_STATE / 2);
-      const int rows = min(CH, len - c * CH) - h * 32;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int rr = (warp % 4) * 8 + 2 * i + lane / 16, x = lane % 16;
-        const uint4 u = *reinterpret_cast<const uint4*>(yt + rr * 256 + x * 16);
-        if (rr < rows && x * 8 < cols) *reinterpret_cast<uint4*>(out + rr * y_step + x * 8) = u;
-      }
-      out += CH * y_step;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.tp_freed[ts]);
     }
     if (live && dst) {
       dst += (size_t)row * DK + h * NS;
