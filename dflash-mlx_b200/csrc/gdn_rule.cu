@@ -517,49 +517,66 @@ struct Split {
   float* add;    // [heads][n - 2][Dv][Dk] N of pieces 1 .. n - 2
   float* map;    // [heads][n - 2][Dk][Dk] M
 };
-constexpr int MAX_PIECES = 16, MIN_PIECE = 4;   // MIN_PIECE chunks: below, three launches cost what they save
+constexpr int MAX_PIECES = 16;
+constexpr int CHAIN_ROWS = 16;
 
-// start[i + 1] = start[i] map[i] + add[i] over the pieces: 32 rows of a head per
-// CTA, kept in shared memory; thread (c, half) a column of 16 of them.
+// start[i + 1] = start[i] map[i] + add[i] over the pieces: 16 rows of a head per
+// CTA, kept in shared memory; a thread has a column of 8 of them.  The next map
+// is copied to shared memory while one is worked with (read from L2 as it is
+// needed, a step took 10 us for 2).
 template <int DK>
 __global__ void __launch_bounds__(2 * DK) gdn_rule_chain(const Split sp, int Dv) {
-  __shared__ __align__(16) float s[32][DK];
-  const int blocks = Dv / 32;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  constexpr int R = CHAIN_ROWS / 2;
+  float* maps = reinterpret_cast<float*>(smem_raw);                                  // [2][DK][DK]
+  float(*s)[DK] = reinterpret_cast<float(*)[DK]>(maps + 2 * DK * DK);                // [CHAIN_ROWS][DK]
+  const int blocks = Dv / CHAIN_ROWS;
   const size_t head = blockIdx.x / blocks;
-  const int row0 = (blockIdx.x % blocks) * 32;
-  const int c = threadIdx.x % DK, r0 = (threadIdx.x / DK) * 16;
+  const int row0 = (blockIdx.x % blocks) * CHAIN_ROWS;
+  const int c = threadIdx.x % DK, r0 = (threadIdx.x / DK) * R;
   float* start = sp.start + head * (sp.n - 1) * Dv * DK + (size_t)row0 * DK;
-  for (int i = 0; i < 16; ++i) s[r0 + i][c] = start[(size_t)(r0 + i) * DK + c];
-  __syncthreads();
-  for (int k = 0; k < sp.n - 2; ++k) {
+  auto fetch = [&](int k) {
     const float* m = sp.map + (head * (sp.n - 2) + k) * DK * DK;
-    const float* add = sp.add + (head * (sp.n - 2) + k) * Dv * DK + (size_t)row0 * DK;
-    float acc[16];
+    const uint32_t to = smem_u32(maps + (k & 1) * DK * DK);
+    for (int i = threadIdx.x; i < DK * DK / 4; i += 2 * DK) cp_async_16(to + i * 16, m + 4 * i, 16);
+    cp_async_commit();
+  };
+  fetch(0);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[i] = add[(size_t)(r0 + i) * DK + c];
+  for (int i = 0; i < R; ++i) s[r0 + i][c] = start[(size_t)(r0 + i) * DK + c];
+  for (int k = 0; k < sp.n - 2; ++k) {
+    const float* m = maps + (k & 1) * DK * DK + c;
+    const float* add = sp.add + (head * (sp.n - 2) + k) * Dv * DK + (size_t)row0 * DK;
+    float acc[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) acc[i] = add[(size_t)(r0 + i) * DK + c];
+    cp_async_wait_all();
+    __syncthreads();   // the map, and the rows
+    if (k + 1 < sp.n - 2) fetch(k + 1);
 #pragma unroll 4
     for (int j = 0; j < DK; j += 4) {
-      const float m0 = m[(size_t)j * DK + c], m1 = m[(size_t)(j + 1) * DK + c], m2 = m[(size_t)(j + 2) * DK + c],
-                  m3 = m[(size_t)(j + 3) * DK + c];
+      const float m0 = m[j * DK], m1 = m[(j + 1) * DK], m2 = m[(j + 2) * DK], m3 = m[(j + 3) * DK];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float4 x = *reinterpret_cast<const float4*>(&s[r0 + i][j]);
-        acc[i] = __fmaf_rn(x.x, m0, acc[i]);
-        acc[i] = __fmaf_rn(x.y, m1, acc[i]);
-        acc[i] = __fmaf_rn(x.z, m2, acc[i]);
-        acc[i] = __fmaf_rn(x.w, m3, acc[i]);
+      for (int i = 0; i < R; ++i) {
+        const float4 y = *reinterpret_cast<const float4*>(&s[r0 + i][j]);
+        acc[i] = __fmaf_rn(y.x, m0, acc[i]);
+        acc[i] = __fmaf_rn(y.y, m1, acc[i]);
+        acc[i] = __fmaf_rn(y.z, m2, acc[i]);
+        acc[i] = __fmaf_rn(y.w, m3, acc[i]);
       }
     }
     __syncthreads();
     float* next = start + (size_t)(k + 1) * Dv * DK;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < R; ++i) {
       s[r0 + i][c] = acc[i];
       next[(size_t)(r0 + i) * DK + c] = acc[i];
     }
-    __syncthreads();
   }
 }
+
+template <int DK>
+constexpr int chain_smem() { return (2 * DK * DK + CHAIN_ROWS * DK) * int(sizeof(float)); }
 
 template <int DK>
 __global__ void __launch_bounds__(C_THREADS, 1)
@@ -1143,15 +1160,25 @@ __global__ void __launch_bounds__(C_THREADS, 1)
   if (warp == 12) tmem_dealloc(tmem, 512);
 }
 
-// Pieces of a sequence: as many as fill the SMs once in the first launch, when a
-// sequence has enough chunks for that (lengths of packed ones are known on the
-// device only: their mean is taken).  Measured at 48 heads, 8192 steps: 610 us
-// whole, see below for 3 pieces.
+// Pieces of a sequence (lengths of packed ones are known on the device only:
+// their mean is taken).  In units of a chunk's time (5 us): whole, L; in n
+// pieces, two launches of L / n chunks that are 1.25 long with every SM at work,
+// 6 for starting two launches more and 0.6 for a step of the chain.  Measured,
+// us whole and cut, 8192 and 2048 steps: 48 heads 658 / 526 and 174 / 172 (3
+// pieces), 16 heads 654 / 327 and 172 / 152 (6), 8 heads of 64 x 64 525 / 181 and
+// 138 / 85 (10); 1024 steps of 48 heads 94 / 118: left whole.
 inline int pieces(long long heads, int tiles, long long chunks, int sms) {
-  const int most = int(chunks / MIN_PIECE < MAX_PIECES ? chunks / MIN_PIECE : MAX_PIECES);
-  for (int n = most; n >= 3; --n)
-    if (heads * (tiles * (n - 1) + n - 2) <= sms) return n;
-  return 1;
+  int best = 1;
+  double least = 0.95 * double(chunks);
+  for (int n = 3; n <= MAX_PIECES; ++n) {
+    if (heads * (tiles * (n - 1) + n - 2) > sms) break;
+    const double cost = 2.5 * double(chunks) / n + 6.0 + 0.6 * (n - 2);
+    if (cost < least) {
+      least = cost;
+      best = n;
+    }
+  }
+  return best;
 }
 
 inline size_t split_layout(Split* sp, uint8_t* base, size_t heads, int Dv, int Dk) {
@@ -1186,6 +1213,9 @@ int launch_chunked(const RuleParams& p, void* workspace, size_t workspace_bytes,
   if (need > 0 && !host::aligned(workspace, 16)) return DFL_ERR_MISALIGNED;
   st = host::ensure_smem(gdn_rule_chunked<DK>, CCfg<DK>::SMEM_BYTES, dev, done);
   if (st != DFL_OK) return st;
+  static std::atomic<uint64_t> chain_done{0};
+  st = host::ensure_smem(gdn_rule_chain<DK>, chain_smem<DK>(), dev, chain_done);
+  if (st != DFL_OK) return st;
   const uint64_t tokens = p.cu ? uint64_t(p.T) : uint64_t(p.B) * p.T;
   CUtensorMap tm_q, tm_k, tm_v;
   if (tokens > 0) {
@@ -1206,7 +1236,7 @@ int launch_chunked(const RuleParams& p, void* workspace, size_t workspace_bytes,
   gdn_rule_chunked<DK><<<int(heads * sp.jobs), C_THREADS, CCfg<DK>::SMEM_BYTES, stream>>>(tm_q, tm_k, tm_v, p, sp);
   st = host::launch_status();
   if (st != DFL_OK || sp.n == 1) return st;
-  gdn_rule_chain<DK><<<int(heads * (p.Dv / 32)), 2 * DK, 0, stream>>>(sp, p.Dv);
+  gdn_rule_chain<DK><<<int(heads * (p.Dv / CHAIN_ROWS)), 2 * DK, chain_smem<DK>(), stream>>>(sp, p.Dv);
   st = host::launch_status();
   if (st != DFL_OK) return st;
   sp.last = 1;
