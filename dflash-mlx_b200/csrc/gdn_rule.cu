@@ -236,9 +236,10 @@ int launch_recurrent(const RuleParams& p, cudaStream_t stream) {
 //
 // fp32 in bf16 products: K and Q are bf16 already.  The state and the update
 // Delta K go in as three bf16 parts (24 bits), so what is carried from chunk to
-// chunk keeps 32-bit accuracy; R and T - I as two each (without the product of
-// the second parts): their product is a correction to R, which is added in
-// fp32.  In y, which ends in 8 bits, the state has two parts, P and Delta one.
+// chunk keeps 32-bit accuracy, and so does R, whose product with T - I is added
+// to R in fp32; T - I has two (16 bits: it is a correction).  In y, which ends
+// in 8 bits, the state, P and Delta have two parts (one each of P and Delta would
+// add 2.2e-3 of y to the 1.7e-3 of its last rounding).
 //
 // Warps: 0-3 prepare T and P of the next chunk (K K^T and Q K^T from one
 // product, inverse by blocks of 16, 32 and 64 in fp32) and put zeros over rows
@@ -264,9 +265,9 @@ struct CCfg {
   static constexpr int ATOM = 128 * 128;                 // 128 rows (K, then Q) x 64 columns
   static constexpr int KQ_BYTES = (DK / 64) * ATOM;
   static constexpr int V_BYTES = CH * 256;               // 64 rows x 128 columns
-  static constexpr int STAGE_BYTES = KQ_BYTES + V_BYTES;
-  static constexpr int TP_BYTES = 3 * PART;              // T's two parts and P
-  static constexpr int TP_OFF = C_STAGES * STAGE_BYTES;
+  static constexpr int V_OFF = C_STAGES * KQ_BYTES;      // of two chunks
+  static constexpr int TP_BYTES = 4 * PART;              // T's two parts and P's
+  static constexpr int TP_OFF = V_OFF + 2 * V_BYTES;
   static constexpr int A_OFF = TP_OFF + 2 * TP_BYTES;    // A's two parts, A in fp32, a place for stores to nowhere
   static constexpr int SMALL_OFF = A_OFF + 2 * PART + A32_FLOATS * 4 + 1024;
   static constexpr int SMALL_BYTES = (C_STAGES * 2 + 2 * 3) * CH * 4;
@@ -279,7 +280,10 @@ struct CCfg {
   static constexpr int COL_G = 256;                      // [K; Q] K^T, over Delta K's second half
   static constexpr int COL_SQ = 320;                     // S Q^T
   static constexpr int COL_R = 384;                      // R's parts, then Delta
-  static constexpr int COL_Y = 448;                      // Delta P^T
+  static constexpr int COL_Y = 448;                      // R's third part, later Delta P^T
+  // R's third part of 16 steps: each half over its own warps' half of y, which
+  // they have read
+  static __host__ __device__ constexpr int col_r3(int k) { return COL_Y + (k / 2) * 32 + (k % 2) * 8; }
 };
 
 // mbar_wait_abortable in few instructions (32 bits of the clock): there are
@@ -361,7 +365,7 @@ __device__ __forceinline__ void store_parts(const uint32_t (&taddr)[PARTS], floa
 }
 
 struct ChunkBars {
-  uint64_t loaded[C_STAGES], full[C_STAGES];
+  uint64_t loaded[C_STAGES], full[C_STAGES], v_loaded[2];
   uint64_t tp_full[2], tp_freed[2];
   uint64_t g_full, g_read;
   uint64_t s_ready, d1_done, r_ready, d3_done, delta_ready, d4_done, q_done, y_done, y_read;
@@ -670,6 +674,7 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       mbar_init(&bars.full[s], C_PREP);
     }
     for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars.v_loaded[s], 1);
       mbar_init(&bars.tp_full[s], C_PREP);
       mbar_init(&bars.tp_freed[s], 1 + C_STATE / 32);
     }
@@ -724,14 +729,11 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       }
       wait(&bars.loaded[s], c / C_STAGES);
       if (!on) {
-        uint8_t* kq = smem + s * C::STAGE_BYTES;
+        uint8_t* kq = smem + s * C::KQ_BYTES;
         const uint4 z = make_uint4(0, 0, 0, 0);
 #pragma unroll 1
         for (int x = 0; x < DK / 8; ++x)   // one of the row's K and Q per thread
           *reinterpret_cast<uint4*>(kq + (x / 8) * C::ATOM + ((t % 2) * 64 + r) * 128 + (x % 8) * 16) = z;
-#pragma unroll 1
-        for (int x = 0; x < 8; ++x)
-          *reinterpret_cast<uint4*>(kq + C::KQ_BYTES + r * 256 + (t % 2) * 128 + x * 16) = z;
       }
       fence_proxy_async_shared();
       mbar_arrive(&bars.full[s]);
@@ -784,6 +786,7 @@ __global__ void __launch_bounds__(C_THREADS, 1)
         }
         if (t >= 64) {
           *reinterpret_cast<uint4*>(tp + 2 * PART + part_at(i, j8)) = take_part8(o);
+          *reinterpret_cast<uint4*>(tp + 3 * PART + part_at(i, j8)) = take_part8(o);
         } else {
           float* at = warp == 1 && j8 < 32 ? off32 + (i - 32) * OFF_LD + j8
                                            : ((j8 / 16) & 1 ? row_odd : row_even) + (j8 % 16);
@@ -883,27 +886,25 @@ __global__ void __launch_bounds__(C_THREADS, 1)
     float r[32];
     auto beta_v = [&](int c) {               // r = beta V of chunk c
       const int st = c % C_STAGES;
-      wait(&bars.full[st], c / C_STAGES);
-      if (unit) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) r[j] = 0.f;
-        return;
-      }
+      wait(&bars.full[st], c / C_STAGES);    // beta
+      wait(&bars.v_loaded[c % 2], c / 2);
       const __nv_bfloat16* vt =
-          reinterpret_cast<const __nv_bfloat16*>(smem + st * C::STAGE_BYTES + C::KQ_BYTES) + h * 32 * 128 + row;
+          reinterpret_cast<const __nv_bfloat16*>(smem + C::V_OFF + (c % 2) * C::V_BYTES) + h * 32 * 128 + row;
       const float* bs = b_of(st) + h * 32;
+      // beta is 0 at steps of no sequence and masked ones, whatever V holds there
+      auto times = [&](float be, int j) { return unit || be == 0.f ? 0.f : be * __bfloat162float(vt[j * 128]); };
 #pragma unroll
       for (int j = 0; j < 32; j += 4) {
         const float4 be = at4(bs + j);
-        r[j] = be.x * __bfloat162float(vt[j * 128]);
-        r[j + 1] = be.y * __bfloat162float(vt[(j + 1) * 128]);
-        r[j + 2] = be.z * __bfloat162float(vt[(j + 2) * 128]);
-        r[j + 3] = be.w * __bfloat162float(vt[(j + 3) * 128]);
+        r[j] = times(be.x, j);
+        r[j + 1] = times(be.y, j + 1);
+        r[j + 2] = times(be.z, j + 2);
+        r[j + 3] = times(be.w, j + 3);
       }
     };
     const size_t y_step = (size_t)p.Hv * p.Dv;
     __nv_bfloat16* out = p.y + ((first + h * 32) * p.Hv + hv) * p.Dv + dv0;
-    auto yt_of = [&](int c) { return smem + (c % C_STAGES) * C::STAGE_BYTES + C::KQ_BYTES + h * 32 * 256; };
+    auto yt_of = [&](int c) { return smem + C::V_OFF + (c % 2) * C::V_BYTES + h * 32 * 256; };
     uint32_t d[2][16];
     float co[16];
     // Turn c ends chunk c - 1 (its state, its y) and begins chunk c.
@@ -1010,7 +1011,8 @@ __global__ void __launch_bounds__(C_THREADS, 1)
           x[j + 1] = r[jj + 1];
         }
         if (b == 0) load16(nbc + 16, co);
-        store_parts<2>({ta + C::COL_R + h * 16 + 8 * b, ta + C::COL_R + 32 + h * 16 + 8 * b}, x);
+        store_parts<3>({ta + C::COL_R + h * 16 + 8 * b, ta + C::COL_R + 32 + h * 16 + 8 * b,
+                        ta + C::COL_Y + h * 32 + 8 * b}, x);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -1035,7 +1037,7 @@ __global__ void __launch_bounds__(C_THREADS, 1)
         if (b == 0) load16(us + 16, co);
         store_parts<3>({ta + C::COL_S + h * 16 + 8 * b, ta + C::COL_S + 32 + h * 16 + 8 * b,
                         ta + C::COL_S + 64 + h * 16 + 8 * b}, w);
-        store_parts<1>({ta + C::COL_R + h * 16 + 8 * b}, x);
+        store_parts<2>({ta + C::COL_R + h * 16 + 8 * b, ta + C::COL_R + 32 + h * 16 + 8 * b}, x);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -1059,7 +1061,7 @@ __global__ void __launch_bounds__(C_THREADS, 1)
     if (warp == 12) {
       for (int c = 0; c < chunks; ++c) {
         const int ts = c % 2;
-        const uint32_t kq = smem_base + (c % C_STAGES) * C::STAGE_BYTES;
+        const uint32_t kq = smem_base + (c % C_STAGES) * C::KQ_BYTES;
         const uint32_t tp = smem_base + C::TP_OFF + ts * C::TP_BYTES;
         wait(&bars.full[c % C_STAGES], c / C_STAGES);
         wait(&bars.s_ready, c);
@@ -1074,11 +1076,14 @@ __global__ void __launch_bounds__(C_THREADS, 1)
         wait(&bars.tp_full[ts], c / 2);
         wait(&bars.r_ready, c);
         tc_fence_after();
-        // first parts, then second part x first part both ways round
+        // two parts of R with two of T, the third with T's first
 #pragma unroll
-        for (int m = 0; m < 3; ++m)
-          mma_bf16_ts_warp_x4<2>(tmem + C::COL_D, tmem + C::COL_R + (m == 1 ? 32 : 0),
-                                 make_sw128_desc(tp + (m == 2 ? PART : 0)), ID64, m > 0);
+        for (int m = 0; m < 4; ++m)
+          mma_bf16_ts_warp_x4<2>(tmem + C::COL_D, tmem + C::COL_R + (m & 1 ? 32 : 0),
+                                 make_sw128_desc(tp + (m & 2 ? PART : 0)), ID64, m > 0);
+#pragma unroll
+        for (int k = 0; k < CH / 16; ++k)
+          mma_bf16_ts_warp(tmem + C::COL_D, tmem + C::col_r3(k), make_sw128_desc(tp + k * 32), ID64, 1);
         tc_commit_warp(&bars.d3_done);
         wait(&bars.delta_ready, c);
         // [K; Q] K^T of the next chunk has left the second half of these columns
@@ -1092,7 +1097,7 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       }
     } else if (warp == 14) {
       auto grams = [&](int c) {   // [K; Q] K^T
-        const uint32_t kq = smem_base + (c % C_STAGES) * C::STAGE_BYTES;
+        const uint32_t kq = smem_base + (c % C_STAGES) * C::KQ_BYTES;
         wait(&bars.full[c % C_STAGES], c / C_STAGES);
 #pragma unroll
         for (int a = 0; a < DK / 64; ++a)
@@ -1104,7 +1109,7 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       wait(&bars.g_read, 0);
       for (int c = 0; c < chunks; ++c) {
         const int ts = c % 2;
-        const uint32_t kq = smem_base + (c % C_STAGES) * C::STAGE_BYTES;
+        const uint32_t kq = smem_base + (c % C_STAGES) * C::KQ_BYTES;
         const uint32_t tp = smem_base + C::TP_OFF + ts * C::TP_BYTES;
         wait(&bars.s_ready, c);
         // the last chunk's Delta K has been read, its second half is free until
@@ -1122,7 +1127,10 @@ __global__ void __launch_bounds__(C_THREADS, 1)
         tc_commit_warp(&bars.q_done);
         wait(&bars.delta_ready, c);
         tc_fence_after();
-        mma_bf16_ts_warp_x4<2>(tmem + C::COL_Y, tmem + C::COL_R, make_sw128_desc(tp + 2 * PART), ID64, 0);
+#pragma unroll
+        for (int m = 0; m < 3; ++m)
+          mma_bf16_ts_warp_x4<2>(tmem + C::COL_Y, tmem + C::COL_R + (m == 1 ? 32 : 0),
+                                 make_sw128_desc(tp + (m == 2 ? 3 : 2) * PART), ID64, m > 0);
         tc_commit_warp(&bars.y_done);
         tc_commit_warp(&bars.tp_freed[ts]);
       }
@@ -1132,25 +1140,41 @@ __global__ void __launch_bounds__(C_THREADS, 1)
     } else if (warp == 13 && lane == 0) {
       // loads, on a thread of their own: issuing a chunk's five takes about as
       // long (2000 cycles) as a round of products
+      auto load_v = [&](int c) {
+        uint64_t* bar = &bars.v_loaded[c % 2];
+        mbar_arrive_expect_tx(bar, C::V_BYTES);
+        tma_load_2d(smem + C::V_OFF + (c % 2) * C::V_BYTES, &tm_v, bar, hv * p.Dv + dv0, int(first) + c * CH);
+      };
+      load_v(0);
+      if (chunks > 1) load_v(1);
       for (int c = 0; c < chunks; ++c) {
-        // chunk c - 3 is done with the stage: its products are complete and its
-        // values read (the next state came after both).  Every phase is waited
-        // for in turn: a parity alone does not tell phase 1 from none.
+        // Chunk c - 3 is done with the stage: its products are complete (the next
+        // state came after them).  So is V's buffer of chunk c - 3, over which
+        // the y of chunk c - 4 was turned: it takes chunk c - 1.  Every phase is
+        // waited for in turn: a parity alone does not tell phase 1 from none.
         if (c == C_STAGES) wait(&bars.s_ready, 0);
-        if (c >= C_STAGES) wait(&bars.s_ready, c - C_STAGES + 1);
-        uint8_t* kq = smem + (c % C_STAGES) * C::STAGE_BYTES;
+        if (c >= C_STAGES) {
+          wait(&bars.s_ready, c - C_STAGES + 1);
+          load_v(c - 1);
+        }
+        uint8_t* kq = smem + (c % C_STAGES) * C::KQ_BYTES;
         uint64_t* bar = &bars.loaded[c % C_STAGES];
         const int tok = int(first) + c * CH;
-        mbar_arrive_expect_tx(bar, C::STAGE_BYTES);
+        mbar_arrive_expect_tx(bar, C::KQ_BYTES);
         for (int a = 0; a < DK / 64; ++a) {
           tma_load_2d(kq + a * C::ATOM, &tm_k, bar, hk * DK + a * 64, tok);
           tma_load_2d(kq + a * C::ATOM + 64 * 128, &tm_q, bar, hk * DK + a * 64, tok);
         }
-        tma_load_2d(kq + C::KQ_BYTES, &tm_v, bar, hv * p.Dv + dv0, tok);
+      }
+      if (chunks >= C_STAGES) {
+        if (chunks == C_STAGES) wait(&bars.s_ready, 0);
+        wait(&bars.s_ready, chunks - C_STAGES + 1);
+        load_v(chunks - 1);
       }
       // whatever went wrong elsewhere, no copy is in flight when the CTA leaves
       for (int c = max(0, chunks - C_STAGES); c < chunks; ++c)
         mbar_wait(&bars.loaded[c % C_STAGES], (c / C_STAGES) & 1);
+      for (int c = max(0, chunks - 2); c < chunks; ++c) mbar_wait(&bars.v_loaded[c % 2], (c / 2) & 1);
     }
   }
   __syncwarp();
