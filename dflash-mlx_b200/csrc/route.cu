@@ -166,8 +166,8 @@ __global__ void route_kernel(const Params p) {
 // be runs of whole lanes: n_groups a power of two up to 32 and E = 32 EPL, or
 // one group.
 //
-// Bound by the instructions of the 64-bit scores and of the k rounds, about 1000
-// a token.
+// Bound by the instructions of the 64-bit scores and of the k rounds (8191 tokens
+// of 256 experts: 27 us, where their 4.7 MB would take 0.7).
 template <typename T, int EPL>
 __global__ void __launch_bounds__(128) route_lanes_kernel(const Params p) {
   constexpr unsigned ALL = 0xffffffffu;
@@ -275,8 +275,8 @@ __global__ void __launch_bounds__(128) route_lanes_kernel(const Params p) {
 }
 
 // The register form where the sizes fit it, else the one on shared memory.
-// Measured at 256 experts, 8 groups, top 8: 16 tokens 5 us for 14 us, 8191
-// tokens 16 us for 45 us.
+// Measured at 256 experts, 8 groups, top 8: 16 tokens 6.2 us for 14.4 us, 8191
+// tokens 27 us for 45 us.
 template <typename T>
 bool launch_lanes(const Params& p, cudaStream_t stream) {
   const bool runs = (p.groups & (p.groups - 1)) == 0 && p.groups <= 32;

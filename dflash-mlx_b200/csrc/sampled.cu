@@ -11,7 +11,8 @@
 // The committed tokens are then distributed as samples of the target alone.
 // z = 0 (or below, or NaN) is greedy: p_i is all on the largest logit's id.
 //
-// Three or four launches.  rows_kernel reads every row once (the one pass that is bound
+// Three to five launches, each after the first started early.  mask_kernel packs
+// the suppress mask into bits, if there is one.  rows_kernel reads every row once (the one pass that is bound
 // by HBM): maximum, its id and sum of exponentials of each segment, in 32 bits.
 // decide_kernel joins a request's segments and accepts.  Where the next token
 // comes from a difference of two softmaxes, norm_kernel adds the two rows'

@@ -195,7 +195,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
       of 0 and 1 included) and starts from ``state[n]``, ``[N, Hv, Dv, Dk]``.
 
     ``out`` receives y (rows that belong to no sequence are left as they were;
-    a new y has zeros there).  ``out_state`` receives the new state and may be
+    a new y has zeros there) and shares no memory with q, k and v.  ``out_state`` receives the new state and may be
     ``state`` itself; without it ``state`` is left untouched.  Nothing is read
     back to the host; the call can be captured into a CUDA graph.
     """
@@ -249,6 +249,8 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     elif (out.dtype != bf16 or out.shape != (b, t_steps, hv, dv) or not out.is_contiguous()
           or out.data_ptr() % 16 != 0):
         raise ValueError(f"out must be contiguous, 16-byte aligned bf16 {(b, t_steps, hv, dv)}")
+    elif any(out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr() for x in (q, k, v)):
+        raise ValueError("out must not share memory with q, k or v")
     if out_state is None:
         out_state = torch.empty(shape, dtype=f32, device=dev)
         state = _aligned(state)

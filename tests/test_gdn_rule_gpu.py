@@ -139,6 +139,26 @@ def test_mask(pkg, dev, t, dk, dv):
     _check(y, s, *ref, arrays, t)
 
 
+@pytest.mark.parametrize("lens", [[3, 1, 5], [40, 0, 90, 64], [700, 900]])
+def test_mask_over_packed_sequences(pkg, dev, lens):
+    arrays = _inputs(sum(lens), 1, sum(lens), 1, 2, 128, 128, n=len(lens))
+    cu = np.cumsum([0] + lens)
+    mask = np.random.default_rng(8).random((1, sum(lens))) < 0.6
+    ref = ogdn.gated_delta_rule(*arrays, mask=mask, lens=list(zip(cu[:-1].tolist(), cu[1:].tolist())))
+    for a in arrays[:5]:
+        a[~mask] = np.nan
+    y, s = pkg.gated_delta_rule(*_dev(arrays, dev), mask=torch.from_numpy(mask).to(dev),
+                                cu_seqlens=torch.from_numpy(cu.astype(np.int32)).to(dev))
+    clean = tuple(np.nan_to_num(a) for a in arrays)
+    _check(y, s, *ref, clean, max(lens))
+
+
+def test_no_sequences(pkg, dev):
+    arrays = _inputs(4, 1, 30, 1, 2, 128, 128, n=0)
+    y, s = pkg.gated_delta_rule(*_dev(arrays, dev), cu_seqlens=torch.zeros(1, dtype=torch.int32, device=dev))
+    assert torch.all(y == 0) and s.shape == (0, 2, 128, 128)
+
+
 def test_no_steps(pkg, dev):
     arrays = _inputs(3, 2, 0, 2, 4, 64, 32)
     y, s = pkg.gated_delta_rule(*_dev(arrays, dev))
@@ -329,6 +349,9 @@ def test_refusals(pkg, dev):
         call(out=torch.empty(2, 4, 4, 32, device=dev))
     with pytest.raises(ValueError):
         call(out_state=torch.empty(2, 4, 64, 32, device=dev))
+    shared = torch.empty(2 * 4 * 4 * 32, dtype=torch.bfloat16, device=dev).view(2, 4, 4, 32)
+    with pytest.raises(ValueError, match="share"):
+        call(2, shared, out=shared)
     one = [x[:1] for x in ins[:5]]
     with pytest.raises(ValueError):
         pkg.gated_delta_rule(*one, ins[5], cu_seqlens=cu.long())
