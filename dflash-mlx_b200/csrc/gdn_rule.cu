@@ -249,8 +249,8 @@ int launch_recurrent(const RuleParams& p, cudaStream_t stream) {
 constexpr int CH = 64;               // steps of a chunk
 constexpr int C_THREADS = 16 * 32;
 // Registers of a thread after the split; the launch has 128 for each, and
-// 128 (preparation, as launched) + 2 x 168 + 48 = 4 x 128.
-constexpr int C_REGS_STATE = 168, C_REGS_ISSUE = 48;
+// 96 + 2 x 184 + 48 = 4 x 128.
+constexpr int C_REGS_PREP = 96, C_REGS_STATE = 184, C_REGS_ISSUE = 48;
 constexpr int C_ORDER = 256;         // packed sequences that are taken longest first
 constexpr int C_STAGES = 3;
 constexpr int C_PREP = 128, C_STATE = 256;
@@ -710,6 +710,7 @@ __global__ void __launch_bounds__(C_THREADS, 1)
 
   if (warp < 4) {
     // ---------------------------------------------------------- preparation
+    fewer_registers<C_REGS_PREP>();
     const int t = threadIdx.x;
     // Chunk c's tiles have landed: zeros over rows of no step, g and beta (1
     // and 0 there: a step that changes nothing) beside them.
