@@ -892,15 +892,18 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       const __nv_bfloat16* vt =
           reinterpret_cast<const __nv_bfloat16*>(smem + C::V_OFF + (c % 2) * C::V_BYTES) + h * 32 * 128 + row;
       const float* bs = b_of(st) + h * 32;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) r[j] = __bfloat162float(vt[j * 128]);
       // beta is 0 at steps of no sequence and masked ones, whatever V holds there
-      auto times = [&](float be, int j) { return unit || be == 0.f ? 0.f : be * __bfloat162float(vt[j * 128]); };
 #pragma unroll
       for (int j = 0; j < 32; j += 4) {
-        const float4 be = at4(bs + j);
-        r[j] = times(be.x, j);
-        r[j + 1] = times(be.y, j + 1);
-        r[j + 2] = times(be.z, j + 2);
-        r[j + 3] = times(be.w, j + 3);
+        const float4 x = at4(bs + j);
+        const float be[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y = be[e] * r[j + e];
+          r[j + e] = be[e] == 0.f || unit ? 0.f : y;
+        }
       }
     };
     const size_t y_step = (size_t)p.Hv * p.Dv;
