@@ -1189,12 +1189,12 @@ __global__ void __launch_bounds__(C_THREADS, 1)
 }
 
 // Pieces of a sequence (lengths of packed ones are known on the device only:
-// their mean is taken).  In units of a chunk's time (5 us): whole, L; in n
+// their mean is taken).  In units of a chunk's time (5.4 us): whole, L; in n
 // pieces, two launches of L / n chunks that are 1.25 long with every SM at work,
 // 6 for starting two launches more and 0.6 for a step of the chain.  Measured,
-// us whole and cut, 8192 and 2048 steps: 48 heads 658 / 526 and 174 / 172 (3
-// pieces), 16 heads 654 / 327 and 172 / 152 (6), 8 heads of 64 x 64 525 / 181 and
-// 138 / 85 (10); 1024 steps of 48 heads 94 / 118: left whole.
+// us whole and cut: 48 heads 695 / 581 at 8192 steps, 355 / 332 at 4096 (3 pieces;
+// 183 at 2048, left whole), 16 heads 690 / 321 at 8192 and 182 / 119 at 2048 (6), 4
+// heads 686 / 171 and 181 / 93 (16), 8 heads of 64 x 64 616 / 165 and 160 / 71 (10).
 inline int pieces(long long heads, int tiles, long long chunks, int sms) {
   int best = 1;
   double least = 0.95 * double(chunks);

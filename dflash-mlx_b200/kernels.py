@@ -195,9 +195,12 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
       of 0 and 1 included) and starts from ``state[n]``, ``[N, Hv, Dv, Dk]``.
 
     ``out`` receives y (rows that belong to no sequence are left as they were;
-    a new y has zeros there) and shares no memory with q, k and v.  ``out_state`` receives the new state and may be
-    ``state`` itself; without it ``state`` is left untouched.  Nothing is read
-    back to the host; the call can be captured into a CUDA graph.
+    a new y has zeros there) and shares no storage with q, k and v.
+    ``out_state`` receives the new state and may be ``state`` itself; without it
+    ``state`` is left untouched.  Nothing is read back to the host; the call can
+    be captured into a CUDA graph.  A NaN or an infinity in a step that counts
+    reaches what follows it, as in the recurrence, and may reach the y of up to
+    63 steps before it (steps are taken 64 at a time).
     """
     require_cuda(state, "state")
     dev = state.device
@@ -273,7 +276,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     tail = (beta.data_ptr(), mask_ptr, cu_ptr, state.data_ptr(), out_state.data_ptr(), out.data_ptr(),
             1 if zero_gaps else 0, seqs, t_steps, hv, hk, dv, dk)
     with on_device(dev):
-        if not vector and (dk == 128 or dk == 64) and steps >= _CHUNKED_STEPS:
+        if not vector and (dk == 128 or dk == 64) and steps >= _chunked_from(seqs * hv * -(-dv // 128), dv, dk):
             entry = "dfl_gdn_rule_chunked"
             status = ctypes.c_int(0)
             n = lib.dfl_gdn_rule_workspace_bytes(seqs, t_steps, 0 if cu_ptr is None else 1, hv, dv, dk,
@@ -289,10 +292,19 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     return out, out_state
 
 
-#: Mean steps per sequence from which 64 steps at a time are faster than one
-#: after the other (48 heads of 128 x 128, one and 40 sequences: 16 steps 13 and 197 us
-#: against 18 and 253, 32 steps 23 and 354 us against 18 and 248).
-_CHUNKED_STEPS = 24
+def _chunked_from(tiles: int, dv: int, dk: int) -> int:
+    """Mean steps of a sequence from which 64 steps at a time are faster than
+    one after the other.  A chunk takes much the same time for any size of the
+    state (up to 128 rows) and has an SM to itself, so small states need more
+    steps once there are more of them than SMs.  Measured, us one after the other and 64 at a time,
+    24 and 64 steps: one sequence of 48 heads of 128 x 128 18.4 / 17.8 and 43 /
+    18, 40 of those 274 / 240 and 671 / 239; 80 heads of 64 x 64 12.3 / 12.7 and
+    27.5 / 12.6, 320 of those 17 / 36 and 39.6 / 35.0; 640 heads of 128 x 64 (Dv x
+    Dk) 41 / 64 and 100 / 65, equal at 40 steps."""
+    size = dk * min(dv, 128)
+    if tiles <= 148 or size >= 128 * 128:
+        return 24
+    return 40 if size >= 128 * 64 else 64
 
 
 def _aligned(x: torch.Tensor) -> torch.Tensor:

@@ -153,6 +153,16 @@ def test_mask_over_packed_sequences(pkg, dev, lens):
     _check(y, s, *ref, clean, max(lens))
 
 
+@pytest.mark.parametrize("t", [24, 39, 40, 63, 64])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (64, 128), (128, 32)])
+def test_many_small_heads(pkg, dev, t, dk, dv):
+    """More heads than SMs, steps on both sides of where 64 are taken at a time."""
+    arrays = _inputs(31 + t, 19, t, 4, 8, dk, dv)
+    y, s = pkg.kernels.gated_delta_rule(*_dev(arrays, dev))
+    ry, rs = ogdn.gated_delta_rule(*arrays)
+    _check(y, s, ry, rs, arrays, t)
+
+
 def test_no_sequences(pkg, dev):
     arrays = _inputs(4, 1, 30, 1, 2, 128, 128, n=0)
     y, s = pkg.gated_delta_rule(*_dev(arrays, dev), cu_seqlens=torch.zeros(1, dtype=torch.int32, device=dev))
