@@ -72,7 +72,10 @@ __device__ __forceinline__ void zero_gap_rows(const RuleParams& p, int n, int hv
 // end in log2(LPR) shuffles.  A thread owns two rows, which share the k and q
 // chunks read from shared memory.  The inputs of up to 16 steps are staged at
 // a time; at one token per sequence the kernel is a pass over the state: read
-// once, written once.
+// once, written once.  40 tokens of 48 heads of 128 x 128 (253 MB) take 54 us,
+// 71% of the measured copy rate; one token 3.9 us, launch and one trip to
+// memory.  Over more steps it is bound by fp32 arithmetic and the shuffles: 0.5
+// us a step of one sequence of 48 heads.
 constexpr int R_THREADS = 128;
 
 template <int DK>
@@ -240,6 +243,14 @@ int launch_recurrent(const RuleParams& p, cudaStream_t stream) {
 // to R in fp32; T - I has two (16 bits: it is a correction).  In y, which ends
 // in 8 bits, the state, P and Delta have two parts (one each of P and Delta would
 // add 2.2e-3 of y to the 1.7e-3 of its last rounding).
+//
+// Bound by the chain through a chunk, not by a rate: S K^T, R, R T^T, Delta, Delta
+// K and the new state wait for one another, 5.4 us (about 10700 cycles) a chunk
+// of a 128 x 128 head.  Most of it is the state's threads at work: 2600 cycles on
+// the last chunk's y, 800 on R, 1100 on Delta, 2100 on beta V, 1800 on the state;
+// they wait 2300 for products.  The preparing warps need 9600 for T and P of the
+// next chunk, beside it.  8192 steps of 48 heads, cut in three, 597 us; 16091
+// steps in 8 prompts 565 us, of which the longest's 79 chunks alone are 430.
 //
 // Warps: 0-3 prepare T and P of the next chunk (K K^T and Q K^T from one
 // product, inverse by blocks of 16, 32 and 64 in fp32) and put zeros over rows

@@ -12,14 +12,15 @@
 // z = 0 (or below, or NaN) is greedy: p_i is all on the largest logit's id.
 //
 // Three to five launches, each after the first started early.  mask_kernel packs
-// the suppress mask into bits, if there is one.  rows_kernel reads every row once (the one pass that is bound
-// by HBM): maximum, its id and sum of exponentials of each segment, in 32 bits.
+// the suppress mask into bits, if there is one.  rows_kernel reads every row once
+// (the one pass that is bound by HBM): maximum, its id and sum of exponentials
+// of each segment, in 32 bits.
 // decide_kernel joins a request's segments and accepts.  Where the next token
 // comes from a difference of two softmaxes, norm_kernel adds the two rows'
 // exponentials again in 64 bits.  pick_kernel adds the weights of that one
-// row's segments in 64 bits, and the last CTA of a request finds the segment and the id.  The 64
-// bits are for the id: with 2^18 ids a weight is 2^-18 of the total, and a sum
-// in 32 bits would move a border by a sizeable part of it.
+// row's segments in 64 bits, and the last CTA of a request finds the segment and
+// the id.  The 64 bits are for the id: with 2^18 ids a weight is 2^-18 of the
+// total, and a sum in 32 bits would move a border by a sizeable part of it.
 //
 // A logit that is NaN or -inf has probability 0; rows with +inf spread over
 // those ids.  A row that has nothing left gives token -1.
@@ -253,7 +254,9 @@ __global__ void __launch_bounds__(THREADS) mask_kernel(const Params p) {
 // ex2, add.  m c is rounded once per maximum, a common factor of all terms that
 // is taken out again at the end.  The quick loop moves the maximum at most
 // once in U vectors; a thread that met NaN or +inf, or nothing above the
-// lowest value, goes over its ids again one by one.
+// lowest value, goes over its ids again one by one.  1488 bf16 rows of 248,320
+// ids (739 MB): 158 us, 72% of the measured copy rate, bound by the issue of
+// its 5 instructions an id beside the loads.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
   __shared__ Stat sh[WARPS];
@@ -604,7 +607,8 @@ __global__ void __launch_bounds__(32 * DECIDE_WARPS) decide_kernel(const Params 
 }
 
 // The 64-bit sums of segment blockIdx.x of the two rows whose difference a
-// request draws from.
+// request draws from.  Bound by 64-bit arithmetic (a dozen operations an
+// exponential): 48 requests of 248,320 ids 34 us.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) norm_kernel(const Params p) {
   __shared__ double sh[WARPS];
@@ -679,6 +683,10 @@ __device__ __forceinline__ double fixed_sum(const double* x, int n, double* sh) 
   return block_sum(t, sh);
 }
 
+// The token: each warp adds its segments' weights; the CTA of a request that
+// comes last finds the segment in which the sum passes sample_u x total, then
+// the id in it.  Bound as norm_kernel is, and by the one CTA at the end: 58 us
+// for 48 requests of 248,320 ids with draft rows.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) pick_kernel(const Params p) {
   __shared__ double sh[WARPS];
