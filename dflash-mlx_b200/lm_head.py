@@ -210,6 +210,8 @@ def verify_accept_sampled(logits: torch.Tensor, verify_ids: torch.Tensor, accept
             raise ValueError(f"suppress_token_mask must be {(v,)}")
         suppress_token_mask = mask_bytes(suppress_token_mask, "suppress_token_mask")
         sup_ptr = suppress_token_mask.data_ptr()
+    if verify_ids.dtype != i32:
+        verify_ids = verify_ids.clamp(-1, v)   # ids past 32 bits stay outside the vocabulary
     ids = verify_ids.to(i32).contiguous()
     accept_u, sample_u = accept_u.contiguous(), sample_u.contiguous()
     acc = torch.empty(b, dtype=i32, device=dev)

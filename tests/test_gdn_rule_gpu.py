@@ -317,6 +317,31 @@ def test_captured_and_on_another_stream(pkg, dev, t):
     assert torch.equal(got[1][0], again[0]) and torch.equal(got[1][1], again[1])
 
 
+@pytest.mark.parametrize("t,hk,hv", [(1800, 1, 2), (300, 2, 4), (20, 2, 4)])
+def test_replayed_with_other_offsets(pkg, dev, t, hk, hv):
+    """A captured packed call holds for any offsets, those that leave all but one
+    sequence empty among them."""
+    arrays = _inputs(41, 1, t, hk, hv, 128, 64, n=3)
+    ins = _dev(arrays, dev)
+    cu = torch.tensor([0, t // 3, t // 2, t], dtype=torch.int32, device=dev)
+    side, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        pkg.gated_delta_rule(*ins, cu_seqlens=cu)
+        side.synchronize()
+        with torch.cuda.graph(g, stream=side):
+            y, s = pkg.gated_delta_rule(*ins, cu_seqlens=cu)
+    for ends in ([0, t // 3, t // 2, t], [0, 0, t, t], [0, 1, 2, t - 1], [t, t, t, t]):
+        cu.copy_(torch.tensor(ends, dtype=torch.int32))
+        g.replay()
+        torch.cuda.synchronize()
+        ry, rs = np.zeros(y.shape), np.zeros(s.shape)
+        for n in range(3):
+            part = [a[:, ends[n]:ends[n + 1]] for a in arrays[:5]] + [arrays[5][n:n + 1]]
+            ry[:, ends[n]:ends[n + 1]], rs[n:n + 1] = ogdn.gated_delta_rule(*part)
+        _check(y, s, ry, rs, arrays, t)
+
+
 def test_refusals(pkg, dev):
     ins = list(_dev(_inputs(27, 2, 4, 2, 4, 64, 32), dev))
 

@@ -204,6 +204,17 @@ def test_ids_outside_the_vocabulary_and_bad_lengths(pkg, dev):
     _same(got, _ref(c))
 
 
+def test_ids_past_32_bits_are_outside_the_vocabulary(pkg, dev):
+    c = _case(16, 3, 4, 101, "fp32", False)
+    c["u"][:] = 0.0
+    args = [c["logits"].to(dev), c["ids"].to(dev).long(), c["u"].to(dev), c["s"].to(dev)]
+    args[1][0, 1] += 2**32
+    args[1][1, 2] -= 2**33
+    acc, _, prob = pkg.verify_accept_sampled(*args, temperature=c["temp"].to(dev).clamp(min=0.5))
+    assert acc.tolist() == [0, 1, 3]
+    assert prob[0, 0] == 0 and prob[1, 1] == 0 and prob[2].min() > 0
+
+
 def test_uniforms_at_the_ends(pkg, dev):
     """u = 0 accepts whatever has a probability and draws the first such id;
     1 (outside the range), the last one; NaN draws as 0 and accepts nothing."""
