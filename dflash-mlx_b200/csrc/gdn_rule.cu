@@ -604,6 +604,11 @@ __global__ void __launch_bounds__(C_THREADS, 1)
   __shared__ volatile int abort_word;
   __shared__ int chosen;
 
+  if (threadIdx.x == 13 * 32 && p.T > 0) {   // without a step there are no maps
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_v);
+  }
   const int tiles = (p.Dv + 127) / 128;
   const int job = blockIdx.x % sp.jobs;
   const int hv = (blockIdx.x / sp.jobs) % p.Hv;
@@ -625,6 +630,7 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       for (int u = 0; u < p.B; ++u) rank += lens[u] > lens[t] || (lens[u] == lens[t] && u < t);
       if (rank == n) chosen = t;
     }
+    fence_proxy_async_shared();   // the first copies land over lens
     __syncthreads();
     n = chosen;
   }
@@ -679,13 +685,26 @@ __global__ void __launch_bounds__(C_THREADS, 1)
   auto nbc_of = [&](int s) { return small + C_STAGES * 2 * CH + s * 3 * CH + 2 * CH; };
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < C_STAGES; ++s) {
-      mbar_init(&bars.loaded[s], 1);
-      mbar_init(&bars.full[s], C_PREP);
+  auto load_kq = [&](int c) {
+    uint8_t* kq = smem + (c % C_STAGES) * C::KQ_BYTES;
+    uint64_t* bar = &bars.loaded[c % C_STAGES];
+    const int tok = int(first) + c * CH;
+    mbar_arrive_expect_tx(bar, C::KQ_BYTES);
+    for (int a = 0; a < DK / 64; ++a) {
+      tma_load_2d(kq + a * C::ATOM, &tm_k, bar, hk * DK + a * 64, tok);
+      tma_load_2d(kq + a * C::ATOM + 64 * 128, &tm_q, bar, hk * DK + a * 64, tok);
     }
+  };
+  if (threadIdx.x == 13 * 32) {
+    // the first chunk's copies are on their way while the rest is set up
+    for (int s = 0; s < C_STAGES; ++s) mbar_init(&bars.loaded[s], 1);
+    for (int s = 0; s < 2; ++s) mbar_init(&bars.v_loaded[s], 1);
+    fence_barrier_init();
+    load_kq(0);
+  }
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C_STAGES; ++s) mbar_init(&bars.full[s], C_PREP);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&bars.v_loaded[s], 1);
       mbar_init(&bars.tp_full[s], C_PREP);
       mbar_init(&bars.tp_freed[s], 1 + C_STATE / 32);
     }
@@ -881,18 +900,36 @@ __global__ void __launch_bounds__(C_THREADS, 1)
     more_registers<C_REGS_STATE>();
     const int h = (warp - 4) / 4;            // which half of the columns
     const int row = (warp % 4) * 32 + lane;  // TMEM lane, value row dv0 + row
-    const bool live = row < cols;
     const uint32_t ta = tmem + (uint32_t((warp % 4) * 32) << 16);
     constexpr int NS = DK / 2;               // state columns of this thread
+    // The warp's 32 rows of half the columns go through shared memory both ways,
+    // so that neighbouring lanes read and write neighbouring 16 bytes (with a row
+    // per lane the state's 64 KB took 3400 cycles to come, the first chunk's
+    // copies waiting behind them, and 5900 to go).
+    constexpr int X = NS / 4;                // 16-byte pieces of a row
+    auto piece_of = [&](float4* part, int r, int x) { return part + r * X + (x ^ (r & (X - 1))); };
     float s[NS];
+    if (src) {
+      // over the second and third stage, which wait for s_ready
+      float4* part = reinterpret_cast<float4*>(smem + C::KQ_BYTES) + (warp - 4) * 32 * X;
 #pragma unroll
-    for (int i = 0; i < NS; i += 4) {
-      const float4 x = live && src ? at4(src + (size_t)row * DK + h * NS + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-      s[i] = x.x; s[i + 1] = x.y; s[i + 2] = x.z; s[i + 3] = x.w;
-    }
-    if (unit) {
+      for (int i = 0; i < X; ++i) {
+        const int r = i * (32 / X) + lane / X, x = lane % X, at = (warp % 4) * 32 + r;
+        cp_async_16(smem_u32(piece_of(part, r, x)), src + (size_t)(at < cols ? at : 0) * DK + h * NS + 4 * x,
+                    at < cols ? 16 : 0);
+      }
+      cp_async_commit();
+      cp_async_wait_all();
+      __syncwarp();
 #pragma unroll
-      for (int i = 0; i < NS; ++i) s[i] = row == h * NS + i ? 1.f : 0.f;
+      for (int i = 0; i < X; ++i) {
+        const float4 x = *piece_of(part, lane, i);
+        s[4 * i] = x.x; s[4 * i + 1] = x.y; s[4 * i + 2] = x.z; s[4 * i + 3] = x.w;
+      }
+      fence_proxy_async_shared();
+    } else {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) s[i] = unit && row == h * NS + i ? 1.f : 0.f;
     }
     const uint32_t s_col = ta + C::COL_S + h * (NS / 2);
     float r[32];
@@ -1058,11 +1095,18 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       tc_fence_before();
       mbar_arrive(&bars.delta_ready);
     }
-    if (live && dst) {
-      dst += (size_t)row * DK + h * NS;
+    if (dst) {
+      // over the first two stages, which every product has read
+      float4* part = reinterpret_cast<float4*>(smem) + (warp - 4) * 32 * X;
 #pragma unroll
-      for (int i = 0; i < NS; i += 4)
-        *reinterpret_cast<float4*>(dst + i) = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
+      for (int i = 0; i < X; ++i)
+        *piece_of(part, lane, i) = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < X; ++i) {
+        const int r = i * (32 / X) + lane / X, x = lane % X, at = (warp % 4) * 32 + r;
+        if (at < cols) *reinterpret_cast<float4*>(dst + (size_t)at * DK + h * NS + 4 * x) = *piece_of(part, r, x);
+      }
     }
   } else {
     // ----------------------------------------------------- loads and products
@@ -1161,28 +1205,21 @@ __global__ void __launch_bounds__(C_THREADS, 1)
         tma_load_2d(smem + C::V_OFF + (c % 2) * C::V_BYTES, &tm_v, bar, hv * p.Dv + dv0, int(first) + c * CH);
       };
       load_v(0);
-      if (chunks > 1) load_v(1);
-      for (int c = 0; c < chunks; ++c) {
+      for (int c = 1; c < chunks; ++c) {
         // Chunk c - 3 is done with the stage: its products are complete (the next
         // state came after them).  So is V's buffer of chunk c - 3, over which
         // the y of chunk c - 4 was turned: it takes chunk c - 1.  Every phase is
-        // waited for in turn: a parity alone does not tell phase 1 from none.
-        if (c == C_STAGES) wait(&bars.s_ready, 0);
+        // waited for in turn: a parity alone does not tell phase 1 from none.  The
+        // first state came through the stages of chunks 1 and 2.
+        if (c == 1) wait(&bars.s_ready, 0);
         if (c >= C_STAGES) {
           wait(&bars.s_ready, c - C_STAGES + 1);
           load_v(c - 1);
         }
-        uint8_t* kq = smem + (c % C_STAGES) * C::KQ_BYTES;
-        uint64_t* bar = &bars.loaded[c % C_STAGES];
-        const int tok = int(first) + c * CH;
-        mbar_arrive_expect_tx(bar, C::KQ_BYTES);
-        for (int a = 0; a < DK / 64; ++a) {
-          tma_load_2d(kq + a * C::ATOM, &tm_k, bar, hk * DK + a * 64, tok);
-          tma_load_2d(kq + a * C::ATOM + 64 * 128, &tm_q, bar, hk * DK + a * 64, tok);
-        }
+        load_kq(c);
+        if (c == 1) load_v(1);
       }
       if (chunks >= C_STAGES) {
-        if (chunks == C_STAGES) wait(&bars.s_ready, 0);
         wait(&bars.s_ready, chunks - C_STAGES + 1);
         load_v(chunks - 1);
       }
