@@ -604,11 +604,6 @@ __global__ void __launch_bounds__(C_THREADS, 1)
   __shared__ volatile int abort_word;
   __shared__ int chosen;
 
-  if (threadIdx.x == 13 * 32 && p.T > 0) {   // without a step there are no maps
-    tma_prefetch_desc(&tm_k);
-    tma_prefetch_desc(&tm_q);
-    tma_prefetch_desc(&tm_v);
-  }
   const int tiles = (p.Dv + 127) / 128;
   const int job = blockIdx.x % sp.jobs;
   const int hv = (blockIdx.x / sp.jobs) % p.Hv;
@@ -630,7 +625,6 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       for (int u = 0; u < p.B; ++u) rank += lens[u] > lens[t] || (lens[u] == lens[t] && u < t);
       if (rank == n) chosen = t;
     }
-    fence_proxy_async_shared();   // the first copies land over lens
     __syncthreads();
     n = chosen;
   }
@@ -685,26 +679,13 @@ __global__ void __launch_bounds__(C_THREADS, 1)
   auto nbc_of = [&](int s) { return small + C_STAGES * 2 * CH + s * 3 * CH + 2 * CH; };
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  auto load_kq = [&](int c) {
-    uint8_t* kq = smem + (c % C_STAGES) * C::KQ_BYTES;
-    uint64_t* bar = &bars.loaded[c % C_STAGES];
-    const int tok = int(first) + c * CH;
-    mbar_arrive_expect_tx(bar, C::KQ_BYTES);
-    for (int a = 0; a < DK / 64; ++a) {
-      tma_load_2d(kq + a * C::ATOM, &tm_k, bar, hk * DK + a * 64, tok);
-      tma_load_2d(kq + a * C::ATOM + 64 * 128, &tm_q, bar, hk * DK + a * 64, tok);
-    }
-  };
-  if (threadIdx.x == 13 * 32) {
-    // the first chunk's copies are on their way while the rest is set up
-    for (int s = 0; s < C_STAGES; ++s) mbar_init(&bars.loaded[s], 1);
-    for (int s = 0; s < 2; ++s) mbar_init(&bars.v_loaded[s], 1);
-    fence_barrier_init();
-    load_kq(0);
-  }
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C_STAGES; ++s) mbar_init(&bars.full[s], C_PREP);
+    for (int s = 0; s < C_STAGES; ++s) {
+      mbar_init(&bars.loaded[s], 1);
+      mbar_init(&bars.full[s], C_PREP);
+    }
     for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars.v_loaded[s], 1);
       mbar_init(&bars.tp_full[s], C_PREP);
       mbar_init(&bars.tp_freed[s], 1 + C_STATE / 32);
     }
@@ -1204,6 +1185,17 @@ __global__ void __launch_bounds__(C_THREADS, 1)
         mbar_arrive_expect_tx(bar, C::V_BYTES);
         tma_load_2d(smem + C::V_OFF + (c % 2) * C::V_BYTES, &tm_v, bar, hv * p.Dv + dv0, int(first) + c * CH);
       };
+      auto load_kq = [&](int c) {
+        uint8_t* kq = smem + (c % C_STAGES) * C::KQ_BYTES;
+        uint64_t* bar = &bars.loaded[c % C_STAGES];
+        const int tok = int(first) + c * CH;
+        mbar_arrive_expect_tx(bar, C::KQ_BYTES);
+        for (int a = 0; a < DK / 64; ++a) {
+          tma_load_2d(kq + a * C::ATOM, &tm_k, bar, hk * DK + a * 64, tok);
+          tma_load_2d(kq + a * C::ATOM + 64 * 128, &tm_q, bar, hk * DK + a * 64, tok);
+        }
+      };
+      load_kq(0);
       load_v(0);
       for (int c = 1; c < chunks; ++c) {
         // Chunk c - 3 is done with the stage: its products are complete (the next
