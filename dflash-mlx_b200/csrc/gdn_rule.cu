@@ -249,8 +249,9 @@ int launch_recurrent(const RuleParams& p, cudaStream_t stream) {
 // of a 128 x 128 head.  Most of it is the state's threads at work: 2600 cycles on
 // the last chunk's y, 800 on R, 1100 on Delta, 2100 on beta V, 1800 on the state;
 // they wait 2300 for products.  The preparing warps need 9600 for T and P of the
-// next chunk, beside it.  8192 steps of 48 heads, cut in three, 597 us; 16091
-// steps in 8 prompts 565 us, of which the longest's 79 chunks alone are 430.
+// next chunk, beside it.  A CTA's start and end take 9 us more.  8192 steps of 48
+// heads, cut in three, 557 us; 16091 steps in 8 prompts 558 us, of which the
+// longest's 79 chunks alone are 430.
 //
 // Warps: 0-3 prepare T and P of the next chunk (K K^T and Q K^T from one
 // product, inverse by blocks of 16, 32 and 64 in fp32) and put zeros over rows
@@ -1232,9 +1233,9 @@ __global__ void __launch_bounds__(C_THREADS, 1)
 // their mean is taken).  In units of a chunk's time (5.4 us): whole, L; in n
 // pieces, two launches of L / n chunks that are 1.25 long with every SM at work,
 // 6 for starting two launches more and 0.6 for a step of the chain.  Measured,
-// us whole and cut: 48 heads 695 / 581 at 8192 steps, 355 / 332 at 4096 (3 pieces;
-// 183 at 2048, left whole), 16 heads 690 / 321 at 8192 and 182 / 119 at 2048 (6), 4
-// heads 686 / 171 and 181 / 93 (16), 8 heads of 64 x 64 616 / 165 and 160 / 71 (10).
+// us whole and cut: 48 heads 685 / 559 at 8192 steps, 349 / 301 at 4096 (3 pieces;
+// 178 at 2048, left whole), 16 heads 681 / 300 at 8192 and 177 / 105 at 2048 (6), 4
+// heads 676 / 158 and 176 / 86 (16), 8 heads of 64 x 64 621 / 167 and 162 / 72 (10).
 inline int pieces(long long heads, int tiles, long long chunks, int sms) {
   int best = 1;
   double least = 0.95 * double(chunks);

@@ -296,13 +296,16 @@ def _chunked_from(tiles: int, dv: int, dk: int) -> int:
     """Mean steps of a sequence from which 64 steps at a time are faster than
     one after the other.  A chunk takes much the same time for any size of the
     state (up to 128 rows) and has an SM to itself, so small states need more
-    steps once there are more of them than SMs.  Measured, us one after the other and 64 at a time,
-    24 and 64 steps: one sequence of 48 heads of 128 x 128 18.4 / 17.8 and 43 /
-    18, 40 of those 274 / 240 and 671 / 239; 80 heads of 64 x 64 12.3 / 12.7 and
-    27.5 / 12.6, 320 of those 17 / 36 and 39.6 / 35.0; 640 heads of 128 x 64 (Dv x
-    Dk) 41 / 64 and 100 / 65, equal at 40 steps."""
+    steps once there are more of them than SMs.  Measured, us one after the
+    other and 64 at a time, 16, 24 and 64 steps: one sequence of 48 heads of 128 x
+    128 13 / 14.6, 18 / 14.7 and 44 / 14, 40 of those 194 / 194, 275 / 193 and
+    671 / 188; 80 heads of 64 x 64 9 / 12.8, 12.3 / 12.7 and 27.6 / 12.5, 320 of those
+    12 / 35, 17 / 35 and 39.6 / 35.0; 320 heads of 64 x 128 (Dv x Dk) 18 / 42, 26 / 41
+    and 62 / 40, equal at 40 steps."""
     size = dk * min(dv, 128)
-    if tiles <= 148 or size >= 128 * 128:
+    if size >= 128 * 128:
+        return 20
+    if tiles <= 148:
         return 24
     return 40 if size >= 128 * 64 else 64
 
