@@ -972,6 +972,10 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       }
       tmem_st_wait();
       tc_fence_before();
+      // The last turn's y was written and read in V's buffer; the copy that fills
+      // it next is issued once this arrival is there, and a barrier alone does
+      // not order these accesses before a TMA write.
+      fence_proxy_async_shared();
       mbar_arrive(&bars.s_ready);
       if (c > 0) {
         // Y = c Q S^T + P Delta of the last chunk, while this one's K S^T runs.

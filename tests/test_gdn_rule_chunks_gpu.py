@@ -1,0 +1,62 @@
+"""Every block of 64 steps of ``gated_delta_rule`` by itself: y and states of
+whole prompts against the recurrence in float64, where a wrong chunk or piece
+must not be averaged away by the others.
+
+Bounds, in the 2-norm.  y of a block: one rounding to bf16 moves every value by at
+most 2^-8 of itself, so the block by 2^-8 of its norm; the products before it hold
+16 bits or more of the state, of Delta and of the decayed Q K^T, 2^-16 of what a
+value is summed from, and with |q| = 1 / sqrt(Dk) spread over the columns that is
+less than 16 times the value's own size: 2^-12 together.  A step of no sequence
+or a masked one is an exact 0.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import gdn as ogdn
+from tests.test_gdn_rule_gpu import _dev, _inputs
+
+Y_BOUND = 2.0 ** -8 + 2.0 ** -12
+BLOCK = 64
+
+
+def _bad_blocks(y, ry, ranges=None):
+    """``(sequence, first step, error / norm)`` of the blocks whose y is off by more
+    than the bound; ``ranges``: token ranges of packed sequences."""
+    if ranges is None:
+        rows = [(b, 0, ry.shape[1]) for b in range(ry.shape[0])]
+    else:
+        rows = [(0, a, e) for a, e in ranges]
+    bad = []
+    for n, (b, a, e) in enumerate(rows):
+        for t in range(a, e, BLOCK):
+            for h in range(ry.shape[2]):
+                want = ry[b, t:min(e, t + BLOCK), h]
+                err = np.linalg.norm(y[b, t:min(e, t + BLOCK), h] - want)
+                if not err <= Y_BOUND * np.linalg.norm(want):
+                    bad.append((n, t - a, h, err / max(np.linalg.norm(want), 1e-300)))
+    return bad
+
+
+def _host(x):
+    return x.float().cpu().numpy().astype(np.float64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,hk,hv,dk,dv", [(1100, 50, 150, 128, 128), (1090, 80, 160, 64, 128)])
+def test_refilled_buffers_on_a_full_card(pkg, dev, t, hk, hv, dk, dv):
+    """More heads than SMs and many chunks each: the shared-memory tile through
+    which a chunk's y is turned is the one that later V tiles are copied to.  All
+    y right in every call, and the same bits."""
+    arrays = _inputs(61, 1, t, hk, hv, dk, dv, slow=True)
+    ins = _dev(arrays, dev)
+    y, s = pkg.gated_delta_rule(*ins)
+    for _ in range(5):
+        y2, s2 = pkg.gated_delta_rule(*ins)
+        assert torch.equal(y, y2) and torch.equal(s, s2)
+    ry, rs = ogdn.gated_delta_rule(*arrays)
+    assert _bad_blocks(_host(y), ry) == []
+    assert np.linalg.norm(_host(s) - rs) <= 1e-5 * np.linalg.norm(rs)
