@@ -13,7 +13,7 @@ Mirrors ``dflash_mlx/kernels.py``:
   untouched.  Same shapes: tape fp32 ``[B, T, Hv, Dv]``, k ``[B, T, Hk, Dk]``
   (bf16 or fp32), g ``[B, T, Hv]`` or ``[B, T, Hv, Dk]``, state fp32
   ``[B, Hv, Dv, Dk]``, optional bool mask ``[B, T]``.
-* ``tape_replay_(state, tape, k, g, steps)`` -- the in-place form the
+* ``tape_replay_(state, tape, k, g, steps, mask)`` -- the in-place form the
   rollback uses on B200: replays the first ``steps[b]`` steps of each
   sequence and does not touch sequences with nothing to replay.
 * ``gated_delta_rule(q, k, v, g, beta, state, ...)`` -- the same recurrence
@@ -107,12 +107,13 @@ def tape_replay_kernel(tape: torch.Tensor, k: torch.Tensor, g: torch.Tensor, sta
 
 
 def tape_replay_(state: torch.Tensor, tape: torch.Tensor, k: torch.Tensor, g: torch.Tensor,
-                 steps: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """In-place replay of the first ``steps[b]`` steps of each sequence."""
+                 steps: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """In-place replay of the first ``steps[b]`` steps of each sequence, without
+    those whose ``mask [B, T]`` is False."""
     if not state.is_contiguous():
         raise ValueError("in-place replay needs a contiguous state")
-    dims = _check(tape, k, g, state, steps=steps)
-    return _launch(tape, k, g, state, state, steps, None, dims)
+    dims = _check(tape, k, g, state, steps=steps, mask=mask)
+    return _launch(tape, k, g, state, state, steps, mask, dims)
 
 
 def gated_delta_kernel_with_tape(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor,

@@ -5,7 +5,7 @@ and the restore policy of ``dflash_mlx/engine/target_qwen_gdn.py:1025-1055``:
 
 * ``arm_rollback`` snapshots ``[conv_state, ssm_state]`` (``:96-103``);
 * ``record_tape`` keeps the verify forward's innovation tape, k, g and qkv
-  (``:110-121``);
+  (``:110-121``), and its mask;
 * ``advance(q, k, v, g, beta)`` runs a layer's recurrence on the cached state:
   with the tape when armed, over a whole prompt or a single token otherwise
   (``engine/target_qwen_gdn.py:610-642``);
@@ -54,6 +54,7 @@ class RecurrentRollbackCache:
         self._tape_k = None
         self._tape_g = None
         self._tape_qkv = None
+        self._tape_mask = None
         self._snapshot = None
 
     def checkpoint(self) -> None:
@@ -66,17 +67,20 @@ class RecurrentRollbackCache:
         self.checkpoint()
 
     def record_tape(self, *, tape: torch.Tensor, k: torch.Tensor, g: torch.Tensor,
-                    qkv: Optional[torch.Tensor] = None) -> None:
+                    qkv: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None) -> None:
         self._tape = tape.contiguous()
         self._tape_k = k.contiguous()
         self._tape_g = g.contiguous()
         self._tape_qkv = None if qkv is None else qkv.contiguous()
+        self._tape_mask = None if mask is None else mask.contiguous()
 
     def advance(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor, *,
                 qkv: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``y`` of a GDN layer's tokens; ``cache[1]`` becomes the state after them
         (an empty cache starts from zeros).  Armed, the verify forward runs and
-        its tape is recorded (T <= 64); otherwise ``gated_delta_rule``."""
+        its tape is recorded (T <= 64); otherwise ``gated_delta_rule``.  A step
+        whose ``mask [B, T]`` is False leaves the state, here and in the replay
+        of ``rollback``, where it counts as a step of the block."""
         state = self.cache[1]
         if state is None:
             state = torch.zeros((k.shape[0], v.shape[2], v.shape[3], k.shape[3]), dtype=torch.float32,
@@ -85,7 +89,7 @@ class RecurrentRollbackCache:
                 self._snapshot[1] = state
         if self._armed:
             y, new, tape = gated_delta_kernel_with_tape(q, k, v, g, beta, state, mask)
-            self.record_tape(tape=tape, k=k, g=g, qkv=qkv)
+            self.record_tape(tape=tape, k=k, g=g, qkv=qkv, mask=mask)
         else:
             y, new = gated_delta_rule(q, k, v, g, beta, state, mask=mask)
         self.cache[1] = new
@@ -129,7 +133,7 @@ class RecurrentRollbackCache:
             target = state_now if state_now is not None and state_now.shape == snap_state.shape \
                 else torch.empty_like(snap_state)
             target.copy_(snap_state)
-            tape_replay_(target, self._tape, self._tape_k, self._tape_g, steps)
+            tape_replay_(target, self._tape, self._tape_k, self._tape_g, steps, self._tape_mask)
             self.cache[1] = target
             self.cache[0] = self._rebuild_conv_state(steps)
         self.clear_transients()
