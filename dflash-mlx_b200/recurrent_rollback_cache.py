@@ -80,7 +80,11 @@ class RecurrentRollbackCache:
         (an empty cache starts from zeros).  Armed, the verify forward runs and
         its tape is recorded (T <= 64); otherwise ``gated_delta_rule``.  A step
         whose ``mask [B, T]`` is False leaves the state, here and in the replay
-        of ``rollback``, where it counts as a step of the block."""
+        of ``rollback``, where it counts as a step of the block.  The tape holds
+        one block: a second one before ``rollback`` (or a new arming) is refused."""
+        if self._armed and self._tape is not None:
+            raise RuntimeError("the cache holds the tape of a block that was neither rolled back nor accepted: "
+                               "call rollback, restore_after_acceptance or arm_rollback first")
         state = self.cache[1]
         if state is None:
             state = torch.zeros((k.shape[0], v.shape[2], v.shape[3], k.shape[3]), dtype=torch.float32,
