@@ -86,6 +86,28 @@ def same_device(dev: torch.device, **tensors) -> None:
         raise ValueError(f"{name} is on {t.device}, not on {dev}")
 
 
+def overlap(a: torch.Tensor, *others) -> bool:
+    """Whether the bytes from ``a``'s first to its last element meet those of
+    another tensor (None: left out).  Parts of one allocation that lie apart do not."""
+    lo, hi = _span(a)
+    for x in others:
+        if x is not None:
+            first, end = _span(x)
+            if first < hi and lo < end:
+                return True
+    return False
+
+
+def _span(x: torch.Tensor):
+    lo = x.data_ptr()
+    if x.is_contiguous():
+        return lo, lo + x.numel() * x.element_size()
+    if x.numel() == 0:
+        return lo, lo
+    last = sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
+    return lo, lo + (last + 1) * x.element_size()
+
+
 def mask_bytes(mask: torch.Tensor, name: str) -> torch.Tensor:
     """A bool or uint8 mask as contiguous uint8 (bool storage is read as it is)."""
     if mask.dtype == torch.bool:

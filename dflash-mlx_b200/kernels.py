@@ -37,7 +37,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._runtime import mask_bytes, on_device, require_cuda, same_device, stream_ptr
+from ._runtime import mask_bytes, on_device, overlap, require_cuda, same_device, stream_ptr
 
 
 def _check(tape, k, g, state, steps=None, mask=None):
@@ -196,7 +196,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
       of 0 and 1 included) and starts from ``state[n]``, ``[N, Hv, Dv, Dk]``.
 
     ``out`` receives y (rows that belong to no sequence are left as they were;
-    a new y has zeros there) and shares no storage with q, k and v.
+    a new y has zeros there) and shares no memory with q, k and v.
     ``out_state`` receives the new state and may be ``state`` itself; without it
     ``state`` is left untouched.  Nothing is read back to the host; the call can
     be captured into a CUDA graph.  A NaN or an infinity in a step that counts
@@ -253,7 +253,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     elif (out.dtype != bf16 or out.shape != (b, t_steps, hv, dv) or not out.is_contiguous()
           or out.data_ptr() % 16 != 0):
         raise ValueError(f"out must be contiguous, 16-byte aligned bf16 {(b, t_steps, hv, dv)}")
-    elif any(out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr() for x in (q, k, v)):
+    elif overlap(out, q, k, v):
         raise ValueError("out must not share memory with q, k or v")
     if out_state is None:
         out_state = torch.empty(shape, dtype=f32, device=dev)
@@ -264,8 +264,8 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
             raise ValueError(f"out_state must be contiguous, 16-byte aligned fp32 {shape}")
         if out_state.data_ptr() == state.data_ptr() and state.is_contiguous():
             pass   # in place
-        elif out_state.untyped_storage().data_ptr() == state.untyped_storage().data_ptr():
-            state = state.clone(memory_format=torch.contiguous_format)   # may overlap in part
+        elif overlap(out_state, state):
+            state = state.clone(memory_format=torch.contiguous_format)   # in part
         else:
             state = _aligned(state)
     q, ldq = _token_rows(q, b, t_steps, hk, dk)

@@ -60,3 +60,24 @@ def test_refilled_buffers_on_a_full_card(pkg, dev, t, hk, hv, dk, dv):
     ry, rs = ogdn.gated_delta_rule(*arrays)
     assert _bad_blocks(_host(y), ry) == []
     assert np.linalg.norm(_host(s) - rs) <= 1e-5 * np.linalg.norm(rs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [1, 100])
+def test_one_arena_for_inputs_and_outputs(pkg, dev, t):
+    """``out`` and ``out_state`` beside q, k, v and the state in one allocation."""
+    arrays = _inputs(62, 2, t, 2, 4, 64, 64)
+    ins = _dev(arrays, dev)
+    want = pkg.gated_delta_rule(*ins)
+    sizes = [ins[0].nbytes, ins[1].nbytes, ins[2].nbytes, ins[2].nbytes, ins[5].nbytes, ins[5].nbytes]
+    arena = torch.zeros(sum(sizes), dtype=torch.uint8, device=dev)
+    q, k, v, out, state, out_state = (
+        part.view(x.dtype).view_as(x)
+        for part, x in zip(arena.split(sizes), (*ins[:3], ins[2], ins[5], ins[5])))
+    for dst, src in zip((q, k, v, state), (*ins[:3], ins[5])):
+        dst.copy_(src)
+    y, s = pkg.gated_delta_rule(q, k, v, *ins[3:5], state, out=out, out_state=out_state)
+    assert y is out and s is out_state
+    assert torch.equal(y, want[0]) and torch.equal(s, want[1]) and torch.equal(state, ins[5])
+    with pytest.raises(ValueError, match="share"):
+        pkg.gated_delta_rule(q, k, v, *ins[3:5], state, out=v)
