@@ -196,9 +196,10 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
       of 0 and 1 included) and starts from ``state[n]``, ``[N, Hv, Dv, Dk]``.
 
     ``out`` receives y (rows that belong to no sequence are left as they were;
-    a new y has zeros there) and shares no memory with q, k and v.
-    ``out_state`` receives the new state and may be ``state`` itself; without it
-    ``state`` is left untouched.  Nothing is read back to the host; the call can
+    a new y has zeros there) and shares no memory with the inputs or
+    ``out_state``.  ``out_state`` receives the new state and may be ``state``
+    itself, whole or in part, but meets no other input; without it ``state`` is
+    left untouched.  Nothing is read back to the host; the call can
     be captured into a CUDA graph.  A NaN or an infinity in a step that counts
     reaches what follows it, as in the recurrence, and may reach the y of up to
     63 steps before it (steps are taken 64 at a time).
@@ -253,8 +254,8 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     elif (out.dtype != bf16 or out.shape != (b, t_steps, hv, dv) or not out.is_contiguous()
           or out.data_ptr() % 16 != 0):
         raise ValueError(f"out must be contiguous, 16-byte aligned bf16 {(b, t_steps, hv, dv)}")
-    elif overlap(out, q, k, v):
-        raise ValueError("out must not share memory with q, k or v")
+    elif overlap(out, q, k, v, g, beta, mask, cu_seqlens, state, out_state):
+        raise ValueError("out must not share memory with an input or out_state")
     if out_state is None:
         out_state = torch.empty(shape, dtype=f32, device=dev)
         state = _aligned(state)
@@ -262,6 +263,8 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
         if (out_state.dtype != f32 or out_state.shape != shape or not out_state.is_contiguous()
                 or out_state.data_ptr() % 16 != 0):
             raise ValueError(f"out_state must be contiguous, 16-byte aligned fp32 {shape}")
+        if overlap(out_state, q, k, v, g, beta, mask, cu_seqlens):
+            raise ValueError("out_state must not share memory with an input other than state")
         if out_state.data_ptr() == state.data_ptr() and state.is_contiguous():
             pass   # in place
         elif overlap(out_state, state):

@@ -81,3 +81,43 @@ def test_one_arena_for_inputs_and_outputs(pkg, dev, t):
     assert torch.equal(y, want[0]) and torch.equal(s, want[1]) and torch.equal(state, ins[5])
     with pytest.raises(ValueError, match="share"):
         pkg.gated_delta_rule(q, k, v, *ins[3:5], state, out=v)
+
+
+@pytest.mark.gpu
+def test_outputs_over_inputs_are_refused(pkg, dev):
+    """Some threads would still read what others have written over."""
+    t, hk, hv, d = 64, 1, 2, 64
+    ins = list(_dev(_inputs(63, 1, t, hk, hv, d, d), dev))
+    q, k, v, g, beta, s0 = ins
+    mask = torch.ones((1, t), dtype=torch.bool, device=dev)
+    cu = torch.tensor([0, t], dtype=torch.int32, device=dev)
+
+    def arena(*tensors):
+        """The tensors again, all from the first byte of one allocation on."""
+        buf = torch.zeros(max(x.nbytes for x in tensors), dtype=torch.uint8, device=dev)
+        return [buf[:x.nbytes].view(x.dtype).view(x.shape) for x in tensors]
+
+    for i in range(5):
+        mine, out = arena(ins[i], v)
+        with pytest.raises(ValueError, match="share"):
+            pkg.gated_delta_rule(*ins[:i], mine, *ins[i + 1:], out=out)
+        mine, held = arena(ins[i], s0)
+        with pytest.raises(ValueError, match="share"):
+            pkg.gated_delta_rule(*ins[:i], mine, *ins[i + 1:], out_state=held)
+    for kw in (dict(mask=mask), dict(cu_seqlens=cu)):
+        (name, x), = kw.items()
+        mine, out = arena(x, v)
+        with pytest.raises(ValueError, match="share"):
+            pkg.gated_delta_rule(*ins, out=out, **{name: mine})
+        mine, held = arena(x, s0)
+        with pytest.raises(ValueError, match="share"):
+            pkg.gated_delta_rule(*ins, out_state=held, **{name: mine})
+    held, out = arena(s0, v)
+    with pytest.raises(ValueError, match="share"):
+        pkg.gated_delta_rule(*ins[:5], held, out=out)
+    with pytest.raises(ValueError, match="share"):
+        pkg.gated_delta_rule(*ins, out=out, out_state=held)
+    # the state's own memory stays open, whole or in part
+    want = pkg.gated_delta_rule(*ins)
+    y, s = pkg.gated_delta_rule(*ins[:5], s0, out_state=s0)
+    assert torch.equal(y, want[0]) and torch.equal(s, want[1])
