@@ -237,21 +237,28 @@ int launch_recurrent(const RuleParams& p, cudaStream_t stream) {
 // products from TMEM, and only K, Q, T and P are read from shared memory, K
 // both as it is and transposed from the same tile.
 //
-// fp32 in bf16 products: K and Q are bf16 already.  The state and the update
-// Delta K go in as three bf16 parts (24 bits), so what is carried from chunk to
-// chunk keeps 32-bit accuracy, and so does R, whose product with T - I is added
-// to R in fp32; T - I has two (16 bits: it is a correction).  In y, which ends
-// in 8 bits, the state, P and Delta have two parts (one each of P and Delta would
-// add 2.2e-3 of y to the 1.7e-3 of its last rounding).
+// fp32 in bf16 products: K and Q are bf16 already.  The state, R, T - I and the
+// update Delta K go in as three bf16 parts (24 bits), and T is joined from 32-bit
+// blocks, so what is carried from chunk to chunk keeps 32-bit accuracy (T - I in
+// two parts would do only for keys at right angles: it is as large as R's own
+// share where they are alike).  The tensor cores cut their sums to 24 bits, so
+// the small parts' products are added up before the large ones.  State error
+// (2-norm) of 520 steps of slow decay, keys of unit length, against 64 bits: 1.3e-7
+// at a mean cosine of 0 between keys, 1.8e-7 at 0.5, 2.7e-7 at 0.95, 4.4e-7 there
+// with beta near 1; cut in pieces 3e-7 to 8e-7; a recurrence in fp32 2e-7.  In y,
+// which ends in 8 bits, the state, P and Delta have two parts (one each of P and
+// Delta would add 2.2e-3 of y to the 1.7e-3 of its last rounding).
 //
-// Bound by the chain through a chunk, not by a rate: S K^T, R, R T^T, Delta, Delta
-// K and the new state wait for one another, 5.4 us (about 10700 cycles) a chunk
-// of a 128 x 128 head.  Most of it is the state's threads at work: 2600 cycles on
-// the last chunk's y, 800 on R, 1100 on Delta, 2100 on beta V, 1800 on the state;
-// they wait 2300 for products.  The preparing warps need 9600 for T and P of the
-// next chunk, beside it.  A CTA's start and end take 9 us more.  8192 steps of 48
-// heads, cut in three, 557 us; 16091 steps in 8 prompts 558 us, of which the
-// longest's 79 chunks alone are 430.
+// Bound by the work on a chunk, not by a rate.  The preparing warps take 11000
+// cycles for T and P of the next chunk (decays 3700, blocks of 16 inverted 1700,
+// joined 6000, a third of it for 32-bit factors), and beside them the chain through a
+// chunk takes 9700: S K^T, R, R T^T, Delta, Delta K and the new state wait for one
+// another.  Most of that is the state's threads at work: 3000 cycles on the last
+// chunk's y, 700 on R, 1000 on Delta, 2500 on beta V, 1800 on the state; they wait
+// 1700 for products, and 1100 to 1600 for T.  A chunk of a 128 x 128 head takes 6.1 us
+// (11200 cycles) with an SM of each pair idle, 6.4 to 7.1 with every SM at work (two
+// share their instruction fetches).  A CTA's start and end take 9 us more.  8192 steps
+// of 48 heads, cut in three, 612 us; 15886 steps in 8 prompts 596 us.
 //
 // Warps: 0-3 prepare T and P of the next chunk (K K^T and Q K^T from one
 // product, inverse by blocks of 16, 32 and 64 in fp32) and put zeros over rows
@@ -278,10 +285,10 @@ struct CCfg {
   static constexpr int KQ_BYTES = (DK / 64) * ATOM;
   static constexpr int V_BYTES = CH * 256;               // 64 rows x 128 columns
   static constexpr int V_OFF = C_STAGES * KQ_BYTES;      // of two chunks
-  static constexpr int TP_BYTES = 4 * PART;              // T's two parts and P's
+  static constexpr int TP_BYTES = 5 * PART;              // T's three parts and P's two
   static constexpr int TP_OFF = V_OFF + 2 * V_BYTES;
-  static constexpr int A_OFF = TP_OFF + 2 * TP_BYTES;    // A's two parts, A in fp32, a place for stores to nowhere
-  static constexpr int SMALL_OFF = A_OFF + 2 * PART + A32_FLOATS * 4 + 1024;
+  static constexpr int A_OFF = TP_OFF + 2 * TP_BYTES;    // A in fp32, a place for stores to nowhere
+  static constexpr int SMALL_OFF = A_OFF + A32_FLOATS * 4 + 1024;
   static constexpr int SMALL_BYTES = (C_STAGES * 2 + 2 * 3) * CH * 4;
   static constexpr int SMEM_BYTES = SMALL_OFF + SMALL_BYTES + 1024;
   static_assert(SMEM_BYTES + 1024 <= 227 * 1024, "with the barriers, what a CTA can have");
@@ -385,13 +392,21 @@ struct ChunkBars {
 
 __device__ __forceinline__ float4 at4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
+__device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; i += 4) {
+    const float4 v = at4(p + i);
+    x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+  }
+}
+
 // Byte offset of element (r, c) in a part of a 64 x 64 matrix.
 __device__ __forceinline__ int part_at(int r, int c) { return r * 128 + (((c / 8) ^ (r & 7)) * 16) + (c % 8) * 2; }
 
 // Inverse of a unit lower triangular block of 16 rows (strictly lower part
-// used) by forward substitution, column c per lane, 16 lanes of one warp a
-// block; then row c of it in parts to row 16 b + c, columns 16 b .. of t.
-__device__ __forceinline__ void invert_block16(float* blk, uint8_t* t, int b, int c) {
+// used) by forward substitution, in place, column c per lane, 16 lanes of one
+// warp a block.
+__device__ __forceinline__ void invert_block16(float* blk, int c) {
   float x[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
@@ -409,113 +424,144 @@ __device__ __forceinline__ void invert_block16(float* blk, uint8_t* t, int b, in
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < 16; ++i) blk[i * DIAG_LD + c] = x[i];
-  __syncwarp();
+}
+
+// Row 16 b + c of T - I in its diagonal block, in parts.
+__device__ __forceinline__ void store_diag_row(const float* diag, uint8_t* t, int b, int c) {
+  float x[16];
+  load16(diag + b * DIAG_BLK + c * DIAG_LD, x);
 #pragma unroll
-  for (int i = 0; i < 16; i += 4) {
-    const float4 y = at4(blk + c * DIAG_LD + i);
-    x[i] = y.x; x[i + 1] = y.y; x[i + 2] = y.z; x[i + 3] = y.w;
-  }
+  for (int i = 0; i < 16; ++i) x[i] = i == c ? 0.f : x[i];
   uint8_t* at0 = t + part_at(16 * b + c, 16 * b);
   uint8_t* at1 = t + part_at(16 * b + c, 16 * b + 8);
-#pragma unroll
-  for (int part = 0; part < 2; ++part) {
+#pragma unroll 1
+  for (int part = 0; part < 3; ++part) {
     *reinterpret_cast<uint4*>(at0 + part * PART) = take_part8(x);
     *reinterpret_cast<uint4*>(at1 + part * PART) = take_part8(x + 8);
   }
 }
 
-// Four 8 x 8 blocks of a part: rows r .. r + 15, columns c .. c + 15, in the order
-// of a left operand (as they are) or of two right operands' k x n (transposed).
-template <bool TRANS>
-__device__ __forceinline__ void load_blocks(uint32_t part, int r, int c, int lane, uint32_t (&f)[4]) {
-  const uint32_t at = part + part_at(r + (lane & 15), c + (lane >> 4) * 8);
-  if constexpr (TRANS)
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3]) : "r"(at) : "memory");
-  else
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3]) : "r"(at) : "memory");
+// x as two numbers of 11 bits, what a factor of a tf32 product can hold: rounded,
+// and what that leaves, cut (together they are off by 2^-23 of x at most).  A NaN
+// stays one in the second.
+__device__ __forceinline__ void two_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
 
-__device__ __forceinline__ void mma_m16n8k16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+__device__ __forceinline__ void mma_m16n8k8(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 
-// acc (16 rows, NP pairs of 8 columns) += A B with B's rows k .. k + 15, columns
-// c .. of a matrix in two parts: first x first, first x second, second x first,
-// each over the tiles in turn, so that neighbours do not wait for one another.
-template <int NP>
-__device__ __forceinline__ void mma_parts(float (&acc)[2 * NP][4], const uint32_t (&a)[2][4], uint32_t b, int k,
-                                          int c, int lane) {
-  uint32_t f[2][NP][4];
+// acc + low (16 rows, NT tiles of 8 columns) += A B over 8 k's.  x: A's rows lane / 4
+// and + 8, k's 2 (lane % 4) and + 1 (row by row); b: this lane's column lane / 4 of row 2
+// (lane % 4) of B's first tile.  The instruction's k's 0-3 and 4-7 stand for the even
+// and the odd ones, so that A's come as pairs, an accumulator's as they lie.  First x
+// first goes to acc, first x second and second x first, which are small, to low; the
+// part left out is 2^-22 of a factor.  Each over the tiles in turn, so that neighbours
+// do not wait for one another.
+template <int NT, int LD>
+__device__ __forceinline__ void mma_tf32(float (*acc)[4], float (*low)[4], const float (&x)[4], const float* b) {
+  uint32_t a[2][4], f[2][NT][2];
 #pragma unroll
-  for (int part = 0; part < 2; ++part)
+  for (int i = 0; i < 4; ++i) two_tf32(x[i], a[0][(i & 1) * 2 + i / 2], a[1][(i & 1) * 2 + i / 2]);
 #pragma unroll
-    for (int i = 0; i < NP; ++i) load_blocks<true>(b + part * PART, k, c + 16 * i, lane, f[part][i]);
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) two_tf32(b[e * LD + 8 * i], f[0][i][e], f[1][i][e]);
 #pragma unroll
   for (int m = 0; m < 3; ++m)
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      mma_m16n8k16(acc[2 * i], a[m == 2], f[m == 1][i][0], f[m == 1][i][1]);
-      mma_m16n8k16(acc[2 * i + 1], a[m == 2], f[m == 1][i][2], f[m == 1][i][3]);
-    }
+    for (int i = 0; i < NT; ++i) mma_m16n8k8(m == 1 ? acc[i] : low[i], a[m == 2], f[m == 0][i]);
 }
 
-// Rows R + r0 .. + 15, columns C + c0 .. + 15 of T = -(T22 A21) T11 for blocks of N
-// rows, T22 at (R, R), A21 at (R, C), T11 at (C, C): the first product's
-// accumulators are the second one's left operand in place, so nothing passes
-// through shared memory between them.
-template <int N>
-__device__ __forceinline__ void join_block(uint8_t* t, uint32_t t_at, uint32_t a_at, int R, int C, int r0, int c0,
-                                           int lane) {
-  float m[N / 8][4];
+template <int NT>
+__device__ __forceinline__ void add_low(float (&acc)[NT][4], const float (&low)[NT][4]) {
 #pragma unroll
-  for (int i = 0; i < N / 8; ++i)
+  for (int i = 0; i < NT; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) m[i][e] = 0.f;
-#pragma unroll
-  for (int k = 0; k < N / 16; ++k) {
-    uint32_t a[2][4];
-    load_blocks<false>(t_at, R + r0, R + 16 * k, lane, a[0]);
-    load_blocks<false>(t_at + PART, R + r0, R + 16 * k, lane, a[1]);
-    mma_parts<N / 16>(m, a, a_at, R + 16 * k, C, lane);
-  }
-  float out[2][4];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) out[i][e] = 0.f;
-#pragma unroll
-  for (int k = 0; k < N / 16; ++k) {
-    uint32_t a[2][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float x = -m[2 * k + i / 2][2 * (i & 1)], y = -m[2 * k + i / 2][2 * (i & 1) + 1];
-      a[0][i] = take_part(x, y);
-      a[1][i] = take_part(x, y);
-    }
-    mma_parts<1>(out, a, t_at, C + 16 * k, C + c0, lane);
-  }
-#pragma unroll
-  for (int part = 0; part < 2; ++part)
+    for (int e = 0; e < 4; ++e) acc[i][e] += low[i][e];
+}
+
+__device__ __forceinline__ void load_rows(const float* a, float (&x)[4]) {   // rows of DIAG_LD
+  const float2 u = *reinterpret_cast<const float2*>(a), v = *reinterpret_cast<const float2*>(a + 8 * DIAG_LD);
+  x[0] = u.x; x[1] = u.y; x[2] = v.x; x[3] = v.y;
+}
+
+// Rows r .. r + 15, columns c .. c + 15 of T, from accumulators, in parts.
+__device__ __forceinline__ void store_join(uint8_t* t, float (&out)[2][4], int r, int c, int lane) {
+#pragma unroll 1
+  for (int part = 0; part < 3; ++part, t += PART)
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int e = 0; e < 4; e += 2)
-        *reinterpret_cast<uint32_t*>(t + part * PART +
-                                     part_at(R + r0 + lane / 4 + 4 * e, C + c0 + 8 * i + 2 * (lane % 4))) =
+        *reinterpret_cast<uint32_t*>(t + part_at(r + lane / 4 + 4 * e, c + 8 * i + 2 * (lane % 4))) =
             take_part(out[i][e], out[i][e + 1]);
 }
 
-__device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
-#pragma unroll
-  for (int i = 0; i < 16; i += 4) {
-    const float4 v = at4(p + i);
-    x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+// T21 = -(T22 A21) T11 for blocks of 16 rows, pair w (rows 32 w + 16 ..): A21 in
+// block 4 + w, which T21 goes over, T22 and T11 in blocks 2 w + 1 and 2 w.  The first
+// product's accumulators are the second one's left operand in place.
+__device__ __forceinline__ void join16(float* diag, uint8_t* t, int w, int lane) {
+  const int at_a = (lane / 4) * DIAG_LD + 2 * (lane % 4), at_b = 2 * (lane % 4) * DIAG_LD + lane / 4;
+  float* off = diag + (4 + w) * DIAG_BLK;
+  const float* t22 = diag + (2 * w + 1) * DIAG_BLK + at_a;
+  const float* t11 = diag + 2 * w * DIAG_BLK + at_b;
+  float m[2][4] = {}, out[2][4] = {}, ml[2][4] = {}, ol[2][4] = {};
+#pragma unroll 1
+  for (int k = 0; k < 16; k += 8) {
+    float x[4];
+    load_rows(t22 + k, x);
+    mma_tf32<2, DIAG_LD>(m, ml, x, off + at_b + k * DIAG_LD);
   }
+  add_low(m, ml);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float x[4] = {-m[k][0], -m[k][1], -m[k][2], -m[k][3]};
+    mma_tf32<2, DIAG_LD>(out, ol, x, t11 + 8 * k * DIAG_LD);
+  }
+  add_low(out, ol);
+  __syncwarp();   // A21 has been read
+  float* to = off + at_a;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; e += 2)
+      *reinterpret_cast<float2*>(to + 4 * e * DIAG_LD + 8 * i) = make_float2(out[i][e], out[i][e + 1]);
+  store_join(t, out, 32 * w + 16, 32 * w, lane);
+}
+
+// The same for blocks of 32: rows 32 + r0 .., columns c0 .. of T by a warp, A21 in
+// off32, T22 and T11 each in two diagonal blocks and the one left of the lower.  What
+// is 0 above the diagonals is passed over: the second 16 k's of the first product
+// for r0 = 0, the first 16 of the second for c0 = 16.
+__device__ __forceinline__ void join32(const float* diag, const float* off32, uint8_t* t, int r0, int c0, int lane) {
+  const int at_a = (lane / 4) * DIAG_LD + 2 * (lane % 4), at_b = 2 * (lane % 4) * DIAG_LD + lane / 4;
+  const float* a21 = off32 + 2 * (lane % 4) * OFF_LD + lane / 4;
+  float m[4][4] = {}, out[2][4] = {}, ml[4][4] = {}, ol[2][4] = {};
+#pragma unroll 1
+  for (int k = 0; k < 16 + r0; k += 8) {
+    // rows 32 + r0 ..: block 2 for r0 = 0, else block 5 and then 3
+    const float* t22 = diag + (r0 == 0 ? 2 : (k < 16 ? 5 : 3)) * DIAG_BLK + at_a + (k & 8);
+    float x[4];
+    load_rows(t22, x);
+    mma_tf32<4, OFF_LD>(m, ml, x, a21 + k * OFF_LD);
+  }
+  add_low(m, ml);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (8 * k < c0) continue;
+    // columns c0 ..: blocks 0 and 4 for c0 = 0, else block 1
+    const float* t11 = diag + (c0 != 0 ? 1 : (k < 2 ? 0 : 4)) * DIAG_BLK + at_b + (k & 1) * 8 * DIAG_LD;
+    const float x[4] = {-m[k][0], -m[k][1], -m[k][2], -m[k][3]};
+    mma_tf32<2, DIAG_LD>(out, ol, x, t11);
+  }
+  add_low(out, ol);
+  store_join(t, out, 32 + r0, c0, lane);
 }
 
 // A long sequence cut in n pieces, where there are too few heads to fill the
@@ -763,8 +809,7 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       if (c >= 2) wait(&bars.tp_freed[ts], (c / 2) - 1);
       const float* gs = g_of(s);
       uint8_t* tp = smem + C::TP_OFF + ts * C::TP_BYTES;
-      uint8_t* ap = smem + C::A_OFF;
-      float* diag = reinterpret_cast<float*>(ap + 2 * PART);
+      float* diag = reinterpret_cast<float*>(smem + C::A_OFF);
       float* off32 = diag + 6 * DIAG_BLK;
       float* nowhere = off32 + 32 * OFF_LD + lane * 8;
       // D_ij along the row, from the diagonal to the left, times beta_i in A's
@@ -798,8 +843,8 @@ __global__ void __launch_bounds__(C_THREADS, 1)
           o[e] *= d;
         }
         if (t >= 64) {
-          *reinterpret_cast<uint4*>(tp + 2 * PART + part_at(i, j8)) = take_part8(o);
           *reinterpret_cast<uint4*>(tp + 3 * PART + part_at(i, j8)) = take_part8(o);
+          *reinterpret_cast<uint4*>(tp + 4 * PART + part_at(i, j8)) = take_part8(o);
         } else {
           float* at = warp == 1 && j8 < 32 ? off32 + (i - 32) * OFF_LD + j8
                                            : ((j8 / 16) & 1 ? row_odd : row_even) + (j8 % 16);
@@ -811,27 +856,8 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       mbar_arrive(&bars.g_read);
       named_bar_sync(1, C_PREP);
       if (t < 64) {
-        invert_block16(diag + (t / 16) * DIAG_BLK, tp, t / 16, t % 16);
+        invert_block16(diag + (t / 16) * DIAG_BLK, t % 16);
       } else {
-        // what lies left of the diagonal blocks, in parts
-        {
-          const int r = (t - 64) / 2, c0 = (t % 2) * 16;
-          float x[16];
-          load16(off32 + r * OFF_LD + c0, x);
-#pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            *reinterpret_cast<uint4*>(ap + part * PART + part_at(32 + r, c0)) = take_part8(x);
-            *reinterpret_cast<uint4*>(ap + part * PART + part_at(32 + r, c0 + 8)) = take_part8(x + 8);
-          }
-          const int b = (t - 64) / 32, rb = (t % 32) / 2, cb = (t % 2) * 8;
-          const float* src = diag + (4 + b) * DIAG_BLK + rb * DIAG_LD + cb;
-          const float4 lo = at4(src), hi = at4(src + 4);
-          x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w;
-          x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
-#pragma unroll
-          for (int part = 0; part < 2; ++part)
-            *reinterpret_cast<uint4*>(ap + part * PART + part_at(32 * b + 16 + rb, 32 * b + cb)) = take_part8(x);
-        }
         // c_i (warp 2) and D_63,j (warp 3): products of the decays up to a step
         // and behind it, two steps per lane
         const float2 gg = *reinterpret_cast<const float2*>(gs + 2 * lane);
@@ -867,15 +893,15 @@ __global__ void __launch_bounds__(C_THREADS, 1)
       // The rest of the inverse from its diagonal blocks: blocks of 16, then of
       // 32.  On the register form of the tensor instructions: at these sizes a
       // TMEM round trip would cost more than the products.
-      const uint32_t t_at = smem_u32(tp), a_at = smem_u32(ap);
-      if (warp < 2) join_block<16>(tp, t_at, a_at, 32 * warp + 16, 32 * warp, 0, 0, lane);
+      if (warp < 2)
+        join16(diag, tp, warp, lane);
+      else
+        store_diag_row(diag, tp, (t - 64) / 16, t % 16);
       named_bar_sync(1, C_PREP);
-      join_block<32>(tp, t_at, a_at, 32, 0, (warp / 2) * 16, (warp % 2) * 16, lane);
-      named_bar_sync(1, C_PREP);
-      // T - I goes into the products
-      if (t < 64) *reinterpret_cast<uint16_t*>(tp + part_at(t, t)) = 0;
+      join32(diag, off32, tp, (warp / 2) * 16, (warp % 2) * 16, lane);
       fence_proxy_async_shared();
       mbar_arrive(&bars.tp_full[ts]);
+      named_bar_sync(1, C_PREP);   // before the next A goes over this one's
     }
   } else if (warp < 12) {
     // --------------------------------------------------------- the state rows
@@ -1112,32 +1138,33 @@ __global__ void __launch_bounds__(C_THREADS, 1)
         wait(&bars.s_ready, c);
         tc_fence_after();
 #pragma unroll
-        for (int part = 0; part < 3; ++part)
+        for (int part = 2; part >= 0; --part)
 #pragma unroll
           for (int a = 0; a < DK / 64; ++a)
             mma_bf16_ts_warp_x4<2>(tmem + C::COL_D, tmem + C::COL_S + part * C::S_PART + a * 32,
-                                   make_sw128_desc(kq + a * C::ATOM), ID64, part + a > 0);
+                                   make_sw128_desc(kq + a * C::ATOM), ID64, part < 2 || a > 0);
         tc_commit_warp(&bars.d1_done);
         wait(&bars.tp_full[ts], c / 2);
         wait(&bars.r_ready, c);
         tc_fence_after();
-        // two parts of R with two of T, the third with T's first
-#pragma unroll
-        for (int m = 0; m < 4; ++m)
-          mma_bf16_ts_warp_x4<2>(tmem + C::COL_D, tmem + C::COL_R + (m & 1 ? 32 : 0),
-                                 make_sw128_desc(tp + (m & 2 ? PART : 0)), ID64, m > 0);
+        // two parts of R with two of T, the third ones with the other's first
 #pragma unroll
         for (int k = 0; k < CH / 16; ++k)
-          mma_bf16_ts_warp(tmem + C::COL_D, tmem + C::col_r3(k), make_sw128_desc(tp + k * 32), ID64, 1);
+          mma_bf16_ts_warp(tmem + C::COL_D, tmem + C::col_r3(k), make_sw128_desc(tp + k * 32), ID64, k > 0);
+        mma_bf16_ts_warp_x4<2>(tmem + C::COL_D, tmem + C::COL_R, make_sw128_desc(tp + 2 * PART), ID64, 1);
+#pragma unroll
+        for (int m = 3; m >= 0; --m)
+          mma_bf16_ts_warp_x4<2>(tmem + C::COL_D, tmem + C::COL_R + (m & 1 ? 32 : 0),
+                                 make_sw128_desc(tp + (m & 2 ? PART : 0)), ID64, 1);
         tc_commit_warp(&bars.d3_done);
         wait(&bars.delta_ready, c);
         // [K; Q] K^T of the next chunk has left the second half of these columns
         if (c + 1 < chunks) wait(&bars.g_read, c + 1);
         tc_fence_after();
 #pragma unroll
-        for (int part = 0; part < 3; ++part)
+        for (int part = 2; part >= 0; --part)
           mma_bf16_ts_warp_x4<128>(tmem + C::COL_D, tmem + C::COL_S + part * 32, make_sw128_mn_desc(kq, C::ATOM), IDK,
-                                   part > 0);
+                                   part < 2);
         tc_commit_warp(&bars.d4_done);
       }
     } else if (warp == 14) {
@@ -1164,18 +1191,18 @@ __global__ void __launch_bounds__(C_THREADS, 1)
         if (c > 0) wait(&bars.y_read, c - 1);
         tc_fence_after();
 #pragma unroll
-        for (int part = 0; part < 2; ++part)
+        for (int part = 1; part >= 0; --part)
 #pragma unroll
           for (int a = 0; a < DK / 64; ++a)
             mma_bf16_ts_warp_x4<2>(tmem + C::COL_SQ, tmem + C::COL_S + part * C::S_PART + a * 32,
-                                   make_sw128_desc(kq + 64 * 128 + a * C::ATOM), ID64, part + a > 0);
+                                   make_sw128_desc(kq + 64 * 128 + a * C::ATOM), ID64, part < 1 || a > 0);
         tc_commit_warp(&bars.q_done);
         wait(&bars.delta_ready, c);
         tc_fence_after();
 #pragma unroll
-        for (int m = 0; m < 3; ++m)
+        for (int m = 2; m >= 0; --m)
           mma_bf16_ts_warp_x4<2>(tmem + C::COL_Y, tmem + C::COL_R + (m == 1 ? 32 : 0),
-                                 make_sw128_desc(tp + (m == 2 ? 3 : 2) * PART), ID64, m > 0);
+                                 make_sw128_desc(tp + (m == 2 ? 4 : 3) * PART), ID64, m < 2);
         tc_commit_warp(&bars.y_done);
         tc_commit_warp(&bars.tp_freed[ts]);
       }

@@ -16,6 +16,7 @@ import numpy as np
 import pytest
 import torch
 
+from oracle import bf16 as obf16
 from oracle import gdn as ogdn
 from tests.test_gdn_rule_gpu import _dev, _inputs
 
@@ -121,3 +122,40 @@ def test_outputs_over_inputs_are_refused(pkg, dev):
     want = pkg.gated_delta_rule(*ins)
     y, s = pkg.gated_delta_rule(*ins[:5], s0, out_state=s0)
     assert torch.equal(y, want[0]) and torch.equal(s, want[1])
+
+
+def _alike(arrays, seed, cosine, norm, beta):
+    """The inputs with keys of the given norm and mean cosine to one another."""
+    q, k, v, g, _, s0 = arrays
+    rng = np.random.default_rng(seed)
+    unit = lambda x: x / np.linalg.norm(x, axis=-1, keepdims=True)  # noqa: E731
+    base = unit(rng.standard_normal((1, 1, *k.shape[2:])))
+    mixed = np.sqrt(cosine) * base + np.sqrt(1 - cosine) * unit(rng.standard_normal(k.shape))
+    k = obf16.round_f32((norm * unit(mixed)).astype(np.float32))
+    spread = rng.standard_normal(arrays[4].shape)
+    b = 1 / (1 + np.exp(-spread)) if beta is None else np.full(spread.shape, beta)
+    return q, k, v, g, b.astype(np.float32), s0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cosine", [0.0, 0.3, 0.5, 0.8, 0.95])
+@pytest.mark.parametrize("norm,beta", [(1.0, None), (1.0, 0.98), (0.3, None), (1.3, 1.0)])
+@pytest.mark.parametrize("t,hk,hv,dk,dv", [(520, 1, 3, 128, 128), (300, 2, 2, 64, 96), (1500, 1, 2, 128, 64)])
+def test_keys_that_are_alike(pkg, dev, t, hk, hv, dk, dv, cosine, norm, beta):
+    """The states keep 32-bit accuracy however the keys lie to one another, as long as
+    beta |k|^2 < 2 (a step does not stretch a state): 2^-19 of their 2-norm, times
+    max(1, beta |k|^2)^2.
+
+    T = (I + A)^-1 is joined twice from blocks, each time by two products of
+    32-bit factors in two parts of 11 bits, 2^-22 of a factor left out: 4 x 2^-22 =
+    2^-20 of entries that are at most b = beta |k|^2, from products of three blocks
+    of such entries, b^2 times as large where b is above 1.  It meets R with 24 bits
+    on both sides.  The same again is left for what the recurrence in 32 bits errs
+    itself (sums over Dk, decays; a quarter of 2^-20 for random roundings)."""
+    arrays = _alike(_inputs(64 + t, 1, t, hk, hv, dk, dv, slow=True), t, cosine, norm, beta)
+    y, s = pkg.gated_delta_rule(*_dev(arrays, dev))
+    ry, rs = ogdn.gated_delta_rule(*arrays)
+    bound = 2.0 ** -19 * max(1.0, (beta or 1.0) * norm ** 2) ** 2
+    for h in range(hv):
+        assert np.linalg.norm(_host(s)[:, h] - rs[:, h]) <= bound * np.linalg.norm(rs[:, h])
+    assert _bad_blocks(_host(y), ry) == []
