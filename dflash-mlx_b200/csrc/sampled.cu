@@ -254,7 +254,8 @@ __global__ void __launch_bounds__(THREADS) mask_kernel(const Params p) {
 // ex2, add.  m c is rounded once per maximum, a common factor of all terms that
 // is taken out again at the end.  The quick loop moves the maximum at most
 // once in U vectors; a thread that met NaN or +inf, or nothing above the
-// lowest value, goes over its ids again one by one.  1488 bf16 rows of 248,320
+// lowest value but that, goes over its ids again one by one; one that met only
+// -inf does not.  1488 bf16 rows of 248,320
 // ids (739 MB): 158 us, 72% of the measured copy rate, bound by the issue of
 // its 5 instructions an id beside the loads.
 template <typename T>
@@ -283,14 +284,15 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
   const int head = min(int((16 - (reinterpret_cast<uintptr_t>(x + v0) & 15)) & 15) / int(sizeof(T)), v1 - v0);
   const int vecs = (v1 - v0 - head) / N;
   const int body = v0 + head;
-  Stat a{-FLT_MAX, 0.f, 0x7fffffff};
-  float mc = -FLT_MAX * c;   // may be -inf
+  Stat a{-INFINITY, 0.f, 0x7fffffff};
+  // mc stays above -inf: -inf, and the lowest value where c > 1, add 0 and not NaN
+  float mc = -FLT_MAX;
   float part[U] = {};        // the sum, in parts that do not wait for one another
   auto raise = [&](float top) {
     const float was = mc;
     a.m = top;
-    mc = a.m * c;
-    const float f = was > -INFINITY ? ex2(was - mc) : 0.f;
+    mc = fmaxf(a.m * c, -FLT_MAX);
+    const float f = ex2(was - mc);
     a.s *= f;
 #pragma unroll
     for (int u = 0; u < U; ++u) part[u] *= f;
@@ -361,10 +363,13 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
     }
     a.s += ex2(__fmaf_rn(f, c, -mc));
   }
+  const bool nothing = a.m == -INFINITY && a.s == 0.f;   // only -inf; NaN would be in the sum
   // the rounding of m c comes out of the sum: 2^d to second order
   const float d = float(fma(-double(a.m), double(c), double(mc))) * 0.693147181f;
   a.s = __fmaf_rn(a.s, __fmaf_rn(0.5f * d, d, d), a.s);
-  if (!(a.s > 0.f && fabsf(d) < 1e-3f) || a.id == 0x7fffffff) {
+  if (nothing) {
+    a = Stat{-INFINITY, 0.f, 0x7fffffff};
+  } else if (!(a.s > 0.f && fabsf(d) < 1e-3f) || a.id == 0x7fffffff) {
     a = Stat{-INFINITY, 0.f, 0x7fffffff};
     if (in_head) {
       const int v = v0 + int(threadIdx.x);
