@@ -543,7 +543,7 @@ class MoEPlanLayer:
             raise ValueError(f"router_logits must be {(self.tokens, self.experts)}")
         dense_shared = self.shared_out is not None and not self.shared_stacked
         if self.router is not None:
-            w, ids = self.router(router_logits, self.top_k)
+            w, ids = self.weights, self.ids = self.router(router_logits, self.top_k)
             sort_pairs(ids, x, self.experts, route_out=self.route, x_sorted=self.x_sorted,
                        x_copy=self.x_in if dense_shared else None)
         else:
