@@ -159,3 +159,95 @@ def test_keys_that_are_alike(pkg, dev, t, hk, hv, dk, dv, cosine, norm, beta):
     for h in range(hv):
         assert np.linalg.norm(_host(s)[:, h] - rs[:, h]) <= bound * np.linalg.norm(rs[:, h])
     assert _bad_blocks(_host(y), ry) == []
+
+
+PADDED = [
+    # (b, t, hk, hv, dk, dv, decay per column)
+    (1, 1, 16, 48, 128, 128, False),
+    (2, 3, 1, 2, 64, 32, True),
+    (1, 65, 1, 2, 256, 96, False),
+    (1, 63, 1, 3, 128, 128, False),
+    (3, 129, 2, 4, 64, 64, False),
+    (2, 200, 1, 1, 128, 256, False),
+    (1, 700, 1, 2, 128, 128, False),
+    (2, 1027, 1, 3, 64, 160, False),
+    (1, 1500, 1, 2, 128, 128, False),
+    (1, 3000, 2, 4, 128, 32, False),
+]
+PACKED = [
+    ([64, 1, 63, 0, 65, 130], 2, 2, 128, 128),
+    ([3, 2000, 0, 700, 1], 1, 2, 128, 128),
+    ([64, 2500], 1, 1, 64, 64),
+]
+
+
+def _ranges(lens):
+    ends = np.cumsum([0] + lens)
+    return list(zip(ends[:-1].tolist(), ends[1:].tolist()))
+
+
+def _states_right(s, rs):
+    """Every sequence's and head's state to 2^-19 of its 2-norm (keys of unit length)."""
+    err = np.linalg.norm((s - rs).reshape(*rs.shape[:2], -1), axis=-1)
+    return bool(np.all(err <= 2.0 ** -19 * np.linalg.norm(rs.reshape(*rs.shape[:2], -1), axis=-1)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("slow", [False, True])
+@pytest.mark.parametrize("b,t,hk,hv,dk,dv,vec", PADDED)
+def test_every_block_of_a_padded_batch(pkg, dev, b, t, hk, hv, dk, dv, vec, slow):
+    arrays = _inputs(81 + t, b, t, hk, hv, dk, dv, vec=vec, slow=slow)
+    y, s = pkg.gated_delta_rule(*_dev(arrays, dev))
+    ry, rs = ogdn.gated_delta_rule(*arrays)
+    assert _bad_blocks(_host(y), ry) == [] and _states_right(_host(s), rs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("slow", [False, True])
+@pytest.mark.parametrize("lens,hk,hv,dk,dv", PACKED)
+def test_every_block_of_packed_sequences(pkg, dev, lens, hk, hv, dk, dv, slow):
+    arrays = _inputs(82 + len(lens), 1, sum(lens), hk, hv, dk, dv, n=len(lens), slow=slow)
+    cu = torch.tensor(np.cumsum([0] + lens), dtype=torch.int32, device=dev)
+    y, s = pkg.gated_delta_rule(*_dev(arrays, dev), cu_seqlens=cu)
+    ry, rs = ogdn.gated_delta_rule(*arrays, lens=_ranges(lens))
+    assert _bad_blocks(_host(y), ry, _ranges(lens)) == [] and _states_right(_host(s), rs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,dk,dv", [(40, 128, 128), (300, 64, 64), (1100, 128, 128)])
+def test_every_block_under_a_mask(pkg, dev, t, dk, dv):
+    arrays = _inputs(83 + t, 2, t, 1, 2, dk, dv, slow=True)
+    mask = np.random.default_rng(t).random((2, t)) < 0.6
+    mask[1, : t // 2] = False
+    y, s = pkg.gated_delta_rule(*_dev(arrays, dev), mask=torch.from_numpy(mask).to(dev))
+    ry, rs = ogdn.gated_delta_rule(*arrays, mask=mask)
+    assert _bad_blocks(_host(y), ry) == [] and _states_right(_host(s), rs)
+
+
+@pytest.mark.parametrize("case", PADDED + PACKED)
+@pytest.mark.parametrize("slow", [False, True])
+def test_the_bounds_reject_wrong_results(case, slow):
+    """On the CPU, from the oracle alone: a rounded y passes; y of zeros, scaled by 1% or
+    with one block of one sequence a step late does not, nor does a state off by 1e-5."""
+    if isinstance(case[0], list):
+        lens, hk, hv, dk, dv = case
+        arrays = _inputs(82 + len(lens), 1, sum(lens), hk, hv, dk, dv, n=len(lens), slow=slow)
+        ranges, rows = _ranges(lens), [(0, a, e) for a, e in _ranges(lens) if e > a]
+        ry, rs = ogdn.gated_delta_rule(*arrays, lens=ranges)
+    else:
+        b, t, hk, hv, dk, dv, vec = case
+        arrays = _inputs(81 + t, b, t, hk, hv, dk, dv, vec=vec, slow=slow)
+        ranges, rows = None, [(i, 0, t) for i in range(b)]
+        ry, rs = ogdn.gated_delta_rule(*arrays)
+    rounded = obf16.round_f32(ry.astype(np.float32)).astype(np.float64)
+    assert _bad_blocks(rounded, ry, ranges) == [] and _states_right(rs.astype(np.float32).astype(np.float64), rs)
+    blocks = sum(-(-(e - a) // BLOCK) for _, a, e in rows) * hv
+    assert len(_bad_blocks(np.zeros_like(ry), ry, ranges)) == blocks
+    assert len(_bad_blocks(rounded * 1.01, ry, ranges)) == blocks
+    b, a, e = max(rows, key=lambda r: r[2] - r[1])
+    if e - a > 1:
+        last = a + (e - a - 1) // BLOCK * BLOCK        # the longest sequence's last block
+        wrong = rounded.copy()
+        wrong[b, last + (last == a):e] = rounded[b, last - (last > a):e - 1]
+        assert _bad_blocks(wrong, ry, ranges) != []
+    assert not _states_right(rs * (1 + 1e-5), rs)
