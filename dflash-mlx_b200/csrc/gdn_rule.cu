@@ -251,11 +251,11 @@ int launch_recurrent(const RuleParams& p, cudaStream_t stream) {
 //
 // Bound by the work on a chunk, not by a rate.  The preparing warps take 11000
 // cycles for T and P of the next chunk (decays 3700, blocks of 16 inverted 1700,
-// joined 6000, a third of it for 32-bit factors), and beside them the chain through a
+// joined 5300, a third of it for 32-bit factors), and beside them the chain through a
 // chunk takes 9700: S K^T, R, R T^T, Delta, Delta K and the new state wait for one
 // another.  Most of that is the state's threads at work: 3000 cycles on the last
-// chunk's y, 700 on R, 1000 on Delta, 2500 on beta V, 1800 on the state; they wait
-// 1700 for products, and 1100 to 1600 for T.  A chunk of a 128 x 128 head takes 6.1 us
+// chunk's y, 700 on R, 1000 on Delta, 2100 on beta V, 1500 on the state; they wait
+// 1800 for products, and 1200 to 1600 for T.  A chunk of a 128 x 128 head takes 6.1 us
 // (11200 cycles) with an SM of each pair idle, 6.4 to 7.1 with every SM at work (two
 // share their instruction fetches).  A CTA's start and end take 9 us more.  8192 steps
 // of 48 heads, cut in three, 612 us; 15886 steps in 8 prompts 596 us.
@@ -1261,18 +1261,19 @@ __global__ void __launch_bounds__(C_THREADS, 1)
 }
 
 // Pieces of a sequence (lengths of packed ones are known on the device only:
-// their mean is taken).  In units of a chunk's time (5.4 us): whole, L; in n
-// pieces, two launches of L / n chunks that are 1.25 long with every SM at work,
-// 6 for starting two launches more and 0.6 for a step of the chain.  Measured,
-// us whole and cut: 48 heads 685 / 559 at 8192 steps, 349 / 301 at 4096 (3 pieces;
-// 178 at 2048, left whole), 16 heads 681 / 300 at 8192 and 177 / 105 at 2048 (6), 4
-// heads 676 / 158 and 176 / 86 (16), 8 heads of 64 x 64 621 / 167 and 162 / 72 (10).
+// their mean is taken, so a long one beside many short ones is not cut).  In units
+// of a chunk's time (6.1 us): whole, L; in n pieces, two launches of L / n chunks that
+// are 1.06 long with every SM at work, 6 for starting two launches more and 0.6 for a
+// step of the chain.  Measured, us whole and cut: 48 heads 781 / 601 at 8192 steps, 398 /
+// 329 at 4096 and 204 / 181 at 2048 (3 pieces; 107 / 112 at 1000, left whole), 16 heads
+// 773 / 323 at 8192 and 200 / 112 at 2048 (6), 4 heads 770 / 169 (16) and 199 / 95 (10 or
+// 16), 8 heads of 64 x 64 687 / 180 and 177 / 75 (10).
 inline int pieces(long long heads, int tiles, long long chunks, int sms) {
   int best = 1;
   double least = 0.95 * double(chunks);
   for (int n = 3; n <= MAX_PIECES; ++n) {
     if (heads * (tiles * (n - 1) + n - 2) > sms) break;
-    const double cost = 2.5 * double(chunks) / n + 6.0 + 0.6 * (n - 2);
+    const double cost = 2.12 * double((chunks + n - 1) / n) + 6.0 + 0.6 * (n - 2);
     if (cost < least) {
       least = cost;
       best = n;
