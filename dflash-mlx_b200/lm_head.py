@@ -165,6 +165,8 @@ def verify_accept_sampled(logits: torch.Tensor, verify_ids: torch.Tensor, accept
     single tokens.  ``draft_prob[b, i]`` is ``p_i`` of the draft (0 past
     ``draft_lens``).  A row with nothing to draw from (every id suppressed, -inf
     or NaN) gives ``next_token = -1``.  Nothing is read back to the host.
+    Acceptance goes by 32-bit sums of a row, good to about 1e-7 of ``p``; the id is
+    drawn by 64-bit ones.
     """
     require_cuda(logits, "logits")
     dev = logits.device

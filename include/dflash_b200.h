@@ -338,9 +338,12 @@ int dfl_gdn_forward_tape(const uint16_t* q, const uint16_t* k, const uint16_t* v
  * Constraints: Dk in {32, 64, 128, 256}, Dv % 32 == 0, Hv % Hk == 0.
  * dfl_gdn_rule_recurrent takes one step after the other (fp32 throughout).
  * dfl_gdn_rule_chunked takes 64 steps at a time as products on the tensor
- * cores (same results up to the order of fp32 sums; Dk 64 or 128, one decay
- * per head, keys of about unit length as for any use of the rule; q, k and v
- * 16-byte aligned, ldq, ldk and ldv multiples of 8).  workspace:
+ * cores (Dk 64 or 128, one decay per head, beta |k|^2 < 2 as for any use of the
+ * rule; q, k and v 16-byte aligned, ldq, ldk and ldv multiples of 8).  Its states
+ * differ from the recurrence's by 32-bit roundings (1e-7 to 8e-7 of the 2-norm for
+ * keys of unit length, whatever their angles; up to 2e-6 at |k| = 1.3 and beta = 1
+ * with a mean cosine of 0.95), y before its rounding to bf16 by about 2^-16; a NaN
+ * or an infinity in a step may reach the y of the 63 steps before it.  workspace:
  * dfl_gdn_rule_workspace_bytes bytes (0: none needed), 16-byte aligned, any
  * content, for states between the pieces of few long sequences.
  * The reference reaches this step, for caches that record no tape, through
@@ -454,6 +457,9 @@ int dfl_match_acceptance(const int32_t* drafted, const int32_t* posterior, int B
  * logit of NaN or -inf has probability 0 (what a suppressed id's logit holds
  * does not matter); a row with nothing left gives next_token -1; a draft id
  * outside [0, V) is rejected.  Rows past draft_lens[b] are not read.
+ * Accepting goes by sums of a row in 32 bits, good to about 1e-7 (a u closer than
+ * that to its border, relative to p, may fall on the other side, and draft_prob
+ * is a last bit off); drawing the id by sums in 64 bits.
  *   logits [B, T, V] and draft_logits [B, T - 1, V]: bf16 (dtype 0), fp16 (1)
  *   or fp32 (2), rows ld_* and requests bs_* elements apart; verify_ids int32
  *   [B, T]; accept_u fp32 [B, T - 1] and sample_u fp32 [B], in [0, 1);
